@@ -11,6 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DS_CUDA_LIB") or os.path.join(HERE, "libds_cuda.so")
 
 c_int, c_float, c_size_t, c_void_p, c_uint64 = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_uint64
+c_int64 = ctypes.c_int64
 P = c_void_p  # all pointers are passed as raw addresses
 
 # name -> (restype, argtypes); must match include/ds_cuda.h
@@ -94,6 +95,13 @@ SIGNATURES = {
     "ds_cuda_ep_pairs_dev": (c_int, [P, c_int, c_int, c_int, P, P, c_int, P, P, P, P]),
     "ds_cuda_prefill_timing": (c_int, [P, c_int]),
     "ds_cuda_prefill_stage_ms": (c_int, [P, P]),
+    "ds_cuda_tree_attention_workspace": (c_size_t, [P, P]),
+    "ds_cuda_tree_attention_dev": (c_int, [P, P, P]),
+    "ds_cuda_tree_mask_dev": (c_int, [P, P, P, c_int, c_int, P, P, P]),
+    "ds_cuda_token_probs_dev": (c_int, [P, c_int, P, c_int, c_int, c_int64, P, P, P]),
+    "ds_cuda_tree_verify_dev": (c_int, [P, P, P]),
+    "ds_cuda_tree_verify_greedy_dev": (c_int, [P, P, P, P, P, c_int, c_int, P, P, P, P]),
+    "ds_cuda_tree_commit_dev": (c_int, [P, P, P]),
     "ds_synth_normal_bf16": (None, [P, c_size_t, c_uint64, c_float, c_float]),
     "ds_synth_normal_f32": (None, [P, c_size_t, c_uint64, c_float, c_float]),
     "ds_synth_normal_f32_bf16exact": (None, [P, c_size_t, c_uint64, c_float, c_float]),

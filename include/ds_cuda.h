@@ -535,6 +535,126 @@ int ds_cuda_prefill_timing(ds_cuda_ctx_t *ctx, int enable);
 int ds_cuda_prefill_stage_ms(ds_cuda_ctx_t *ctx, float *ms);
 
 /* ---------------------------------------------------------------------
+ * Speculative decoding (no counterpart in the reference, which decodes one
+ * token a step): several drafted tokens a step for each of `batch`
+ * sequences, arranged as a tree. Node 0 of a tree is the last accepted
+ * token, whose K and V are not cached yet; a node's parent has a smaller
+ * index, and nodes at or past nodes[b] (NULL: n_nodes for every sequence)
+ * are padding. A step attends the whole tree over the cache, turns the
+ * target's logits into probabilities, verifies the drafted tokens and
+ * commits the accepted ones' K and V rows.
+ * Every pointer is device memory except the descriptors themselves, which
+ * are host structs read before the call returns; work is enqueued on
+ * `stream` (NULL = the context's stream; a caller on the legacy default
+ * stream passes cudaStreamLegacy) and nothing is allocated, synchronised or
+ * kept between calls, so calls on several streams may overlap and may be
+ * captured in a CUDA graph. Limits: n_nodes <= 256.
+ * --------------------------------------------------------------------- */
+#define DS_CUDA_SPEC_BF16 0 /* BF16 */
+#define DS_CUDA_SPEC_F16 1  /* FP16 */
+#define DS_CUDA_SPEC_F32 2  /* F32; K and V rows are two BF16 planes (value = plane + lo plane), the decoder's cache form */
+
+/* Attention of the trees' nodes over cache and tree. Node i of sequence b
+ * attends the lens[b] cached rows and the nodes j < nodes[b] whose bit j is
+ * set in its mask words; head h reads K and V head h / (n_heads / n_kv_heads).
+ * out = softmax(scale * q k) v with maximum, sums and products in F32. A row
+ * that attends nothing, and padding, is zeros (its lse -infinity). Rows and
+ * nodes that a query does not attend have no influence, whatever they hold
+ * (NaN and infinities included). lens and nodes are clamped to
+ * [0, kv_max] and [0, n_nodes].
+ * Strides are in elements; the head dimension is contiguous; base addresses
+ * and strides are multiples of 16 bytes. The lo planes share their
+ * tensor's strides and may be NULL (rows exact in BF16). head_dim 64 or 128. */
+typedef struct {
+    int type;                               /* DS_CUDA_SPEC_*: of q and out, and of the cache */
+    int batch, n_nodes, n_heads, n_kv_heads, head_dim;
+    int kv_max;                             /* cached rows that k and v have room for */
+    float scale;
+    const void *q; int64_t q_stride[3];     /* sequence, node, head */
+    const void *k, *k_lo; int64_t k_stride[3];   /* cache: sequence, head, row */
+    const void *v, *v_lo; int64_t v_stride[3];
+    const void *tree_k, *tree_k_lo; int64_t tree_k_stride[3]; /* nodes: sequence, head, node */
+    const void *tree_v, *tree_v_lo; int64_t tree_v_stride[3];
+    const int *lens;                        /* [batch] */
+    const int *nodes;                       /* [batch] or NULL */
+    const uint64_t *mask;                   /* [batch x n_nodes x ceil(n_nodes / 64)] */
+    void *out; int64_t out_stride[3];       /* sequence, node, head */
+    float *lse;                             /* optional [batch x n_nodes x n_heads]: log of the sum of exp(scale q k) */
+    void *workspace; size_t workspace_bytes; /* 256-byte aligned; not shared by calls that may overlap */
+} ds_cuda_tree_attention_t;
+/* Bytes of workspace a call with these sizes needs (pointers not read); 0
+ * also where the sizes are refused. */
+size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *ctx, const ds_cuda_tree_attention_t *d);
+int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *ctx, const ds_cuda_tree_attention_t *d, void *stream);
+
+/* Mask words and depths (root 0) of trees given by parents
+ * [batch x n_nodes] (a root's is -1): node i attends itself and its
+ * ancestors. A parent outside [0, i) makes its node a root; padding gets
+ * empty words and depth 0. */
+int ds_cuda_tree_mask_dev(ds_cuda_ctx_t *ctx, const int *parents, const int *nodes, int batch, int n_nodes,
+                          uint64_t *mask, int *depth, void *stream);
+
+/* probs[r] = softmax(logits[r] / temperature[r]) in F32 for `rows` rows of
+ * `vocab` logits of a DS_CUDA_SPEC_* type, row_stride elements apart; probs
+ * is [rows x vocab]. temperature [rows] or NULL (1). A temperature <= 0
+ * gives 1 at the row's largest logit (the lowest index wins ties). -infinity
+ * is probability 0, a row of nothing else is zeros, a NaN or +infinity
+ * makes its row NaN. */
+int ds_cuda_token_probs_dev(ds_cuda_ctx_t *ctx, int type, const void *logits, int rows, int vocab, int64_t row_stride,
+                            const float *temperature, float *probs, void *stream);
+
+/* Verification of drafted tokens by speculative sampling over a tree. From
+ * the root, the current node p's children are tried in index order: the
+ * child c with token x is accepted if
+ *     accept_u[c] * (draft_p(x) * mass) < r(x),
+ * with r = target_p and mass = 1 at first, and becomes the current node;
+ * otherwise r <- max(r - mass * draft_p, 0) and mass <- the sum of r. When
+ * no child is left, the next token is drawn from r: the first index whose
+ * cumulative sum exceeds sample_u * (sum of r); should r have no mass, from
+ * target_p; -1 if that has none either. draft NULL: a drafted token is
+ * certain (draft_p(x) = 1 for that token alone), as with n-gram drafts.
+ * Products and differences are single F32 operations; sums are taken in
+ * whole multiples of 2^-44 (values clamped to [0, 1], NaN counts as 0), so
+ * the result depends on no order of summation; sample_u counts in steps of
+ * 2^-24. A drafted token outside [0, vocab) is rejected.
+ * path [batch x n_nodes]: node indices of the accepted path from 0, then -1;
+ * accepted [batch]: drafted tokens accepted (path length - 1); token [batch].
+ * Limits: vocab <= 2^18. */
+typedef struct {
+    int batch, n_nodes, vocab;
+    const int *tokens, *parents, *nodes;    /* [batch x n_nodes], [batch x n_nodes], [batch] or NULL */
+    const float *target; int64_t target_stride[2]; /* [batch][node][vocab]: sequence, node strides */
+    const float *draft; int64_t draft_stride[2];   /* row p: what p's children were drawn from; or NULL */
+    const float *accept_u;                  /* [batch x n_nodes] in [0, 1) */
+    const float *sample_u;                  /* [batch] in [0, 1) */
+    int *path, *accepted, *token;
+} ds_cuda_tree_verify_t;
+int ds_cuda_tree_verify_dev(ds_cuda_ctx_t *ctx, const ds_cuda_tree_verify_t *d, void *stream);
+/* The greedy rule: target_tokens [batch x n_nodes] are the target's argmax
+ * after each node; a child (the first in index order) is accepted if its
+ * token is its parent's target token; token = the last accepted node's. */
+int ds_cuda_tree_verify_greedy_dev(ds_cuda_ctx_t *ctx, const int *tokens, const int *parents, const int *nodes,
+                                   const int *target_tokens, int batch, int n_nodes, int *path, int *accepted,
+                                   int *token, void *stream);
+
+/* Accepted rows into the cache, every layer and plane in one launch:
+ *     cache[l][b][h][lens[b] + j] = tree[l][b][h][path[b][j]], j = 0 .. accepted[b],
+ * and new_lens[b] = lens[b] + accepted[b] + 1 (both stop at kv_max: rows
+ * past it are not written). n_tensors (<= 8) pairs of cache and tree
+ * tensors of 16-bit elements (K and V, or their planes); strides in
+ * elements: layer, sequence, head, row (node). Base addresses and strides
+ * are multiples of 16 bytes, head_dim a multiple of 8. The trees must not
+ * overlap the caches, nor new_lens lens. */
+typedef struct {
+    int n_tensors, layers, batch, n_nodes, n_kv_heads, head_dim, kv_max;
+    void *cache[8]; int64_t cache_stride[8][4];
+    const void *tree[8]; int64_t tree_stride[8][4];
+    const int *lens, *path, *accepted;      /* [batch], [batch x n_nodes], [batch] */
+    int *new_lens;                          /* [batch] */
+} ds_cuda_tree_commit_t;
+int ds_cuda_tree_commit_dev(ds_cuda_ctx_t *ctx, const ds_cuda_tree_commit_t *d, void *stream);
+
+/* ---------------------------------------------------------------------
  * Host-side synthetic data (seeded, counter-based: value i of a stream
  * depends only on (seed, i)); used to build the benchmark workloads.
  * normal_bf16: RNE-rounded N(mean, std); normal_f32: F32 N(mean, std);
