@@ -1,7 +1,19 @@
 // spec_attn.cu — attention of a tree of drafted tokens over the KV cache
 // (ds_cuda_tree_attention_dev), and the trees' mask words.
+//
+// The R = n_nodes * group query rows that share a key head are taken
+// together, so K and V are read once for all of them. The keys of a
+// (sequence, key head, row tile) item come in tiles of KT: first the cached
+// rows, then the tree's nodes. All items' tiles form one list, cut into equal
+// runs, one per CTA (one persistent CTA per SM, two for head_dim 64): a
+// ragged batch and a single long sequence are spread alike, and nothing
+// about the lengths is needed on the host. A run that covers an item writes
+// its result; an item cut between CTAs leaves (max, sum, weighted V) parts
+// in the workspace, joined by sa_join_kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "ctx.h"
@@ -9,97 +21,697 @@
 namespace ds {
 
 constexpr int SA_MAX_NODES = 256;
+constexpr int SA_THREADS = 256;
+constexpr int SA_WARPS = SA_THREADS / 32;
+constexpr int SA_STAGES = 3;
 
 struct SaArgs {
     ds_cuda_tree_attention_t d;
-    int words;  // mask words per node
+    int words;      // mask words per node
+    int group;      // query heads per key head
+    int rows;       // n_nodes * group
+    int row_tiles;  // ceil(rows / row tile)
+    int ctas;       // runs the tile list is cut into, at most
+    float scale2;   // scale * log2(e)
+    float *part;    // workspace: [ctas][2][row tile][head_dim], then ...
+    float2 *ml;     // ... [ctas][2][row tile] (max in log2 units, sum)
 };
 
-__device__ __forceinline__ float sa_load(const void *p, int64_t i, int type) {
-    if (type == DS_CUDA_SPEC_F16) return __half2float(reinterpret_cast<const __half *>(p)[i]);
-    return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
+// ---- the tile list ---------------------------------------------------------
+struct SaSeq {
+    int len, cnt, cache_tiles, tiles;
+};
+template <int KT>
+__device__ __forceinline__ SaSeq sa_seq(const ds_cuda_tree_attention_t &d, int b) {
+    SaSeq s;
+    s.cnt = d.nodes ? min(max(d.nodes[b], 0), d.n_nodes) : d.n_nodes;
+    s.len = s.cnt ? min(max(d.lens[b], 0), d.kv_max) : 0;  // no rows: one empty tile, whose results are zeros
+    s.cache_tiles = (s.len + KT - 1) / KT;
+    s.tiles = max(1, s.cache_tiles + (s.cnt + KT - 1) / KT);
+    return s;
+}
+// Sums the sequences' tiles over the batch: returns the total, *mine the
+// tiles before this thread's run of sequences [b0, b1).
+template <int KT>
+__device__ __forceinline__ long long sa_scan(const SaArgs &a, int b0, int b1, long long *sh, long long *mine) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = a.d.n_kv_heads * a.row_tiles;
+    long long s = 0;
+    for (int b = b0; b < b1; b++) s += (long long)sa_seq<KT>(a.d, b).tiles * per;
+    long long v = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(DS_FULL, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) sh[warp] = v;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; w++) {
+        if (w < warp) before += sh[w];
+        total += sh[w];
+    }
+    *mine = before + v - s;
+    return total;
+}
+__device__ __forceinline__ long long sa_start(long long c, long long total, long long ctas) { return c * total / ctas; }
+__device__ __forceinline__ int sa_cta_of(long long x, long long total, long long ctas) {
+    return (int)(((x + 1) * ctas - 1) / total);
 }
 
-// One CTA per (node, head, sequence): four warps take the keys in turn, each
-// lane HD / 32 dimensions, with a running maximum and sum per warp; the
-// warps' parts are joined at the end.
-template <int HD>
-__global__ void __launch_bounds__(128) sa_rows_kernel(const __grid_constant__ SaArgs a) {
-    constexpr int PL = HD / 32;
+// ---- loads and matrix instructions -----------------------------------------
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 8 keys at a time (BF16).
+__device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5},{%6},{%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b0));
+}
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float x, float y) {
+    uint32_t r;
+    if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+// Two values as three BF16 planes each: 24 bits, the value itself.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&p)[3]) {
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        p[k] = pack2<false>(x, y);
+        x = __fsub_rn(x, __uint_as_float(p[k] << 16));
+        y = __fsub_rn(y, __uint_as_float(p[k] & 0xffff0000u));
+    }
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Byte offset of 16-byte chunk c of row r in a [rows][HD] 16-bit tile: the
+// chunk is xor-ed with the row, so that ldmatrix's 8 rows meet 8 bank groups.
+template <int HD> __device__ __forceinline__ uint32_t sw(int r, int c) { return (uint32_t)(r * HD * 2 + ((c ^ (r & 7)) << 4)); }
+
+// Result or part of one row's dimensions [x, x + 4).
+__device__ __forceinline__ void sa_store4(const ds_cuda_tree_attention_t &d, int64_t o, const float (&v)[4]) {
+    if (d.type == DS_CUDA_SPEC_F32)
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(d.out) + o) = make_float4(v[0], v[1], v[2], v[3]);
+    else if (d.type == DS_CUDA_SPEC_F16)
+        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(d.out) + o) =
+            make_uint2(pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3]));
+    else
+        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(d.out) + o) =
+            make_uint2(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]));
+}
+
+// Shapes of one instantiation. QP planes of the queries and of the weights
+// (F32: three, all 24 bits; 16-bit types: one), PL planes of K and V. Eight
+// warps: MT row tiles of 16 times KS slices of KW keys.
+template <int HD_, int MT_, int PL_, int QT_> struct SaShape {
+    static constexpr int HD = HD_, MT = MT_, PL = PL_, QT = QT_;
+    static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
+    static constexpr int RT = 16 * MT;
+    static constexpr int KT = PL == 2 ? 64 : 128;  // a stage is 64 KB (32 KB for head_dim 64) either way
+    static constexpr int KS = SA_WARPS / MT, KW = KT / KS, NT = KW / 8;
+    static constexpr int PLANE = KT * HD * 2, STAGE = 2 * PL * PLANE;
+    static constexpr int QPLANE = RT * HD * 2;
+    static constexpr int SMEM = SA_STAGES * STAGE + QP * QPLANE;
+    static constexpr int MINB = HD == 64 ? 2 : 1;
+};
+
+template <class S>
+__global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_constant__ SaArgs a) {
+    constexpr int HD = S::HD, KT = S::KT, NT = S::NT, KW = S::KW, CH = HD / 8;
+    constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16, F32 = S::QT == DS_CUDA_SPEC_F32;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ long long sh_scan[SA_WARPS];
+    __shared__ long long sh_off;
+    __shared__ int sh_b;
+    __shared__ float2 sh_ml[SA_WARPS][16];
+    __shared__ uint64_t sh_mask[2][S::RT][KT / 64];  // by tile parity
     const ds_cuda_tree_attention_t &d = a.d;
-    const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = h / (d.n_heads / d.n_kv_heads);
-    const int len = min(max(d.lens[b], 0), d.kv_max);
-    const int cnt = d.nodes ? min(max(d.nodes[b], 0), d.n_nodes) : d.n_nodes;
-    const int total = i < cnt ? len + cnt : 0;
-    const uint64_t *mask = d.mask + ((size_t)b * d.n_nodes + i) * a.words;
-    const int64_t qo = b * d.q_stride[0] + i * d.q_stride[1] + h * d.q_stride[2] + lane * PL;
-    float q[PL], o[PL], m = -__FLT_MAX__, l = 0.f;
-#pragma unroll
-    for (int c = 0; c < PL; c++) {
-        q[c] = d.type == DS_CUDA_SPEC_F32 ? reinterpret_cast<const float *>(d.q)[qo + c] : sa_load(d.q, qo + c, d.type);
-        q[c] *= d.scale;
-        o[c] = 0.f;
-    }
-    for (int j = warp; j < total; j += 4) {
-        const bool node = j >= len;
-        const int t = j - len;
-        if (node && !((mask[t >> 6] >> (t & 63)) & 1)) continue;
-        const void *kp = node ? d.tree_k : d.k, *kl = node ? d.tree_k_lo : d.k_lo;
-        const void *vp = node ? d.tree_v : d.v, *vl = node ? d.tree_v_lo : d.v_lo;
-        const int64_t *ks = node ? d.tree_k_stride : d.k_stride, *vs = node ? d.tree_v_stride : d.v_stride;
-        const int64_t row = node ? t : j;
-        const int64_t ko = b * ks[0] + g * ks[1] + row * ks[2] + lane * PL;
-        const int64_t vo = b * vs[0] + g * vs[1] + row * vs[2] + lane * PL;
-        float s = 0.f;
-#pragma unroll
-        for (int c = 0; c < PL; c++) {
-            float k = sa_load(kp, ko + c, d.type);
-            if (d.type == DS_CUDA_SPEC_F32 && kl) k += sa_load(kl, ko + c, d.type);
-            s += q[c] * k;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int mt = warp % S::MT, ks = warp / S::MT;
+    const uint32_t q_s = smem_u32(smem) + SA_STAGES * S::STAGE;
+    pdl_launch();
+
+    // this CTA's run of the tile list
+    const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
+    const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
+    long long at;
+    const long long total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
+    const long long ctas = min((long long)a.ctas, total);
+    if (blockIdx.x >= ctas) return;
+    const long long first = sa_start(blockIdx.x, total, ctas), last = sa_start(blockIdx.x + 1, total, ctas);
+    for (int b = b0; b < b1; b++) {
+        const long long n = (long long)sa_seq<KT>(d, b).tiles * d.n_kv_heads * a.row_tiles;
+        if (at <= first && first < at + n) {
+            sh_b = b;
+            sh_off = first - at;
         }
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s), f = expf(m - mn), p = expf(s - mn);
-        l = l * f + p;
-        m = mn;
-#pragma unroll
-        for (int c = 0; c < PL; c++) {
-            float v = sa_load(vp, vo + c, d.type);
-            if (d.type == DS_CUDA_SPEC_F32 && vl) v += sa_load(vl, vo + c, d.type);
-            o[c] = o[c] * f + p * v;
-        }
+        at += n;
     }
-    __shared__ float sm[4], sl[4], so[4][HD];
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
-#pragma unroll
-    for (int c = 0; c < PL; c++) so[warp][lane * PL + c] = o[c];
     __syncthreads();
-    if (warp) return;
-    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    l = 0.f;
-#pragma unroll
-    for (int c = 0; c < PL; c++) o[c] = 0.f;
-    for (int w = 0; w < 4; w++) {
-        const float f = expf(sm[w] - m);
-        l += sl[w] * f;
-#pragma unroll
-        for (int c = 0; c < PL; c++) o[c] += so[w][lane * PL + c] * f;
+
+    struct Cursor {
+        int b, g, rt, t;
+        SaSeq s;
+    } ld, cu;
+    {
+        ld.b = sh_b;
+        ld.s = sa_seq<KT>(d, ld.b);
+        const int off = (int)(sh_off / ld.s.tiles);
+        ld.t = (int)(sh_off % ld.s.tiles);
+        ld.rt = off % a.row_tiles;
+        ld.g = off / a.row_tiles;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int64_t oo = b * d.out_stride[0] + i * d.out_stride[1] + h * d.out_stride[2] + lane * PL;
+    cu = ld;
+    auto next = [&](Cursor &c) {
+        if (++c.t < c.s.tiles) return;
+        c.t = 0;
+        if (++c.rt < a.row_tiles) return;
+        c.rt = 0;
+        if (++c.g < d.n_kv_heads) return;
+        c.g = 0;
+        if (++c.b < d.batch) c.s = sa_seq<KT>(d, c.b);
+    };
+    // the rows of tile c into stage st; rows past the valid ones are zeros
+    auto load = [&](const Cursor &c, int st) {
+        const bool node = c.t >= c.s.cache_tiles;
+        const int r0 = (node ? c.t - c.s.cache_tiles : c.t) * KT;
+        const int valid = (node ? c.s.cnt : c.s.len) - r0;
+        const void *base[4];
+        int64_t step[2];
+        {
+            const int64_t *s = node ? d.tree_k_stride : d.k_stride;
+            const int64_t o = c.b * s[0] + c.g * s[1] + (int64_t)r0 * s[2];
+            base[0] = (const uint16_t *)(node ? d.tree_k : d.k) + o;
+            base[1] = (const uint16_t *)(node ? d.tree_k_lo : d.k_lo) + o;
+            step[0] = s[2];
+        }
+        {
+            const int64_t *s = node ? d.tree_v_stride : d.v_stride;
+            const int64_t o = c.b * s[0] + c.g * s[1] + (int64_t)r0 * s[2];
+            base[2] = (const uint16_t *)(node ? d.tree_v : d.v) + o;
+            base[3] = (const uint16_t *)(node ? d.tree_v_lo : d.v_lo) + o;
+            step[1] = s[2];
+        }
+        const bool lo[2] = {(node ? d.tree_k_lo : d.k_lo) != nullptr, (node ? d.tree_v_lo : d.v_lo) != nullptr};
+        const uint32_t dst = smem_u32(smem) + st * S::STAGE;
+        const int cc = tid % CH, rr = tid / CH;
 #pragma unroll
-    for (int c = 0; c < PL; c++) {
-        const float x = l == 0.f ? 0.f : o[c] * inv;
-        if (d.type == DS_CUDA_SPEC_F32) reinterpret_cast<float *>(d.out)[oo + c] = x;
-        else if (d.type == DS_CUDA_SPEC_F16) reinterpret_cast<__half *>(d.out)[oo + c] = __float2half_rn(x);
-        else reinterpret_cast<__nv_bfloat16 *>(d.out)[oo + c] = __float2bfloat16_rn(x);
+        for (int kv = 0; kv < 2; kv++)
+#pragma unroll
+            for (int p = 0; p < S::PL; p++)
+#pragma unroll
+                for (int x = 0; x < KT / (SA_THREADS / CH); x++) {
+                    const int r = rr + x * (SA_THREADS / CH);
+                    const bool ok = r < valid && (p == 0 || lo[kv]);
+                    cp16(dst + (kv * S::PL + p) * S::PLANE + sw<HD>(r, cc),
+                         ok ? (const uint16_t *)base[2 * kv + p] + r * step[kv] + 8 * cc : d.q, ok);
+                }
+    };
+
+    const long long tiles = last - first;
+#pragma unroll
+    for (int i = 0; i < SA_STAGES - 1; i++) {
+        if (i < tiles) {
+            load(ld, i);
+            next(ld);
+        }
+        cp_commit();
+    }
+
+    float o[CH][4], m[2], l[2];
+    bool fresh = true;          // the item's queries are not in shared memory yet
+    bool whole = cu.t == 0;     // this CTA has the item from its first tile
+    int st = 0, fill = SA_STAGES - 1;
+    for (long long i = 0; i < tiles; i++) {
+        cp_wait<SA_STAGES - 2>();
+        if (fresh) {  // (the previous item's readers of these are past the last barrier of its end)
+            fresh = false;
+            for (int x = tid; x < S::RT * CH; x += SA_THREADS) {
+                const int r = x / CH, c = x % CH, row = cu.rt * S::RT + r;
+                const bool ok = row < a.rows;
+                const int64_t qo = ok ? cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
+                                            (cu.g * a.group + row % a.group) * d.q_stride[2] + 8 * c : 0;
+                if (F32) {
+                    float4 u = make_float4(0, 0, 0, 0), v = u;
+                    if (ok) {
+                        u = *reinterpret_cast<const float4 *>((const float *)d.q + qo);
+                        v = *reinterpret_cast<const float4 *>((const float *)d.q + qo + 4);
+                    }
+                    uint32_t p[4][3];
+                    split3(u.x, u.y, p[0]);
+                    split3(u.z, u.w, p[1]);
+                    split3(v.x, v.y, p[2]);
+                    split3(v.z, v.w, p[3]);
+#pragma unroll
+                    for (int k = 0; k < S::QP; k++)
+                        *reinterpret_cast<uint4 *>(smem + SA_STAGES * S::STAGE + k * S::QPLANE + sw<HD>(r, c)) =
+                            make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+                } else {
+                    uint4 u = make_uint4(0, 0, 0, 0);
+                    if (ok) u = *reinterpret_cast<const uint4 *>((const uint16_t *)d.q + qo);
+                    *reinterpret_cast<uint4 *>(smem + SA_STAGES * S::STAGE + sw<HD>(r, c)) = u;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < CH; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+            m[0] = m[1] = -__FLT_MAX__;
+            l[0] = l[1] = 0.f;
+        }
+        const bool node = cu.t >= cu.s.cache_tiles;
+        const int r0 = (node ? cu.t - cu.s.cache_tiles : cu.t) * KT;
+        const int valid = (node ? cu.s.cnt : cu.s.len) - r0;
+        if (node)
+            for (int x = tid; x < S::RT * (KT / 64); x += SA_THREADS) {
+                const int r = x / (KT / 64), w = x % (KT / 64), row = cu.rt * S::RT + r, nd = row / a.group;
+                const int word = r0 / 64 + w, left = cu.s.cnt - 64 * word;
+                uint64_t bits = 0;
+                if (row < a.rows && nd < cu.s.cnt && left > 0)
+                    bits = d.mask[((size_t)cu.b * d.n_nodes + nd) * a.words + word] &
+                           (left < 64 ? (1ull << left) - 1 : ~0ull);
+                sh_mask[i & 1][r][w] = bits;
+            }
+        __syncthreads();
+        if (i + SA_STAGES - 1 < tiles) {
+            load(ld, fill);
+            next(ld);
+        }
+        cp_commit();
+        fill = fill + 1 == SA_STAGES ? 0 : fill + 1;
+
+        const uint32_t k_s = smem_u32(smem) + st * S::STAGE, v_s = k_s + S::PL * S::PLANE;
+        // scores of 16 rows and KW keys; the products of lower planes apart
+        float s[NT][4], s2[F32 ? NT : 1][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[n][e] = 0.f;
+                if (F32) s2[n][e] = 0.f;
+            }
+        const int qr = 16 * mt + (lane & 15), qc = lane >> 4;
+        if (NT == 1) {
+            const int kr = ks * KW + (lane & 7), kc = lane >> 3;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk += 2) {
+                uint32_t qf[2][S::QP][4], kf[S::PL][4];
+#pragma unroll
+                for (int p = 0; p < S::PL; p++) ldsm4(kf[p], k_s + p * S::PLANE + sw<HD>(kr, 2 * kk + kc));
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+#pragma unroll
+                    for (int p = 0; p < S::QP; p++) ldsm4(qf[h][p], q_s + p * S::QPLANE + sw<HD>(qr, 2 * kk + 2 * h + qc));
+#pragma unroll
+                    for (int pq = 0; pq < S::QP; pq++)
+#pragma unroll
+                        for (int pk = 0; pk < S::PL; pk++)
+                            if (pq + pk < 3)
+                                mma16<F16>(pq + pk ? s2[0] : s[0], qf[h][pq], kf[pk][2 * h], kf[pk][2 * h + 1]);
+                }
+            }
+        } else {
+            const int kr = ks * KW + (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk++) {
+                uint32_t qf[S::QP][4];
+#pragma unroll
+                for (int p = 0; p < S::QP; p++) ldsm4(qf[p], q_s + p * S::QPLANE + sw<HD>(qr, 2 * kk + qc));
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+#pragma unroll
+                    for (int pk = 0; pk < S::PL; pk++) {
+                        uint32_t kf[4];
+                        ldsm4(kf, k_s + pk * S::PLANE + sw<HD>(kr + 8 * n, 2 * kk + kc));
+#pragma unroll
+                        for (int pq = 0; pq < S::QP; pq++)
+                            if (pq + pk < 3) {
+                                mma16<F16>(pq + pk ? s2[F32 ? n : 0] : s[n], qf[pq], kf[0], kf[1]);
+                                mma16<F16>(pq + pk ? s2[F32 ? n + 1 : 0] : s[n + 1], qf[pq], kf[2], kf[3]);
+                            }
+                    }
+                }
+            }
+        }
+        if (F32)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[n][e] += s2[n][e];
+
+        // running maximum (of the scaled scores, in log2 units), weights, sums
+        const bool masked = node || valid < KT;
+        uint64_t see[2] = {~0ull, ~0ull};
+        if (masked) {
+            const int key = ks * KW;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (node) see[h] = sh_mask[i & 1][16 * mt + (lane >> 2) + 8 * h][key >> 6] >> (key & 63);
+                else see[h] = valid - key >= 64 ? ~0ull : valid > key ? (1ull << (valid - key)) - 1 : 0;
+            }
+        }
+        float mx[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (!masked || ((see[e >> 1] >> (8 * n + 2 * (lane & 3) + (e & 1))) & 1))
+                    mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e] * a.scale2);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(DS_FULL, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(DS_FULL, mx[h], 2));
+        }
+        if (__any_sync(DS_FULL, mx[0] > m[0] || mx[1] > m[1])) {
+            const float f0 = ex2(m[0] - mx[0]), f1 = ex2(m[1] - mx[1]);
+            l[0] *= f0;
+            l[1] *= f1;
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                o[c][0] *= f0;
+                o[c][1] *= f0;
+                o[c][2] *= f1;
+                o[c][3] *= f1;
+            }
+            m[0] = mx[0];
+            m[1] = mx[1];
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool ok = !masked || ((see[e >> 1] >> (8 * n + 2 * (lane & 3) + (e & 1))) & 1);
+                s[n][e] = ok ? ex2(__fmaf_rn(s[n][e], a.scale2, -m[e >> 1])) : 0.f;
+                l[e >> 1] += s[n][e];
+            }
+
+        if (node) {
+            // A node's V may hold NaN or infinities that some rows must not
+            // see, and 0 * NaN would spread through the product: such values
+            // are added here to the rows that attend them, then zeroed.
+            bool bad = false;
+            for (int x = tid; x < KT * CH; x += SA_THREADS) {
+                const uint32_t off = sw<HD>(x / CH, x % CH);
+#pragma unroll
+                for (int p = 0; p < S::PL; p++) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(smem + st * S::STAGE + (S::PL + p) * S::PLANE + off);
+                    constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t e = ((&u.x)[k] & E) ^ E;
+                        bad |= !(e & 0xffffu) || !(e >> 16);
+                    }
+                }
+            }
+            if (__syncthreads_or(bad)) {
+                for (int kk = 0; kk < KW; kk++) {
+                    const int key = ks * KW + kk;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int r = 16 * mt + (lane >> 2) + 8 * h;
+                        if (!((sh_mask[i & 1][r][key >> 6] >> (key & 63)) & 1)) continue;
+#pragma unroll
+                        for (int c = 0; c < CH; c++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                float v = 0.f;
+#pragma unroll
+                                for (int p = 0; p < S::PL; p++) {
+                                    const uint16_t w = *reinterpret_cast<const uint16_t *>(
+                                        smem + st * S::STAGE + (S::PL + p) * S::PLANE + sw<HD>(key, c) + 2 * (2 * (lane & 3) + e));
+                                    v += F16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
+                                }
+                                if (!isfinite(v)) o[c][2 * h + e] += v;
+                            }
+                    }
+                }
+                __syncthreads();
+                for (int x = tid; x < KT * HD; x += SA_THREADS) {
+                    const uint32_t off = sw<HD>(x / HD, x % HD / 8) + 2 * (x % 8);
+                    bool nf = false;
+#pragma unroll
+                    for (int p = 0; p < S::PL; p++) {
+                        const uint16_t w = *reinterpret_cast<uint16_t *>(smem + st * S::STAGE + (S::PL + p) * S::PLANE + off);
+                        nf |= (w & (F16 ? 0x7c00 : 0x7f80)) == (F16 ? 0x7c00 : 0x7f80);
+                    }
+                    if (nf)
+#pragma unroll
+                        for (int p = 0; p < S::PL; p++)
+                            *reinterpret_cast<uint16_t *>(smem + st * S::STAGE + (S::PL + p) * S::PLANE + off) = 0;
+                }
+                __syncthreads();
+            }
+        }
+
+        // O += P V
+        if (NT == 1) {
+            uint32_t p0[3], p1[3];
+            split3(s[0][0], s[0][1], p0);
+            split3(s[0][2], s[0][3], p1);
+            const int vr = ks * KW + (lane & 7), vc = lane >> 3;
+#pragma unroll
+            for (int c = 0; c < CH; c += 4) {
+                uint32_t vf[S::PL][4];
+#pragma unroll
+                for (int p = 0; p < S::PL; p++) ldsm4t(vf[p], v_s + p * S::PLANE + sw<HD>(vr, c + vc));
+#pragma unroll
+                for (int pq = 0; pq < S::QP; pq++)
+#pragma unroll
+                    for (int pk = 0; pk < S::PL; pk++)
+                        if (pq + pk < 3)
+#pragma unroll
+                            for (int x = 0; x < 4; x++) mma8(o[c + x], p0[pq], p1[pq], vf[pk][x]);
+            }
+        } else {
+            const int vr = ks * KW + (lane & 15), vc = lane >> 4;
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t pf[S::QP][4];
+                if (F32) {
+                    uint32_t t[3];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        split3(s[n + (x >> 1)][2 * (x & 1)], s[n + (x >> 1)][2 * (x & 1) + 1], t);
+#pragma unroll
+                        for (int p = 0; p < S::QP; p++) pf[p][x] = t[p];
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        pf[0][x] = pack2<F16>(s[n + (x >> 1)][2 * (x & 1)], s[n + (x >> 1)][2 * (x & 1) + 1]);
+                }
+#pragma unroll
+                for (int c = 0; c < CH; c += 2) {
+#pragma unroll
+                    for (int pk = 0; pk < S::PL; pk++) {
+                        uint32_t vf[4];
+                        ldsm4t(vf, v_s + pk * S::PLANE + sw<HD>(vr + 8 * n, c + vc));
+#pragma unroll
+                        for (int pq = 0; pq < S::QP; pq++)
+                            if (pq + pk < 3) {
+                                mma16<F16>(o[c], pf[pq], vf[0], vf[1]);
+                                mma16<F16>(o[c + 1], pf[pq], vf[2], vf[3]);
+                            }
+                    }
+                }
+            }
+        }
+
+        const bool end = cu.t + 1 == cu.s.tiles;
+        if (end || i + 1 == tiles) {
+            // the item, or this CTA's part of it, is done: the warps' parts
+            // are joined through this stage, which is free until the next
+            // iteration's barrier
+            __syncthreads();
+            float *so = reinterpret_cast<float *>(smem + st * S::STAGE) + warp * 16 * HD;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                l[h] += __shfl_xor_sync(DS_FULL, l[h], 1);
+                l[h] += __shfl_xor_sync(DS_FULL, l[h], 2);
+                if ((lane & 3) == 0) sh_ml[warp][(lane >> 2) + 8 * h] = make_float2(m[h], l[h]);
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    const int r = (lane >> 2) + 8 * h, x = 8 * c + 2 * (lane & 3);
+                    *reinterpret_cast<float2 *>(so + r * HD + (x ^ ((r & 3) << 3))) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
+                }
+            }
+            __syncthreads();
+            const bool alone = end && whole;
+            const int slot = whole ? 1 : 0;
+            for (int x = tid; x < S::RT * (HD / 4); x += SA_THREADS) {
+                const int r = x / (HD / 4), c = 4 * (x % (HD / 4)), t16 = r >> 4, rr = r & 15;
+                float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < S::KS; w++) mm = fmaxf(mm, sh_ml[w * S::MT + t16][rr].x);
+#pragma unroll
+                for (int w = 0; w < S::KS; w++) {
+                    const float2 ml = sh_ml[w * S::MT + t16][rr];
+                    const float f = ex2(ml.x - mm);
+                    const float4 u = *reinterpret_cast<const float4 *>(
+                        reinterpret_cast<const float *>(smem + st * S::STAGE) + (w * S::MT + t16) * 16 * HD + rr * HD +
+                        (c ^ ((rr & 3) << 3)));
+                    ll += ml.y * f;
+                    v[0] += u.x * f;
+                    v[1] += u.y * f;
+                    v[2] += u.z * f;
+                    v[3] += u.w * f;
+                }
+                const int row = cu.rt * S::RT + r;
+                if (row >= a.rows) continue;
+                if (alone) {
+                    const int nd = row / a.group, head = cu.g * a.group + row % a.group;
+                    const bool none = nd >= cu.s.cnt || ll == 0.f;
+                    const float inv = 1.f / ll;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) v[k] = none ? 0.f : v[k] * inv;
+                    sa_store4(d, cu.b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c, v);
+                    if (d.lse && c == 0)
+                        d.lse[((size_t)cu.b * d.n_nodes + nd) * d.n_heads + head] =
+                            none ? -INFINITY : (mm + log2f(ll)) * 0.69314718f;
+                } else {
+                    const size_t pr = ((size_t)blockIdx.x * 2 + slot) * S::RT + r;
+                    *reinterpret_cast<float4 *>(a.part + pr * HD + c) = make_float4(v[0], v[1], v[2], v[3]);
+                    if (c == 0) a.ml[pr] = make_float2(mm, ll);
+                }
+            }
+            fresh = true;
+            whole = true;
+            __syncthreads();  // the join's readers are done: the stage and the queries may be refilled
+        }
+        next(cu);
+        st = st + 1 == SA_STAGES ? 0 : st + 1;
+    }
+    cp_wait<0>();
+}
+
+// The items that several CTAs had parts of: one warp per row, the parts in
+// list order.
+template <class S>
+__global__ void __launch_bounds__(SA_THREADS) sa_join_kernel(const __grid_constant__ SaArgs a) {
+    constexpr int HD = S::HD, KT = S::KT, PL = HD / 32;
+    __shared__ long long sh_scan[SA_WARPS];
+    __shared__ long long sh_off;
+    const ds_cuda_tree_attention_t &d = a.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int b = blockIdx.y, item = blockIdx.x / (S::RT / SA_WARPS);
+    const int r = blockIdx.x % (S::RT / SA_WARPS) * SA_WARPS + warp;
+    const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
+    const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
+    long long at;
+    const long long total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
+    if (b0 <= b && b < b1) {
+        for (int x = b0; x < b; x++) at += (long long)sa_seq<KT>(d, x).tiles * d.n_kv_heads * a.row_tiles;
+        sh_off = at;
+    }
+    const SaSeq s = sa_seq<KT>(d, b);
+    __syncthreads();
+    const long long ctas = min((long long)a.ctas, total), x0 = sh_off + (long long)item * s.tiles;
+    const int c0 = sa_cta_of(x0, total, ctas), c1 = sa_cta_of(x0 + s.tiles - 1, total, ctas);
+    const int rt = item % a.row_tiles, g = item / a.row_tiles, row = rt * S::RT + r;
+    pdl_wait();
+    if (c0 == c1 || row >= a.rows) return;
+    float m = -__FLT_MAX__, l = 0.f, o[PL] = {};
+    for (int c = c0; c <= c1; c += 8) {
+        float2 ml[8];
+        float v[8][PL];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int cc = min(c + k, c1);
+            const size_t pr = ((size_t)cc * 2 + (cc == c0)) * S::RT + r;
+            ml[k] = a.ml[pr];
+            if (PL == 4) {
+                const float4 u = *reinterpret_cast<const float4 *>(a.part + pr * HD + lane * 4);
+                v[k][0] = u.x, v[k][1] = u.y, v[k][PL - 2] = u.z, v[k][PL - 1] = u.w;
+            } else {
+                const float2 u = *reinterpret_cast<const float2 *>(a.part + pr * HD + lane * 2);
+                v[k][0] = u.x, v[k][1] = u.y;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (c + k > c1) break;
+            const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn), e = ex2(ml[k].x - mn);
+            m = mn;
+            l = l * f + ml[k].y * e;
+#pragma unroll
+            for (int x = 0; x < PL; x++) o[x] = o[x] * f + v[k][x] * e;
+        }
+    }
+    const int nd = row / a.group, head = g * a.group + row % a.group;
+    const bool none = nd >= s.cnt || l == 0.f;
+    const float inv = 1.f / l;
+    const int64_t oo = b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + lane * PL;
+#pragma unroll
+    for (int x = 0; x < PL; x++) o[x] = none ? 0.f : o[x] * inv;
+    if (d.type == DS_CUDA_SPEC_F32) {
+#pragma unroll
+        for (int x = 0; x < PL; x += 2)
+            *reinterpret_cast<float2 *>((float *)d.out + oo + x) = make_float2(o[x], o[x + 1]);
+    } else {
+#pragma unroll
+        for (int x = 0; x < PL; x += 2)
+            *reinterpret_cast<uint32_t *>((uint16_t *)d.out + oo + x) =
+                d.type == DS_CUDA_SPEC_F16 ? pack2<true>(o[x], o[x + 1]) : pack2<false>(o[x], o[x + 1]);
     }
     if (d.lse && lane == 0)
-        d.lse[((size_t)b * d.n_nodes + i) * d.n_heads + h] = l == 0.f ? -INFINITY : m + logf(l);
+        d.lse[((size_t)b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718f;
+}
+
+template <class S> static cudaError_t sa_run(SaArgs a, int device, cudaStream_t st) {
+    static std::atomic<uint64_t> ready;  // devices (of the first 64) whose attribute is set
+    if (device >= 64 || !(ready.load() >> device & 1)) {
+        const cudaError_t e = cudaFuncSetAttribute(sa_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e != cudaSuccess) return e;
+        if (device < 64) ready.fetch_or(1ull << device);
+    }
+    sa_kernel<S><<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    void *args[] = {&a};
+    return launch_ex((const void *)sa_join_kernel<S>,
+                     dim3(a.d.n_kv_heads * a.row_tiles * (S::RT / SA_WARPS), a.d.batch), dim3(SA_THREADS), 0, st, true, args);
+}
+
+// The row tile: up to 64 rows, or 32 with F32 queries, whose three planes
+// take the shared memory.
+static int sa_row_tile(const ds_cuda_tree_attention_t *d) {
+    const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
+    return rows <= 16 ? 16 : rows <= 32 || d->type == DS_CUDA_SPEC_F32 ? 32 : 64;
+}
+
+template <int HD> static cudaError_t sa_pick(const SaArgs &a, bool two, int rt, int dev, cudaStream_t st) {
+    constexpr int B = DS_CUDA_SPEC_BF16, H = DS_CUDA_SPEC_F16, F = DS_CUDA_SPEC_F32;
+    if (a.d.type == F && two) return rt == 16 ? sa_run<SaShape<HD, 1, 2, F>>(a, dev, st) : sa_run<SaShape<HD, 2, 2, F>>(a, dev, st);
+    if (a.d.type == F) return rt == 16 ? sa_run<SaShape<HD, 1, 1, F>>(a, dev, st) : sa_run<SaShape<HD, 2, 1, F>>(a, dev, st);
+    if (a.d.type == H)
+        return rt == 16 ? sa_run<SaShape<HD, 1, 1, H>>(a, dev, st)
+               : rt == 32 ? sa_run<SaShape<HD, 2, 1, H>>(a, dev, st) : sa_run<SaShape<HD, 4, 1, H>>(a, dev, st);
+    return rt == 16 ? sa_run<SaShape<HD, 1, 1, B>>(a, dev, st)
+           : rt == 32 ? sa_run<SaShape<HD, 2, 1, B>>(a, dev, st) : sa_run<SaShape<HD, 4, 1, B>>(a, dev, st);
 }
 
 // One CTA per sequence, one thread per node: a node's word bits are set by
@@ -148,9 +760,14 @@ static int sa_check(ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
     return DS_CUDA_OK;
 }
 
+static int sa_ctas(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
+    return c->sm_count * (d->head_dim == 64 ? 2 : 1);
+}
+
 extern "C" size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d) {
     if (!c || !c->ok || sa_check(nullptr, d) < 0) return 0;
-    return 0;
+    // two parts a CTA, each of at most 64 rows with their maxima and sums
+    return sa_ctas(c, d) * (size_t)2 * 64 * (d->head_dim * 4 + 8);
 }
 
 extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d, void *stream) {
@@ -177,13 +794,25 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
         if (t.lo && d->type != DS_CUDA_SPEC_F32)
             return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: %s has a lo plane, which only the F32 type takes", t.name);
     }
-    SaArgs a = {*d, (d->n_nodes + 63) / 64};
+    const size_t need = ds_cuda_tree_attention_workspace(c, d);
+    if (!d->workspace || d->workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->workspace) & 255))
+        return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: workspace of %zu bytes, 256-byte aligned, wanted", need);
+    const bool two = d->type == DS_CUDA_SPEC_F32 && (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo);
+    const int rt = sa_row_tile(d);
+    SaArgs a = {};
+    a.d = *d;
+    a.words = (d->n_nodes + 63) / 64;
+    a.group = d->n_heads / d->n_kv_heads;
+    a.rows = d->n_nodes * a.group;
+    a.row_tiles = (a.rows + rt - 1) / rt;
+    a.ctas = sa_ctas(c, d);
+    a.scale2 = d->scale * 1.44269504f;
+    a.part = (float *)d->workspace;
+    a.ml = (float2 *)(a.part + (size_t)a.ctas * 2 * rt * d->head_dim);
     cudaSetDevice(c->device);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    const dim3 grid(d->n_nodes, d->n_heads, d->batch);
-    if (d->head_dim == 64) sa_rows_kernel<64><<<grid, 128, 0, st>>>(a);
-    else sa_rows_kernel<128><<<grid, 128, 0, st>>>(a);
-    return ctx_cuda(c, cudaGetLastError(), "tree_attention launch");
+    const cudaError_t e = d->head_dim == 64 ? sa_pick<64>(a, two, rt, c->device, st) : sa_pick<128>(a, two, rt, c->device, st);
+    return ctx_cuda(c, e, "tree_attention launch");
 }
 
 extern "C" int ds_cuda_tree_mask_dev(ds_cuda_ctx_t *c, const int *parents, const int *nodes, int batch, int n_nodes,
