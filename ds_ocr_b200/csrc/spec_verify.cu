@@ -2,17 +2,27 @@
 // ds_cuda_tree_verify_greedy_dev), the target's probabilities
 // (ds_cuda_token_probs_dev) and the commit of accepted K and V rows
 // (ds_cuda_tree_commit_dev).
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "ctx.h"
 
+namespace cg = cooperative_groups;
+
 namespace ds {
 
 constexpr int SV_MAX_NODES = 256;
 constexpr int SV_MAX_VOCAB = 1 << 18;
-constexpr int SV_THREADS = 1024;
+constexpr int SV_THREADS = 512;
+constexpr int SV_WARPS = SV_THREADS / 32;
+constexpr int SV_CLUSTER = 8;  // CTAs a row of the vocabulary is spread over, at most
+
+// Every CTA of a cluster arrives when it starts and waits before it first
+// writes to another's shared memory, which has to exist by then.
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait_started() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // A probability as a whole multiple of 2^-44, clamped to [0, 1] (NaN is 0):
 // at most 2^18 of them sum to less than 2^63, whatever the order.
@@ -20,99 +30,192 @@ __device__ __forceinline__ unsigned long long sv_fixed(float p) {
     if (!(p > 0.f)) return 0;
     return (unsigned long long)__fmul_rn(fminf(p, 1.f), 0x1p44f);
 }
-
-__device__ __forceinline__ unsigned long long sv_block_sum(unsigned long long v, unsigned long long *sh) {
+__device__ __forceinline__ unsigned long long warp_sum_u64(unsigned long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(DS_FULL, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < SV_THREADS / 32; w++) v += sh[w];
+    return v;
+}
+__device__ __forceinline__ unsigned long long warp_scan_u64(unsigned long long v) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(DS_FULL, v, o);
+        if ((int)(threadIdx.x & 31) >= o) v += u;
+    }
     return v;
 }
 
-// One CTA per sequence. r(x) is recomputed from the probabilities by
-// replaying the node's rejections (their masses and tokens are kept).
+// One cluster per sequence; its CTAs hold a row's residual r in registers,
+// up to VPT values a thread: CTA k the indices from k * slice, warp w of it
+// `run` consecutive ones, read 32 at a time. Every CTA walks the tree by
+// itself (the walk needs single probabilities, gathered at the start, and
+// the masses of the rejections at the current node); a row is read only
+// where a rejection needs its residual's mass, or the next token is drawn.
+// What bounds it is latency: the gather, then per row pass one read of the
+// row (two with a draft) and one exchange of sums in the cluster.
+template <int VPT>
 __global__ void __launch_bounds__(SV_THREADS) tree_verify_kernel(const __grid_constant__ ds_cuda_tree_verify_t d) {
-    __shared__ unsigned long long sh[SV_THREADS / 32];
-    __shared__ float mass[SV_MAX_NODES];
+    __shared__ int par[SV_MAX_NODES], tok[SV_MAX_NODES], way[SV_MAX_NODES];
+    __shared__ float acc_u[SV_MAX_NODES], pt[SV_MAX_NODES], pd[SV_MAX_NODES], mass[SV_MAX_NODES];
     __shared__ int gone[SV_MAX_NODES];
-    __shared__ unsigned long long part[SV_THREADS];
-    const int b = blockIdx.x, n = d.n_nodes, V = d.vocab, tid = threadIdx.x;
+    __shared__ unsigned long long wsum[SV_WARPS], csum[2][SV_CLUSTER];
+    const cg::cluster_group cl = cg::this_cluster();
+    cluster_started();
+    const int ncta = cl.num_blocks(), rank = cl.block_rank();
+    const int b = blockIdx.x / ncta, n = d.n_nodes, V = d.vocab, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cnt = d.nodes ? min(max(d.nodes[b], 0), n) : n;
-    const int *par = d.parents + (size_t)b * n, *tok = d.tokens + (size_t)b * n;
-    int *path = d.path + (size_t)b * n;
     const float *target = d.target + b * d.target_stride[0];
     const float *draft = d.draft ? d.draft + b * d.draft_stride[0] : nullptr;
+    const float u_last = d.sample_u[b];
+    if (tid < cnt) {
+        const int p = d.parents[(size_t)b * n + tid], x = d.tokens[(size_t)b * n + tid];
+        par[tid] = p;
+        tok[tid] = x;
+        acc_u[tid] = d.accept_u[(size_t)b * n + tid];
+        const bool ok = p >= 0 && p < tid && x >= 0 && x < V;
+        pt[tid] = ok ? target[p * d.target_stride[1] + x] : 0.f;
+        pd[tid] = ok && draft ? draft[p * d.draft_stride[1] + x] : 1.f;
+    }
+    __syncthreads();
+    cluster_wait_started();
+
+    const int slice = (V + ncta - 1) / ncta, run = (slice + SV_THREADS - 1) / SV_THREADS * 32;  // run <= 32 VPT
+    const int v0 = rank * slice + warp * run + lane;            // this thread's indices: v0 + 32 j
+    const int vend = min(min(V, (rank + 1) * slice), rank * slice + (warp + 1) * run);
+    const int jn = max(0, (vend - v0 + 31) / 32);
+    float r[VPT];
+    unsigned long long total = 0, below = 0;
+    int parity = 0;
+    // the sum over the vocabulary; leaves the warps' sums in wsum and the
+    // CTAs' in csum[parity ^ 1]
+    auto sum = [&]() {
+        unsigned long long s = 0;
+#pragma unroll
+        for (int j = 0; j < VPT; j++)
+            if (j < jn) s += sv_fixed(r[j]);
+        s = warp_sum_u64(s);
+        __syncthreads();  // the previous readers of wsum are done
+        if (lane == 0) wsum[warp] = s;
+        __syncthreads();
+        if (tid < ncta) {
+            unsigned long long c = 0;
+#pragma unroll
+            for (int w = 0; w < SV_WARPS; w++) c += wsum[w];
+            cl.map_shared_rank(&csum[parity][0], tid)[rank] = c;
+        }
+        cl.sync();
+        total = below = 0;
+        for (int k = 0; k < ncta; k++) {
+            if (k < rank) below += csum[parity][k];
+            total += csum[parity][k];
+        }
+        parity ^= 1;
+    };
+    auto load = [&](const float *row) {
+#pragma unroll
+        for (int j = 0; j < VPT; j++)
+            if (j < jn) r[j] = __ldg(row + v0 + 32 * j);
+    };
+
     int cur = 0, nrej = 0, deep = 0;
     float m = 1.f;
-    auto resid = [&](int x) {
-        float r = target[cur * d.target_stride[1] + x];
-        if (draft) {
-            const float p = draft[cur * d.draft_stride[1] + x];
-            for (int k = 0; k < nrej; k++) r = fmaxf(__fsub_rn(r, __fmul_rn(mass[k], p)), 0.f);
-        } else {
-            for (int k = 0; k < nrej; k++)
-                if (gone[k] == x) r = fmaxf(__fsub_rn(r, mass[k]), 0.f);
-        }
-        return r;
-    };
-    if (tid == 0) path[0] = 0;
+    if (tid == 0) way[0] = 0;
     for (int c = 1; c < cnt; c++) {
         if (par[c] != cur) continue;
         const int x = tok[c];
-        bool ok = false;
-        if (x >= 0 && x < V) {
-            const float p = draft ? draft[cur * d.draft_stride[1] + x] : 1.f;
-            ok = __fmul_rn(d.accept_u[(size_t)b * n + c], __fmul_rn(p, m)) < resid(x);
-        }
-        if (ok) {
+        const float p = pd[c];
+        float rx = pt[c];  // r(x): the rejections so far replayed for one token
+        for (int k = 0; k < nrej; k++)
+            if (draft || gone[k] == x) rx = fmaxf(__fsub_rn(rx, __fmul_rn(mass[k], p)), 0.f);
+        if (x >= 0 && x < V && __fmul_rn(acc_u[c], __fmul_rn(p, m)) < rx) {
             cur = c;
             nrej = 0;
             m = 1.f;
             deep++;
-            if (tid == 0) path[deep] = c;
+            if (tid == 0) way[deep] = c;
+            continue;
+        }
+        const float *row = target + cur * d.target_stride[1];
+        if (nrej == 0) load(row);
+        if (draft) {
+            const float *drow = draft + cur * d.draft_stride[1];
+            float q[VPT];
+#pragma unroll
+            for (int j = 0; j < VPT; j++)
+                if (j < jn) q[j] = __ldg(drow + v0 + 32 * j);
+#pragma unroll
+            for (int j = 0; j < VPT; j++)
+                if (j < jn) r[j] = fmaxf(__fsub_rn(r[j], __fmul_rn(m, q[j])), 0.f);
         } else {
-            __syncthreads();
-            if (tid == 0) {
-                mass[nrej] = m;
-                gone[nrej] = x;
-            }
-            __syncthreads();
-            nrej++;
-            unsigned long long s = 0;
-            for (int v = tid; v < V; v += SV_THREADS) s += sv_fixed(resid(v));
-            m = __fmul_rn((float)sv_block_sum(s, sh), 0x1p-44f);
+#pragma unroll
+            for (int j = 0; j < VPT; j++)
+                if (j < jn && v0 + 32 * j == x) r[j] = fmaxf(__fsub_rn(r[j], m), 0.f);
+        }
+        if (tid == 0) {
+            mass[nrej] = m;
+            gone[nrej] = x;
+        }
+        nrej++;
+        sum();
+        m = __fmul_rn((float)total, 0x1p-44f);
+    }
+    // the next token: from the residual whose sums were taken last, or from
+    // the target's row where nothing was rejected or no mass is left
+    if (nrej == 0 || total == 0) {
+        load(target + cur * d.target_stride[1]);
+        sum();
+    }
+    if (rank == 0) {
+        __syncthreads();  // way is written
+        for (int j = tid; j < n; j += SV_THREADS) d.path[(size_t)b * n + j] = j <= deep ? way[j] : -1;
+        if (tid == 0) d.accepted[b] = deep;
+        if (tid == 0 && total == 0) d.token[b] = -1;
+    }
+    const unsigned long long u = (unsigned long long)__fmul_rn(fminf(fmaxf(u_last, 0.f), 0x1.fffffep-1f), 0x1p24f);
+    const unsigned long long lim = (total >> 24) * u + (((total & 0xffffffull) * u) >> 24);  // < total
+    // the warp whose indices hold the threshold finds the 32 and the one
+    for (int w = 0; w < warp; w++) below += wsum[w];
+    if (lim < below || lim >= below + wsum[warp]) return;
+    unsigned long long s[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; j++) s[j] = j < jn ? sv_fixed(r[j]) : 0;
+    int j0 = 0;
+    if (VPT == 64) {  // which half
+        unsigned long long h = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j++) h += s[j];
+        h = warp_sum_u64(h);
+        if (lim >= below + h) {
+            below += h;
+            j0 = 32;
+#pragma unroll
+            for (int j = 0; j < 32; j++) s[j] = s[VPT - 32 + j];
         }
     }
-    for (int j = deep + 1 + tid; j < n; j += SV_THREADS) path[j] = -1;
-    // the next token: each thread's run of V, then the run that holds the threshold
-    const int run = (V + SV_THREADS - 1) / SV_THREADS, v0 = min(V, tid * run), v1 = min(V, v0 + run);
-    unsigned long long total = 0;
-    for (int pass = 0; pass < 2 && total == 0; pass++) {
-        if (pass) nrej = 0;
-        unsigned long long s = 0;
-        for (int v = v0; v < v1; v++) s += sv_fixed(resid(v));
-        total = sv_block_sum(s, sh);
-        part[tid] = s;
-    }
-    __syncthreads();
-    if (tid) return;
-    int t = -1;
-    if (total) {
-        const unsigned long long u = (unsigned long long)__fmul_rn(fminf(fmaxf(d.sample_u[b], 0.f), 0x1.fffffep-1f), 0x1p24f);
-        const unsigned long long lim = (total >> 24) * u + (((total & 0xffffffull) * u) >> 24);
-        unsigned long long cum = 0;
-        int k = 0;
-        while (k < SV_THREADS - 1 && cum + part[k] <= lim) cum += part[k++];
-        for (t = k * run; t < V - 1; t++) {
-            cum += sv_fixed(resid(t));
-            if (cum > lim) break;
+    unsigned long long own[32];
+#pragma unroll
+    for (int j = 0; j < 32; j++) own[j] = s[j];
+    // sums over the lanes of 32 values at once: after the step of width o a
+    // lane holds o values, those whose index agrees with it in the upper bits
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int k = 0; k < o; k++) {
+            const unsigned long long keep = up ? s[k + o] : s[k], give = up ? s[k] : s[k + o];
+            s[k] = keep + __shfl_xor_sync(DS_FULL, give, o);
         }
     }
-    d.token[b] = t;
-    d.accepted[b] = deep;
+    unsigned long long cum = warp_scan_u64(s[0]);  // lane j: the sum of the values up to j
+    unsigned hit = __ballot_sync(DS_FULL, below + cum > lim);
+    const int j = __ffs(hit) - 1;
+    below += __shfl_sync(DS_FULL, cum - s[0], j);
+    unsigned long long e = 0;
+#pragma unroll
+    for (int k = 0; k < 32; k++)
+        if (k == j) e = own[k];
+    cum = warp_scan_u64(e);
+    hit = __ballot_sync(DS_FULL, below + cum > lim);
+    if (lane == __ffs(hit) - 1) d.token[b] = v0 + 32 * (j0 + j);
 }
 
 __global__ void tree_verify_greedy_kernel(const int *tokens, const int *parents, const int *nodes, const int *want,
@@ -137,50 +240,102 @@ template <typename T> __device__ __forceinline__ float tp_f(T v) { return (float
 template <> __device__ __forceinline__ float tp_f(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float tp_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// One CTA per row, three passes.
-template <typename T>
-__global__ void __launch_bounds__(1024) token_probs_kernel(const T *logits, int V, int64_t stride, const float *temp, float *out) {
-    __shared__ float sh[32];
+// One cluster per row, its CTAs taking consecutive slices. HELD: the slice is
+// kept in registers, VPT values a thread, so the logits are read once; wider
+// vocabularies read them three times (from L2 but for the first). A CTA
+// takes its own maximum m and sum s of e = 2^((x - m) c), c = log2(e) /
+// temperature; one exchange of (m, s) in the cluster gives every CTA the
+// row's M and S, and p = e * (2^((m - M) c) / S). Bound by the memory:
+// reads of consecutive elements, one per thread, whatever a row's alignment.
+constexpr int TP_VPT = 32;
+template <typename T, bool HELD>
+__global__ void __launch_bounds__(SV_THREADS, 2) token_probs_kernel(const T *logits, int V, int64_t stride,
+                                                                 const float *temp, float *out) {
+    __shared__ float sh[SV_WARPS];
+    __shared__ float2 ms[SV_CLUSTER];
+    __shared__ unsigned long long key[SV_CLUSTER];
+    __shared__ int bad[SV_CLUSTER];
     __shared__ unsigned long long best;
-    const T *x = logits + blockIdx.x * stride;
-    out += (size_t)blockIdx.x * V;
-    const float tt = temp ? temp[blockIdx.x] : 1.f;
-    const int tid = threadIdx.x;
+    const cg::cluster_group cl = cg::this_cluster();
+    cluster_started();
+    const int ncta = cl.num_blocks(), rank = cl.block_rank(), row = blockIdx.x / ncta;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int slice = (V + ncta - 1) / ncta, i0 = min(V, rank * slice), len = min(V, i0 + slice) - i0;
+    const T *x = logits + row * stride + i0;
+    out += (size_t)row * V + i0;
+    const float tt = temp ? temp[row] : 1.f, c = __fdiv_rn(1.44269504f, tt);
+    auto each = [&](auto f) {  // f(index in the slice, its place in registers)
+        if (HELD) {
+#pragma unroll
+            for (int j = 0; j < TP_VPT; j++)
+                if (tid + j * SV_THREADS < len) f(tid + j * SV_THREADS, j);
+        } else {
+            for (int i = tid; i < len; i += SV_THREADS) f(i, 0);
+        }
+    };
+    float v[HELD ? TP_VPT : 1];
+    if (HELD) each([&](int i, int j) { v[j] = tp_f(x[i]); });
+    cluster_wait_started();
+    auto val = [&](int i, int j) { return HELD ? v[j] : tp_f(x[i]); };
+
+    if (tt <= 0.f || c == INFINITY) {  // the largest logit has everything
+        unsigned long long k = 0;
+        bool nan = false;
+        each([&](int i, int j) {
+            const float l = val(i, j);
+            nan |= !(l < INFINITY);
+            const unsigned long long kk = argmax_key(l, i0 + i);
+            if (l > -INFINITY && kk > k) k = kk;
+        });
+        if (tid == 0) best = 0;
+        nan = __syncthreads_or(nan);
+        atomicMax(&best, k);
+        __syncthreads();
+        if (tid < ncta) {
+            cl.map_shared_rank(key, tid)[rank] = best;
+            cl.map_shared_rank(bad, tid)[rank] = nan;
+        }
+        cl.sync();
+        k = 0;
+        for (int r = 0; r < ncta; r++) {
+            nan |= bad[r];
+            if (key[r] > k) k = key[r];
+        }
+        const int at = k ? (int)(0xffffffffu - (uint32_t)k) - i0 : -1;
+        each([&](int i, int) { out[i] = nan ? NAN : i == at ? 1.f : 0.f; });
+        return;
+    }
+
     float m = -INFINITY;
-    bool bad = false;
-    unsigned long long key = 0;
-    for (int v = tid; v < V; v += 1024) {
-        const float l = tp_f(x[v]);
-        bad |= isnan(l);
-        m = fmaxf(m, l);
-        const unsigned long long k = argmax_key(l, v);
-        if (!isnan(l) && k > key) key = k;
-    }
-    if (tid == 0) best = 0;
-    bad = __syncthreads_or(bad);
-    atomicMax(&best, key);
+    each([&](int i, int j) { m = fmaxf(m, val(i, j)); });
     m = warp_max(m);
-    if ((tid & 31) == 0) sh[tid >> 5] = m;
+    if (lane == 0) sh[warp] = m;
     __syncthreads();
-    for (int w = 0; w < 32; w++) m = fmaxf(m, sh[w]);
-    __syncthreads();
-    if (bad || m == INFINITY || isnan(tt)) {
-        for (int v = tid; v < V; v += 1024) out[v] = NAN;
-        return;
-    }
-    if (m == -INFINITY || tt <= 0.f) {
-        const int at = m == -INFINITY ? -1 : (int)(0xffffffffu - (uint32_t)best);
-        for (int v = tid; v < V; v += 1024) out[v] = v == at ? 1.f : 0.f;
-        return;
-    }
+#pragma unroll
+    for (int w = 0; w < SV_WARPS; w++) m = fmaxf(m, sh[w]);
+    // -infinity first: the slice may hold nothing else
+    auto weight = [&](float l) { return l == -INFINITY ? 0.f : exp2f((l - m) * c); };
     float s = 0.f;
-    for (int v = tid; v < V; v += 1024) s += expf((tp_f(x[v]) - m) / tt);
+    each([&](int i, int j) {
+        const float e = weight(val(i, j));
+        if (HELD) v[j] = e;
+        s += e;
+    });
     s = warp_sum(s);
-    if ((tid & 31) == 0) sh[tid >> 5] = s;
+    __syncthreads();
+    if (lane == 0) sh[warp] = s;
     __syncthreads();
     s = 0.f;
-    for (int w = 0; w < 32; w++) s += sh[w];
-    for (int v = tid; v < V; v += 1024) out[v] = expf((tp_f(x[v]) - m) / tt) / s;
+#pragma unroll
+    for (int w = 0; w < SV_WARPS; w++) s += sh[w];
+    if (tid < ncta) cl.map_shared_rank(ms, tid)[rank] = make_float2(m, s);
+    cl.sync();
+    float M = -INFINITY, S = 0.f;
+    for (int r = 0; r < ncta; r++) M = fmaxf(M, ms[r].x);
+    // a slice of -infinity alone has s = 0 (or NaN, which stays)
+    for (int r = 0; r < ncta; r++) S += ms[r].x == -INFINITY ? ms[r].y : ms[r].y * exp2f((ms[r].x - M) * c);
+    const float f = S == 0.f ? 0.f : (m == -INFINITY ? 1.f : exp2f((m - M) * c)) / S;
+    each([&](int i, int j) { __stcs(out + i, (HELD ? v[j] : weight(tp_f(x[i]))) * f); });
 }
 
 // One thread per 16 bytes of a row.
@@ -211,6 +366,20 @@ static cudaStream_t sv_stream(ds_cuda_ctx *c, void *s) {
     return s ? (cudaStream_t)s : c->stream;
 }
 
+static cudaError_t launch_cluster(const void *f, long long ctas, int ncta, cudaStream_t st, void **args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(SV_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ncta;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelExC(&cfg, f, args);
+}
+
 extern "C" int ds_cuda_tree_verify_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_verify_t *d, void *stream) {
     if (!c || !c->ok) return DS_CUDA_EINVAL;
     if (!d || d->batch < 0 || d->n_nodes <= 0 || d->n_nodes > SV_MAX_NODES || d->vocab <= 0 || d->vocab > SV_MAX_VOCAB)
@@ -220,8 +389,17 @@ extern "C" int ds_cuda_tree_verify_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_veri
     if (!d->tokens || !d->parents || !d->target || !d->accept_u || !d->sample_u || !d->path || !d->accepted || !d->token)
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_verify: null pointer");
     cudaStream_t st = sv_stream(c, stream);
-    tree_verify_kernel<<<d->batch, SV_THREADS, 0, st>>>(*d);
-    return ctx_cuda(c, cudaGetLastError(), "tree_verify launch");
+    // enough CTAs for the row to fit the registers; more where the batch
+    // leaves SMs idle, which shortens a row's pass
+    const bool wide = d->vocab > SV_CLUSTER * SV_THREADS * 32;
+    int ncta = 1;
+    while (ncta < SV_CLUSTER && (ncta * SV_THREADS * 32 < d->vocab ||
+                                 (d->vocab > ncta * SV_THREADS && d->batch * ncta * 2 <= c->sm_count)))
+        ncta *= 2;
+    ds_cuda_tree_verify_t a = *d;
+    void *args[] = {&a};
+    return ctx_cuda(c, launch_cluster(wide ? (const void *)tree_verify_kernel<64> : (const void *)tree_verify_kernel<32>,
+                                      (long long)d->batch * ncta, ncta, st, args), "tree_verify launch");
 }
 
 extern "C" int ds_cuda_tree_verify_greedy_dev(ds_cuda_ctx_t *c, const int *tokens, const int *parents, const int *nodes,
@@ -248,13 +426,19 @@ extern "C" int ds_cuda_token_probs_dev(ds_cuda_ctx_t *c, int type, const void *l
     if (rows == 0) return DS_CUDA_OK;  // an empty tensor has no address
     if (!logits || !probs) return ctx_fail(c, DS_CUDA_EINVAL, "token_probs: null pointer");
     cudaStream_t st = sv_stream(c, stream);
-    if (type == DS_CUDA_SPEC_F32)
-        token_probs_kernel<<<rows, 1024, 0, st>>>((const float *)logits, vocab, row_stride, temperature, probs);
-    else if (type == DS_CUDA_SPEC_F16)
-        token_probs_kernel<<<rows, 1024, 0, st>>>((const __half *)logits, vocab, row_stride, temperature, probs);
-    else
-        token_probs_kernel<<<rows, 1024, 0, st>>>((const __nv_bfloat16 *)logits, vocab, row_stride, temperature, probs);
-    return ctx_cuda(c, cudaGetLastError(), "token_probs launch");
+    const bool held = vocab <= SV_CLUSTER * SV_THREADS * TP_VPT;
+    int ncta = 1;
+    while (ncta < SV_CLUSTER && (ncta * SV_THREADS * TP_VPT < vocab ||
+                                 (vocab > ncta * SV_THREADS * 4 && rows * ncta * 2 <= c->sm_count)))
+        ncta *= 2;
+    const void *f = type == DS_CUDA_SPEC_F32 ? (held ? (const void *)token_probs_kernel<float, true>
+                                                     : (const void *)token_probs_kernel<float, false>)
+                    : type == DS_CUDA_SPEC_F16 ? (held ? (const void *)token_probs_kernel<__half, true>
+                                                       : (const void *)token_probs_kernel<__half, false>)
+                    : held ? (const void *)token_probs_kernel<__nv_bfloat16, true>
+                           : (const void *)token_probs_kernel<__nv_bfloat16, false>;
+    void *args[] = {(void *)&logits, &vocab, &row_stride, (void *)&temperature, &probs};
+    return ctx_cuda(c, launch_cluster(f, (long long)rows * ncta, ncta, st, args), "token_probs launch");
 }
 
 extern "C" int ds_cuda_tree_commit_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_commit_t *d, void *stream) {

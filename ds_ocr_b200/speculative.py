@@ -20,6 +20,7 @@ on another stream needs the usual event or record_stream. Nothing
 synchronises and nothing is kept between calls.
 """
 import ctypes
+import struct
 
 from .cuda import Context
 
@@ -56,6 +57,25 @@ class TreeCommitDesc(ctypes.Structure):
                 ("accepted", _ptr), ("new_lens", _ptr)]
 
 
+def _packer(cls):
+    """A struct.Struct that packs a descriptor's fields in order (a tenth of
+    the time of setting them one by one)."""
+    code = {_int: "i", ctypes.c_float: "f", _ptr: "P", _i64: "q", ctypes.c_size_t: "N"}
+
+    def one(t):
+        n = 1
+        while issubclass(t, ctypes.Array):
+            n, t = n * t._length_, t._type_
+        return f"{n}{code[t]}"
+
+    s = struct.Struct("@" + "".join(one(t) for _, t in cls._fields_))
+    assert s.size == ctypes.sizeof(cls)
+    return s.pack
+
+
+_pack_attention, _pack_verify, _pack_commit = (_packer(c) for c in (TreeAttentionDesc, TreeVerifyDesc, TreeCommitDesc))
+
+
 class Speculative:
     """The speculative-decoding operators of one context."""
 
@@ -65,7 +85,9 @@ class Speculative:
         self.ctx = ctx or Context(0)
         self.lib = self.ctx.lib
         self.device = torch.device("cuda", self.ctx.device)
+        self._index = self.ctx.device
         self._types = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
+        self._workspace = {}  # bytes by sizes
 
     def _stream(self):
         # torch's default stream is the legacy stream (handle 0), which the C
@@ -73,32 +95,37 @@ class Speculative:
         return self.torch.cuda.current_stream(self.device).cuda_stream or 1
 
     def _want(self, name, t, shape, dtype, contiguous=True):
-        if t.device != self.device or t.dtype != dtype or t.shape != shape:
+        """The address of a tensor that has to be as given."""
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index:
             raise ValueError(f"{name}: expected {dtype} {tuple(shape)} on {self.device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
         if contiguous and not t.is_contiguous():
             raise ValueError(f"{name}: must be contiguous")
         return t.data_ptr()
 
+    def _strided(self, name, t, shape, dtype):
+        """(address, strides without the last, which is 1)."""
+        p = self._want(name, t, shape, dtype, False)
+        *st, last = t.stride()
+        if last != 1 and shape[-1] > 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous")
+        return p, st
+
     def _rows(self, name, planes, shape, dtype, pair):
-        """(address, lo address, strides) of a K or V tensor: one tensor, or
+        """Address, lo address, strides of a K or V tensor: one tensor, or
         with F32 queries its BF16 plane and optional lo plane."""
         if isinstance(planes, self.torch.Tensor):
             planes = (planes,)
         if not 1 <= len(planes) <= (2 if pair else 1):
             raise ValueError(f"{name}: {len(planes)} planes" + (" (at most 2)" if pair else
                                                                " (a second plane goes with float32 queries)"))
-        a = planes[0]
-        p = self._want(name, a, shape, dtype, False)
-        st = a.stride()
-        if st[-1] != 1:
-            raise ValueError(f"{name}: the head dimension must be contiguous")
+        p, st = self._strided(name, planes[0], shape, dtype)
         if len(planes) == 1:
-            return p, None, st
-        lo = planes[1]
-        if lo.stride() != st:
+            return p, 0, *st
+        lo, lst = self._strided(name + " lo plane", planes[1], shape, dtype)
+        if lst != st:
             raise ValueError(f"{name}: the planes must have the same strides")
-        return p, self._want(name + " lo plane", lo, shape, dtype, False), st
+        return p, lo, *st
 
     def tree_mask(self, parents, counts=None):
         """Mask words [batch x n_nodes x ceil(n_nodes / 64)] (int64 bits) and
@@ -125,47 +152,35 @@ class Speculative:
         [batch x n_nodes x n_heads] float32 output. Returns out."""
         torch = self.torch
         b, n, heads, hd = q.shape
-        ty = self._types.get(q.dtype)
+        qt = q.dtype
+        ty = self._types.get(qt)
         if ty is None:
-            raise ValueError(f"q: unsupported dtype {q.dtype}")
-        kt = torch.bfloat16 if ty == F32 else q.dtype
+            raise ValueError(f"q: unsupported dtype {qt}")
+        pair = ty == F32
+        kt = torch.bfloat16 if pair else qt
         k0 = k if isinstance(k, torch.Tensor) else k[0]
         if k0.dim() != 4:
             raise ValueError("k: expected [batch x n_kv_heads x kv_max x head_dim]")
-        kv, cap = k0.shape[1], k0.shape[2]
-        qp = self._want("q", q, (b, n, heads, hd), q.dtype, False)
-        qs = q.stride()
-        if qs[3] != 1:
-            raise ValueError("q: the head dimension must be contiguous")
+        _, kv, cap, _ = k0.shape
         if out is None:
-            out = torch.empty((b, n, heads, hd), dtype=q.dtype, device=self.device)
-        op = self._want("out", out, (b, n, heads, hd), q.dtype, False)
-        os = out.stride()
-        if os[3] != 1:
-            raise ValueError("out: the head dimension must be contiguous")
-        d = TreeAttentionDesc()
-        d.type, d.batch, d.n_nodes, d.n_heads, d.n_kv_heads, d.head_dim, d.kv_max = ty, b, n, heads, kv, hd, cap
-        d.scale = hd ** -0.5 if scale is None else scale
-        d.q, d.q_stride = qp, qs[:3]
-        d.out, d.out_stride = op, os[:3]
-        d.k, d.k_lo, st = self._rows("k", k, (b, kv, cap, hd), kt, ty == F32)
-        d.k_stride = st[:3]
-        d.v, d.v_lo, st = self._rows("v", v, (b, kv, cap, hd), kt, ty == F32)
-        d.v_stride = st[:3]
-        d.tree_k, d.tree_k_lo, st = self._rows("tree_k", tree_k, (b, kv, n, hd), kt, ty == F32)
-        d.tree_k_stride = st[:3]
-        d.tree_v, d.tree_v_lo, st = self._rows("tree_v", tree_v, (b, kv, n, hd), kt, ty == F32)
-        d.tree_v_stride = st[:3]
-        d.lens = self._want("lens", lens, (b,), torch.int32)
-        d.mask = self._want("mask", mask, (b, n, (n + 63) // 64), torch.int64)
-        d.nodes = None if counts is None else self._want("counts", counts, (b,), torch.int32)
-        d.lse = None if lse is None else self._want("lse", lse, (b, n, heads), torch.float32)
-        need = self.lib.ds_cuda_tree_attention_workspace(self.ctx.h, ctypes.byref(d))
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            d.workspace, d.workspace_bytes = ws.data_ptr(), need
-        self.ctx.check(self.lib.ds_cuda_tree_attention_dev(self.ctx.h, ctypes.byref(d), self._stream()),
-                       "tree_attention")
+            out = torch.empty((b, n, heads, hd), dtype=qt, device=self.device)
+        cache, tree, i32 = (b, kv, cap, hd), (b, kv, n, hd), torch.int32
+        qp, qs = self._strided("q", q, (b, n, heads, hd), qt)
+        op, os = self._strided("out", out, (b, n, heads, hd), qt)
+        head = (ty, b, n, heads, kv, hd, cap)
+        fields = (*head, hd ** -0.5 if scale is None else scale, qp, *qs,
+                  *self._rows("k", k, cache, kt, pair), *self._rows("v", v, cache, kt, pair),
+                  *self._rows("tree_k", tree_k, tree, kt, pair), *self._rows("tree_v", tree_v, tree, kt, pair),
+                  self._want("lens", lens, (b,), i32), 0 if counts is None else self._want("counts", counts, (b,), i32),
+                  self._want("mask", mask, (b, n, (n + 63) // 64), torch.int64), op, *os,
+                  0 if lse is None else self._want("lse", lse, (b, n, heads), torch.float32))
+        need = self._workspace.get(head)
+        if need is None:
+            need = self._workspace[head] = self.lib.ds_cuda_tree_attention_workspace(self.ctx.h,
+                                                                                     _pack_attention(*fields, 0, 0))
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self.ctx.check(self.lib.ds_cuda_tree_attention_dev(self.ctx.h, _pack_attention(*fields, ws.data_ptr(), need),
+                                                           self._stream()), "tree_attention")
         return out
 
     def token_probs(self, logits, temperature=None, out=None):
@@ -177,22 +192,14 @@ class Speculative:
         ty = self._types.get(logits.dtype)
         if ty is None:
             raise ValueError(f"logits: unsupported dtype {logits.dtype}")
-        lp = self._want("logits", logits, (rows, vocab), logits.dtype, False)
-        if vocab > 1 and logits.stride(1) != 1:
-            raise ValueError("logits: the vocabulary must be contiguous")
+        lp, st = self._strided("logits", logits, (rows, vocab), logits.dtype)
         tp = None if temperature is None else self._want("temperature", temperature, (rows,), torch.float32)
         if out is None:
             out = torch.empty((rows, vocab), dtype=torch.float32, device=self.device)
-        self.ctx.check(self.lib.ds_cuda_token_probs_dev(self.ctx.h, ty, lp, rows, vocab, logits.stride(0), tp,
+        self.ctx.check(self.lib.ds_cuda_token_probs_dev(self.ctx.h, ty, lp, rows, vocab, st[0], tp,
                                                         self._want("out", out, (rows, vocab), torch.float32),
                                                         self._stream()), "token_probs")
         return out
-
-    def _probs(self, name, p, b, n, vocab):
-        a = self._want(name, p, (b, n, vocab), self.torch.float32, False)
-        if vocab > 1 and p.stride(2) != 1:
-            raise ValueError(f"{name}: the vocabulary must be contiguous")
-        return a, p.stride()[:2]
 
     def verify(self, tokens, parents, target, draft, accept_u, sample_u, counts=None):
         """Speculative sampling over each sequence's tree: tokens, parents
@@ -207,19 +214,16 @@ class Speculative:
         if target.dim() != 3:
             raise ValueError("target: expected [batch x n_nodes x vocab]")
         vocab = target.shape[2]
-        d = TreeVerifyDesc()
-        d.batch, d.n_nodes, d.vocab = b, n, vocab
-        d.tokens = self._want("tokens", tokens, (b, n), torch.int32)
-        d.parents = self._want("parents", parents, (b, n), torch.int32)
-        d.nodes = None if counts is None else self._want("counts", counts, (b,), torch.int32)
-        d.target, d.target_stride = self._probs("target", target, b, n, vocab)
-        if draft is not None:
-            d.draft, d.draft_stride = self._probs("draft", draft, b, n, vocab)
-        d.accept_u = self._want("accept_u", accept_u, (b, n), torch.float32)
-        d.sample_u = self._want("sample_u", sample_u, (b,), torch.float32)
+        i32, f32, shape = torch.int32, torch.float32, (b, n, vocab)
+        tp, ts = self._strided("target", target, shape, f32)
+        dp, ds = (0, (0, 0)) if draft is None else self._strided("draft", draft, shape, f32)
         res = self._results(b, n)
-        d.path, d.accepted, d.token = (t.data_ptr() for t in res)
-        self.ctx.check(self.lib.ds_cuda_tree_verify_dev(self.ctx.h, ctypes.byref(d), self._stream()), "tree_verify")
+        d = _pack_verify(b, n, vocab, self._want("tokens", tokens, (b, n), i32),
+                         self._want("parents", parents, (b, n), i32),
+                         0 if counts is None else self._want("counts", counts, (b,), i32), tp, *ts, dp, *ds,
+                         self._want("accept_u", accept_u, (b, n), f32), self._want("sample_u", sample_u, (b,), f32),
+                         *(t.data_ptr() for t in res))
+        self.ctx.check(self.lib.ds_cuda_tree_verify_dev(self.ctx.h, d, self._stream()), "tree_verify")
         return res
 
     def _results(self, b, n):
@@ -258,21 +262,15 @@ class Speculative:
         if first.dim() != 5 or first.element_size() != 2:
             raise ValueError("caches: expected 16-bit [layers x batch x n_kv_heads x kv_max x head_dim]")
         layers, _, kv, cap, hd = first.shape
-        d = TreeCommitDesc()
-        d.n_tensors, d.layers, d.batch, d.n_nodes, d.n_kv_heads, d.head_dim, d.kv_max = (len(caches), layers, b, n, kv,
-                                                                                         hd, cap)
-        for i, (c, t) in enumerate(zip(caches, trees)):
-            d.cache[i] = self._want("cache", c, (layers, b, kv, cap, hd), first.dtype, False)
-            d.tree[i] = self._want("tree", t, (layers, b, kv, n, hd), first.dtype, False)
-            cs, ts = c.stride(), t.stride()
-            if cs[4] != 1 or ts[4] != 1:
-                raise ValueError("commit: the head dimension must be contiguous")
-            d.cache_stride[i][:] = cs[:4]
-            d.tree_stride[i][:] = ts[:4]
-        d.lens = self._want("lens", lens, (b,), torch.int32)
-        d.path = self._want("path", path, (b, n), torch.int32)
-        d.accepted = self._want("accepted", accepted, (b,), torch.int32)
-        new = torch.empty(b, dtype=torch.int32, device=self.device)
-        d.new_lens = new.data_ptr()
-        self.ctx.check(self.lib.ds_cuda_tree_commit_dev(self.ctx.h, ctypes.byref(d), self._stream()), "tree_commit")
+        m, shape, rows, dt = len(caches), (layers, b, kv, cap, hd), (layers, b, kv, n, hd), first.dtype
+        i32 = torch.int32
+        cp, cs, tp, ts = [0] * 8, [0] * 32, [0] * 8, [0] * 32
+        for i in range(m):
+            cp[i], cs[4 * i:4 * i + 4] = self._strided("cache", caches[i], shape, dt)
+            tp[i], ts[4 * i:4 * i + 4] = self._strided("tree", trees[i], rows, dt)
+        new = torch.empty(b, dtype=i32, device=self.device)
+        d = _pack_commit(m, layers, b, n, kv, hd, cap, *cp, *cs, *tp, *ts, self._want("lens", lens, (b,), i32),
+                         self._want("path", path, (b, n), i32), self._want("accepted", accepted, (b,), i32),
+                         new.data_ptr())
+        self.ctx.check(self.lib.ds_cuda_tree_commit_dev(self.ctx.h, d, self._stream()), "tree_commit")
         return new
