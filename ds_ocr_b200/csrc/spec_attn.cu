@@ -5,7 +5,7 @@
 // together, so K and V are read once for all of them. The keys of a
 // (sequence, key head, row tile) item come in tiles of KT: first the cached
 // rows, then the tree's nodes. All items' tiles form one list, cut into equal
-// runs, one per CTA (one persistent CTA per SM, two for head_dim 64): a
+// runs, one per CTA (two persistent CTAs an SM, up to four for head_dim 64): a
 // ragged batch and a single long sequence are spread alike, and nothing
 // about the lengths is needed on the host. A run that covers an item writes
 // its result; an item cut between CTAs leaves (max, sum, weighted V) parts
@@ -21,9 +21,10 @@
 namespace ds {
 
 constexpr int SA_MAX_NODES = 256;
-constexpr int SA_THREADS = 256;
+constexpr int SA_THREADS = 128;
 constexpr int SA_WARPS = SA_THREADS / 32;
 constexpr int SA_STAGES = 3;
+constexpr int SA_MAX_CTAS = 4;  // resident CTAs an SM
 
 struct SaArgs {
     ds_cuda_tree_attention_t d;
@@ -31,7 +32,8 @@ struct SaArgs {
     int group;      // query heads per key head
     int rows;       // n_nodes * group
     int row_tiles;  // ceil(rows / row tile)
-    int ctas;       // runs the tile list is cut into, at most
+    int per_seq;    // n_kv_heads * row_tiles: items of a sequence
+    int sms, ctas;  // SMs; runs the tile list is cut into, at most
     float scale2;   // scale * log2(e)
     float *part;    // workspace: [ctas][2][row tile][head_dim], then ...
     float2 *ml;     // ... [ctas][2][row tile] (max in log2 units, sum)
@@ -51,34 +53,45 @@ __device__ __forceinline__ SaSeq sa_seq(const ds_cuda_tree_attention_t &d, int b
     return s;
 }
 // Sums the sequences' tiles over the batch: returns the total, *mine the
-// tiles before this thread's run of sequences [b0, b1).
-template <int KT>
-__device__ __forceinline__ long long sa_scan(const SaArgs &a, int b0, int b1, long long *sh, long long *mine) {
+// tiles before this thread's run of sequences [b0, b1). (The host refuses
+// what could pass 2^31 tiles.)
+template <int KT, int WARPS>
+__device__ __forceinline__ int sa_scan(const SaArgs &a, int b0, int b1, int *sh, int *mine) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = a.d.n_kv_heads * a.row_tiles;
-    long long s = 0;
-    for (int b = b0; b < b1; b++) s += (long long)sa_seq<KT>(a.d, b).tiles * per;
-    long long v = s;
+    int s = 0;
+    for (int b = b0; b < b1; b++) s += sa_seq<KT>(a.d, b).tiles * a.per_seq;
+    int v = s;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(DS_FULL, v, o);
+        const int u = __shfl_up_sync(DS_FULL, v, o);
         if (lane >= o) v += u;
     }
     if (lane == 31) sh[warp] = v;
     __syncthreads();
-    long long before = 0, total = 0;
+    int before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < SA_WARPS; w++) {
+    for (int w = 0; w < WARPS; w++) {
         if (w < warp) before += sh[w];
         total += sh[w];
     }
     *mine = before + v - s;
     return total;
 }
-__device__ __forceinline__ long long sa_start(long long c, long long total, long long ctas) { return c * total / ctas; }
-__device__ __forceinline__ int sa_cta_of(long long x, long long total, long long ctas) {
-    return (int)(((x + 1) * ctas - 1) / total);
-}
+// The list cut into `ctas` runs whose lengths differ by one at most, the
+// longer ones first.
+struct SaCut {
+    int ctas, len, more;
+    __device__ __forceinline__ SaCut(int total, int most) {
+        ctas = min(most, total);
+        len = total / ctas;
+        more = total - len * ctas;
+    }
+    __device__ __forceinline__ int start(int c) const { return c * len + min(c, more); }
+    __device__ __forceinline__ int cta_of(int x) const {
+        const int head = more * (len + 1);
+        return x < head ? x / (len + 1) : more + (x - head) / len;
+    }
+};
 
 // ---- loads and matrix instructions -----------------------------------------
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
@@ -146,68 +159,138 @@ __device__ __forceinline__ void sa_store4(const ds_cuda_tree_attention_t &d, int
             make_uint2(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]));
 }
 
+// A part (weighted V u, sum l, factor f) added to (v, ll).
+__device__ __forceinline__ void sa_add(float (&v)[4], float &ll, float4 u, float l, float f) {
+    ll += l * f;
+    v[0] += u.x * f;
+    v[1] += u.y * f;
+    v[2] += u.z * f;
+    v[3] += u.w * f;
+}
+// Dimensions [c, c + 4) of a row's result, from its maximum, sum and weighted V.
+__device__ __forceinline__ void sa_finish(const SaArgs &a, int b, int g, int row, int cnt, int c, float m, float l,
+                                          float (&v)[4]) {
+    const ds_cuda_tree_attention_t &d = a.d;
+    const int nd = row / a.group, head = g * a.group + row % a.group;
+    const bool none = nd >= cnt || l == 0.f;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = none ? 0.f : v[k] * inv;
+    sa_store4(d, b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c, v);
+    if (d.lse && c == 0)
+        d.lse[((size_t)b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718f;
+}
+
+// ---- clusters ----------------------------------------------------------------
+__device__ __forceinline__ int cluster_rank() {
+    int r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ int cluster_ctas() {
+    int r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// CTA k's copy of a shared variable.
+__device__ __forceinline__ uint32_t cluster_addr(const void *p, int k) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(k));
+    return r;
+}
+__device__ __forceinline__ float2 cluster_ld2(const float2 *p, int k) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr(p, k)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_ld4(const float4 *p, int k) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr(p, k)) : "memory");
+    return v;
+}
+
 // Shapes of one instantiation. QP planes of the queries and of the weights
-// (F32: three, all 24 bits; 16-bit types: one), PL planes of K and V. Eight
-// warps: MT row tiles of 16 times KS slices of KW keys.
+// (F32: three, all 24 bits; 16-bit types: one), PL planes of K and V. Four
+// warps: MT row tiles of 16 times KS slices of KW keys. The CTAs are small,
+// two to four an SM, so that one's loads, products and softmax run beside
+// another's.
 template <int HD_, int MT_, int PL_, int QT_> struct SaShape {
     static constexpr int HD = HD_, MT = MT_, PL = PL_, QT = QT_;
     static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
     static constexpr int RT = 16 * MT;
-    static constexpr int KT = PL == 2 ? 64 : 128;  // a stage is 64 KB (32 KB for head_dim 64) either way
+    static constexpr int KT = PL == 2 ? 32 : 64;  // a stage is 32 KB (16 KB for head_dim 64) either way
     static constexpr int KS = SA_WARPS / MT, KW = KT / KS, NT = KW / 8;
     static constexpr int PLANE = KT * HD * 2, STAGE = 2 * PL * PLANE;
     static constexpr int QPLANE = RT * HD * 2;
     static constexpr int SMEM = SA_STAGES * STAGE + QP * QPLANE;
-    static constexpr int MINB = HD == 64 ? 2 : 1;
+    static constexpr int FIT = (226 << 10) / (SMEM + 3072);  // by shared memory
+    static constexpr int PER_SM = FIT < SA_MAX_CTAS ? FIT : SA_MAX_CTAS;
 };
 
-template <class S>
-__global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_constant__ SaArgs a) {
+// CLUSTER: an item is shared by one cluster, its tiles cut into the CTAs'
+// runs, and joined through their shared memory.
+template <class S, bool CLUSTER>
+__global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_constant__ SaArgs a) {
     constexpr int HD = S::HD, KT = S::KT, NT = S::NT, KW = S::KW, CH = HD / 8;
     constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16, F32 = S::QT == DS_CUDA_SPEC_F32;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ long long sh_scan[SA_WARPS];
-    __shared__ long long sh_off;
-    __shared__ int sh_b;
+    __shared__ int sh_scan[SA_WARPS], sh_off, sh_b;
     __shared__ float2 sh_ml[SA_WARPS][16];
-    __shared__ uint64_t sh_mask[2][S::RT][KT / 64];  // by tile parity
+    __shared__ uint64_t sh_mask[2][S::RT];  // by tile parity
+    // a cluster's part: over the first stage, unused by then
+    float4 *const sh_part = reinterpret_cast<float4 *>(smem);
+    float2 *const sh_pml = reinterpret_cast<float2 *>(smem + S::RT * HD * 4);
     const ds_cuda_tree_attention_t &d = a.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int mt = warp % S::MT, ks = warp / S::MT;
     const uint32_t q_s = smem_u32(smem) + SA_STAGES * S::STAGE;
-    pdl_launch();
-
-    // this CTA's run of the tile list
-    const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
-    const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
-    long long at;
-    const long long total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
-    const long long ctas = min((long long)a.ctas, total);
-    if (blockIdx.x >= ctas) return;
-    const long long first = sa_start(blockIdx.x, total, ctas), last = sa_start(blockIdx.x + 1, total, ctas);
-    for (int b = b0; b < b1; b++) {
-        const long long n = (long long)sa_seq<KT>(d, b).tiles * d.n_kv_heads * a.row_tiles;
-        if (at <= first && first < at + n) {
-            sh_b = b;
-            sh_off = first - at;
-        }
-        at += n;
-    }
-    __syncthreads();
 
     struct Cursor {
         int b, g, rt, t;
         SaSeq s;
     } ld, cu;
-    {
+    int tiles;  // of this CTA's run
+    if (CLUSTER) {
+        cluster_arrive();
+        const int item = blockIdx.x / cluster_ctas(), rank = cluster_rank();
+        ld.b = item / a.per_seq;
+        ld.rt = item % a.row_tiles;
+        ld.g = item % a.per_seq / a.row_tiles;
+        ld.s = sa_seq<KT>(d, ld.b);
+        const SaCut cut(ld.s.tiles, cluster_ctas());
+        ld.t = rank < cut.ctas ? cut.start(rank) : 0;
+        tiles = rank < cut.ctas ? cut.start(rank + 1) - ld.t : 0;
+    } else {
+        pdl_launch();
+        const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
+        const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
+        int at;
+        const int total = sa_scan<KT, SA_WARPS>(a, b0, b1, sh_scan, &at);
+        const SaCut cut(total, a.ctas);
+        if ((int)blockIdx.x >= cut.ctas) return;
+        const int first = cut.start(blockIdx.x);
+        tiles = cut.start(blockIdx.x + 1) - first;
+        for (int b = b0; b < b1; b++) {
+            const int n = sa_seq<KT>(d, b).tiles * a.per_seq;
+            if (at <= first && first < at + n) {
+                sh_b = b;
+                sh_off = first - at;
+            }
+            at += n;
+        }
+        __syncthreads();
         ld.b = sh_b;
         ld.s = sa_seq<KT>(d, ld.b);
-        const int off = (int)(sh_off / ld.s.tiles);
-        ld.t = (int)(sh_off % ld.s.tiles);
+        const int off = sh_off / ld.s.tiles;
+        ld.t = sh_off - off * ld.s.tiles;
         ld.rt = off % a.row_tiles;
         ld.g = off / a.row_tiles;
     }
     cu = ld;
+    const int item_b = ld.b, item_g = ld.g, item_rt = ld.rt, item_tiles = ld.s.tiles, cnt = ld.s.cnt;  // CLUSTER's one item
     auto next = [&](Cursor &c) {
         if (++c.t < c.s.tiles) return;
         c.t = 0;
@@ -254,7 +337,6 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
                 }
     };
 
-    const long long tiles = last - first;
 #pragma unroll
     for (int i = 0; i < SA_STAGES - 1; i++) {
         if (i < tiles) {
@@ -268,7 +350,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
     bool fresh = true;          // the item's queries are not in shared memory yet
     bool whole = cu.t == 0;     // this CTA has the item from its first tile
     int st = 0, fill = SA_STAGES - 1;
-    for (long long i = 0; i < tiles; i++) {
+    for (int i = 0; i < tiles; i++) {
         cp_wait<SA_STAGES - 2>();
         if (fresh) {  // (the previous item's readers of these are past the last barrier of its end)
             fresh = false;
@@ -307,14 +389,13 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
         const int r0 = (node ? cu.t - cu.s.cache_tiles : cu.t) * KT;
         const int valid = (node ? cu.s.cnt : cu.s.len) - r0;
         if (node)
-            for (int x = tid; x < S::RT * (KT / 64); x += SA_THREADS) {
-                const int r = x / (KT / 64), w = x % (KT / 64), row = cu.rt * S::RT + r, nd = row / a.group;
-                const int word = r0 / 64 + w, left = cu.s.cnt - 64 * word;
-                uint64_t bits = 0;
-                if (row < a.rows && nd < cu.s.cnt && left > 0)
-                    bits = d.mask[((size_t)cu.b * d.n_nodes + nd) * a.words + word] &
-                           (left < 64 ? (1ull << left) - 1 : ~0ull);
-                sh_mask[i & 1][r][w] = bits;
+            for (int r = tid; r < S::RT; r += SA_THREADS) {
+                const int row = cu.rt * S::RT + r, nd = row / a.group;
+                uint64_t bits = 0;  // KT <= 64 and r0 is a multiple of KT: within one word
+                if (row < a.rows && nd < cu.s.cnt && valid > 0)
+                    bits = d.mask[((size_t)cu.b * d.n_nodes + nd) * a.words + r0 / 64] >> (r0 & 63) &
+                           (valid < 64 ? (1ull << valid) - 1 : ~0ull);
+                sh_mask[i & 1][r] = bits;
             }
         __syncthreads();
         if (i + SA_STAGES - 1 < tiles) {
@@ -325,14 +406,15 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
         fill = fill + 1 == SA_STAGES ? 0 : fill + 1;
 
         const uint32_t k_s = smem_u32(smem) + st * S::STAGE, v_s = k_s + S::PL * S::PLANE;
-        // scores of 16 rows and KW keys; the products of lower planes apart
-        float s[NT][4], s2[F32 ? NT : 1][4];
+        // scores of 16 rows and KW keys; the planes' products of each order of
+        // magnitude apart (shorter chains, smaller rounding)
+        float s[NT][4], low[F32 ? NT : 1][2][4];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 s[n][e] = 0.f;
-                if (F32) s2[n][e] = 0.f;
+                if (F32) low[n][0][e] = low[n][1][e] = 0.f;
             }
         const int qr = 16 * mt + (lane & 15), qc = lane >> 4;
         if (NT == 1) {
@@ -351,7 +433,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
 #pragma unroll
                         for (int pk = 0; pk < S::PL; pk++)
                             if (pq + pk < 3)
-                                mma16<F16>(pq + pk ? s2[0] : s[0], qf[h][pq], kf[pk][2 * h], kf[pk][2 * h + 1]);
+                                mma16<F16>(pq + pk ? low[0][(pq + pk + 1) & 1] : s[0], qf[h][pq], kf[pk][2 * h], kf[pk][2 * h + 1]);
                 }
             }
         } else {
@@ -369,10 +451,11 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
                         ldsm4(kf, k_s + pk * S::PLANE + sw<HD>(kr + 8 * n, 2 * kk + kc));
 #pragma unroll
                         for (int pq = 0; pq < S::QP; pq++)
-                            if (pq + pk < 3) {
-                                mma16<F16>(pq + pk ? s2[F32 ? n : 0] : s[n], qf[pq], kf[0], kf[1]);
-                                mma16<F16>(pq + pk ? s2[F32 ? n + 1 : 0] : s[n + 1], qf[pq], kf[2], kf[3]);
-                            }
+                            if (pq + pk < 3)
+#pragma unroll
+                                for (int x = 0; x < 2; x++)
+                                    mma16<F16>(pq + pk ? low[F32 ? n + x : 0][(pq + pk + 1) & 1] : s[n + x], qf[pq],
+                                               kf[2 * x], kf[2 * x + 1]);
                     }
                 }
             }
@@ -381,7 +464,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[n][e] += s2[n][e];
+                for (int e = 0; e < 4; e++) s[n][e] += low[n][0][e] + low[n][1][e];
 
         // running maximum (of the scaled scores, in log2 units), weights, sums
         const bool masked = node || valid < KT;
@@ -390,7 +473,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
             const int key = ks * KW;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                if (node) see[h] = sh_mask[i & 1][16 * mt + (lane >> 2) + 8 * h][key >> 6] >> (key & 63);
+                if (node) see[h] = sh_mask[i & 1][16 * mt + (lane >> 2) + 8 * h] >> key;
                 else see[h] = valid - key >= 64 ? ~0ull : valid > key ? (1ull << (valid - key)) - 1 : 0;
             }
         }
@@ -453,7 +536,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const int r = 16 * mt + (lane >> 2) + 8 * h;
-                        if (!((sh_mask[i & 1][r][key >> 6] >> (key & 63)) & 1)) continue;
+                        if (!((sh_mask[i & 1][r] >> key) & 1)) continue;
 #pragma unroll
                         for (int c = 0; c < CH; c++)
 #pragma unroll
@@ -545,9 +628,11 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
         if (end || i + 1 == tiles) {
             // the item, or this CTA's part of it, is done: the warps' parts
             // are joined through this stage, which is free until the next
-            // iteration's barrier
+            // iteration's barrier (a cluster's run ends here: every stage is
+            // free, and the join goes from the second into the first)
             __syncthreads();
-            float *so = reinterpret_cast<float *>(smem + st * S::STAGE) + warp * 16 * HD;
+            const float *parts = reinterpret_cast<const float *>(smem + (CLUSTER ? 1 : st) * S::STAGE);
+            float *so = const_cast<float *>(parts) + warp * 16 * HD;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 l[h] += __shfl_xor_sync(DS_FULL, l[h], 1);
@@ -560,7 +645,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
                 }
             }
             __syncthreads();
-            const bool alone = end && whole;
+            const bool alone = end && whole && !CLUSTER;
             const int slot = whole ? 1 : 0;
             for (int x = tid; x < S::RT * (HD / 4); x += SA_THREADS) {
                 const int r = x / (HD / 4), c = 4 * (x % (HD / 4)), t16 = r >> 4, rr = r & 15;
@@ -570,28 +655,17 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
 #pragma unroll
                 for (int w = 0; w < S::KS; w++) {
                     const float2 ml = sh_ml[w * S::MT + t16][rr];
-                    const float f = ex2(ml.x - mm);
-                    const float4 u = *reinterpret_cast<const float4 *>(
-                        reinterpret_cast<const float *>(smem + st * S::STAGE) + (w * S::MT + t16) * 16 * HD + rr * HD +
-                        (c ^ ((rr & 3) << 3)));
-                    ll += ml.y * f;
-                    v[0] += u.x * f;
-                    v[1] += u.y * f;
-                    v[2] += u.z * f;
-                    v[3] += u.w * f;
+                    const float4 u = *reinterpret_cast<const float4 *>(parts + ((w * S::MT + t16) * 16 + rr) * HD +
+                                                                       (c ^ ((rr & 3) << 3)));
+                    sa_add(v, ll, u, ml.y, ex2(ml.x - mm));
                 }
                 const int row = cu.rt * S::RT + r;
                 if (row >= a.rows) continue;
-                if (alone) {
-                    const int nd = row / a.group, head = cu.g * a.group + row % a.group;
-                    const bool none = nd >= cu.s.cnt || ll == 0.f;
-                    const float inv = 1.f / ll;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = none ? 0.f : v[k] * inv;
-                    sa_store4(d, cu.b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c, v);
-                    if (d.lse && c == 0)
-                        d.lse[((size_t)cu.b * d.n_nodes + nd) * d.n_heads + head] =
-                            none ? -INFINITY : (mm + log2f(ll)) * 0.69314718f;
+                if (CLUSTER) {
+                    sh_part[r * (HD / 4) + c / 4] = make_float4(v[0], v[1], v[2], v[3]);
+                    if (c == 0) sh_pml[r] = make_float2(mm, ll);
+                } else if (alone) {
+                    sa_finish(a, cu.b, cu.g, row, cu.s.cnt, c, mm, ll, v);
                 } else {
                     const size_t pr = ((size_t)blockIdx.x * 2 + slot) * S::RT + r;
                     *reinterpret_cast<float4 *>(a.part + pr * HD + c) = make_float4(v[0], v[1], v[2], v[3]);
@@ -606,113 +680,154 @@ __global__ void __launch_bounds__(SA_THREADS, S::MINB) sa_kernel(const __grid_co
         st = st + 1 == SA_STAGES ? 0 : st + 1;
     }
     cp_wait<0>();
+    if (CLUSTER) {
+        __syncwarp();
+        cluster_wait();  // (the arrival at the start)
+        cluster_arrive();
+        cluster_wait();  // every CTA's part is in its shared memory
+        const int n = cluster_ctas(), used = min(n, item_tiles), left = min(S::RT, a.rows - item_rt * S::RT);
+        for (int x = cluster_rank() * SA_THREADS + tid; x < left * (HD / 4); x += n * SA_THREADS) {
+            const int r = x / (HD / 4);
+            float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < used; k++) mm = fmaxf(mm, cluster_ld2(&sh_pml[r], k).x);
+            for (int k = 0; k < used; k++) {
+                const float2 ml = cluster_ld2(&sh_pml[r], k);
+                sa_add(v, ll, cluster_ld4(&sh_part[x], k), ml.y, ex2(ml.x - mm));
+            }
+            sa_finish(a, item_b, item_g, item_rt * S::RT + r, cnt, 4 * (x % (HD / 4)), mm, ll, v);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();  // no CTA leaves while another reads its part
+    }
 }
 
-// The items that several CTAs had parts of: one warp per row, the parts in
-// list order.
+// The items that several CTAs had parts of: HD / 4 threads per row, the parts
+// in list order.
 template <class S>
 __global__ void __launch_bounds__(SA_THREADS) sa_join_kernel(const __grid_constant__ SaArgs a) {
-    constexpr int HD = S::HD, KT = S::KT, PL = HD / 32;
-    __shared__ long long sh_scan[SA_WARPS];
-    __shared__ long long sh_off;
+    constexpr int HD = S::HD, KT = S::KT;
+    __shared__ int sh_scan[SA_WARPS], sh_off;
     const ds_cuda_tree_attention_t &d = a.d;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int b = blockIdx.y, item = blockIdx.x / (S::RT / SA_WARPS);
-    const int r = blockIdx.x % (S::RT / SA_WARPS) * SA_WARPS + warp;
+    const int tid = threadIdx.x, b = blockIdx.y;
+    const int x = blockIdx.x * SA_THREADS + tid, item = x / (S::RT * (HD / 4)), r = x / (HD / 4) % S::RT, c = 4 * (x % (HD / 4));
     const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
     const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
-    long long at;
-    const long long total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
+    int at;
+    const int total = sa_scan<KT, SA_WARPS>(a, b0, b1, sh_scan, &at);
     if (b0 <= b && b < b1) {
-        for (int x = b0; x < b; x++) at += (long long)sa_seq<KT>(d, x).tiles * d.n_kv_heads * a.row_tiles;
+        for (int y = b0; y < b; y++) at += sa_seq<KT>(d, y).tiles * a.per_seq;
         sh_off = at;
     }
     const SaSeq s = sa_seq<KT>(d, b);
     __syncthreads();
-    const long long ctas = min((long long)a.ctas, total), x0 = sh_off + (long long)item * s.tiles;
-    const int c0 = sa_cta_of(x0, total, ctas), c1 = sa_cta_of(x0 + s.tiles - 1, total, ctas);
-    const int rt = item % a.row_tiles, g = item / a.row_tiles, row = rt * S::RT + r;
+    const SaCut cut(total, a.ctas);
+    const int x0 = sh_off + item * s.tiles, c0 = cut.cta_of(x0), c1 = cut.cta_of(x0 + s.tiles - 1);
+    const int row = item % a.row_tiles * S::RT + r;
     pdl_wait();
     if (c0 == c1 || row >= a.rows) return;
-    float m = -__FLT_MAX__, l = 0.f, o[PL] = {};
-    for (int c = c0; c <= c1; c += 8) {
+    float m = -__FLT_MAX__, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = c0; k0 <= c1; k0 += 8) {
         float2 ml[8];
-        float v[8][PL];
+        float4 v[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const int cc = min(c + k, c1);
+            const int cc = min(k0 + k, c1);
             const size_t pr = ((size_t)cc * 2 + (cc == c0)) * S::RT + r;
             ml[k] = a.ml[pr];
-            if (PL == 4) {
-                const float4 u = *reinterpret_cast<const float4 *>(a.part + pr * HD + lane * 4);
-                v[k][0] = u.x, v[k][1] = u.y, v[k][PL - 2] = u.z, v[k][PL - 1] = u.w;
-            } else {
-                const float2 u = *reinterpret_cast<const float2 *>(a.part + pr * HD + lane * 2);
-                v[k][0] = u.x, v[k][1] = u.y;
-            }
+            v[k] = *reinterpret_cast<const float4 *>(a.part + pr * HD + c);
         }
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            if (c + k > c1) break;
-            const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn), e = ex2(ml[k].x - mn);
+            if (k0 + k > c1) break;
+            const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn);
             m = mn;
-            l = l * f + ml[k].y * e;
+            l *= f;
 #pragma unroll
-            for (int x = 0; x < PL; x++) o[x] = o[x] * f + v[k][x] * e;
+            for (int e = 0; e < 4; e++) o[e] *= f;
+            sa_add(o, l, v[k], ml[k].y, ex2(ml[k].x - mn));
         }
     }
-    const int nd = row / a.group, head = g * a.group + row % a.group;
-    const bool none = nd >= s.cnt || l == 0.f;
-    const float inv = 1.f / l;
-    const int64_t oo = b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + lane * PL;
-#pragma unroll
-    for (int x = 0; x < PL; x++) o[x] = none ? 0.f : o[x] * inv;
-    if (d.type == DS_CUDA_SPEC_F32) {
-#pragma unroll
-        for (int x = 0; x < PL; x += 2)
-            *reinterpret_cast<float2 *>((float *)d.out + oo + x) = make_float2(o[x], o[x + 1]);
-    } else {
-#pragma unroll
-        for (int x = 0; x < PL; x += 2)
-            *reinterpret_cast<uint32_t *>((uint16_t *)d.out + oo + x) =
-                d.type == DS_CUDA_SPEC_F16 ? pack2<true>(o[x], o[x + 1]) : pack2<false>(o[x], o[x + 1]);
-    }
-    if (d.lse && lane == 0)
-        d.lse[((size_t)b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718f;
+    sa_finish(a, b, item / a.row_tiles, row, s.cnt, c, m, l, o);
 }
 
-template <class S> static cudaError_t sa_run(SaArgs a, int device, cudaStream_t st) {
-    static std::atomic<uint64_t> ready;  // devices (of the first 64) whose attribute is set
-    if (device >= 64 || !(ready.load() >> device & 1)) {
-        const cudaError_t e = cudaFuncSetAttribute(sa_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+constexpr int SA_CLUSTER = 16;
+
+// Calls whose items are few enough for a cluster each in one wave, with at
+// most 8 tiles a CTA, are joined in the clusters: one launch, no workspace.
+// Their tiles are bounded by the cache's room, the lengths not being known
+// here. Others take the list.
+template <class S> static bool sa_clusters(const ds_cuda_tree_attention_t *d, int items, int sms) {
+    const long long tiles = (d->kv_max + S::KT - 1) / S::KT + (d->n_nodes + S::KT - 1) / S::KT;
+    return (long long)items * SA_CLUSTER <= sms * S::PER_SM && tiles <= 8 * SA_CLUSTER;
+}
+
+template <class S> struct SaRun {
+    static bool clusters(const SaArgs &a) { return sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
+    static size_t workspace(const SaArgs &a) {
+        // two parts a CTA, then their maxima and sums
+        return clusters(a) ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
+    }
+    template <bool CLUSTER> static cudaError_t attributes(int device) {
+        static std::atomic<uint64_t> ready;  // devices (of the first 64) that have them
+        if (device < 64 && ready.load() >> device & 1) return cudaSuccess;
+        cudaError_t e = cudaFuncSetAttribute(sa_kernel<S, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e == cudaSuccess && CLUSTER)
+            e = cudaFuncSetAttribute(sa_kernel<S, CLUSTER>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess && device < 64) ready.fetch_or(1ull << device);
+        return e;
+    }
+    static cudaError_t run(SaArgs a, int device, cudaStream_t st) {
+        void *args[] = {&a};
+        if (clusters(a)) {
+            const cudaError_t e = attributes<true>(device);
+            if (e != cudaSuccess) return e;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(a.d.batch * a.per_seq * SA_CLUSTER);
+            cfg.blockDim = dim3(SA_THREADS);
+            cfg.dynamicSmemBytes = S::SMEM;
+            cfg.stream = st;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = SA_CLUSTER;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            return cudaLaunchKernelExC(&cfg, (const void *)sa_kernel<S, true>, args);
+        }
+        a.ctas = a.sms * S::PER_SM;
+        a.part = (float *)a.d.workspace;
+        a.ml = (float2 *)(a.part + (size_t)a.ctas * 2 * S::RT * S::HD);
+        cudaError_t e = attributes<false>(device);
         if (e != cudaSuccess) return e;
-        if (device < 64) ready.fetch_or(1ull << device);
+        sa_kernel<S, false><<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        return launch_ex((const void *)sa_join_kernel<S>, dim3(a.per_seq * (S::RT * (S::HD / 4) / SA_THREADS), a.d.batch),
+                         dim3(SA_THREADS), 0, st, true, args);
     }
-    sa_kernel<S><<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    void *args[] = {&a};
-    return launch_ex((const void *)sa_join_kernel<S>,
-                     dim3(a.d.n_kv_heads * a.row_tiles * (S::RT / SA_WARPS), a.d.batch), dim3(SA_THREADS), 0, st, true, args);
-}
+};
 
-// The row tile: up to 64 rows, or 32 with F32 queries, whose three planes
-// take the shared memory.
-static int sa_row_tile(const ds_cuda_tree_attention_t *d) {
+// f(instantiation) for a call. The row tile: up to 64 rows, or 32 with F32
+// queries, whose three planes take the shared memory.
+template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, F f) {
+    constexpr int B = DS_CUDA_SPEC_BF16, H = DS_CUDA_SPEC_F16, P = DS_CUDA_SPEC_F32;
     const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
-    return rows <= 16 ? 16 : rows <= 32 || d->type == DS_CUDA_SPEC_F32 ? 32 : 64;
+    if (d->type == P) {
+        const bool two = d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo;
+        if (two) return rows <= 16 ? f(SaRun<SaShape<HD, 1, 2, P>>()) : f(SaRun<SaShape<HD, 2, 2, P>>());
+        return rows <= 16 ? f(SaRun<SaShape<HD, 1, 1, P>>()) : f(SaRun<SaShape<HD, 2, 1, P>>());
+    }
+    if (d->type == H)
+        return rows <= 16   ? f(SaRun<SaShape<HD, 1, 1, H>>())
+               : rows <= 32 ? f(SaRun<SaShape<HD, 2, 1, H>>()) : f(SaRun<SaShape<HD, 4, 1, H>>());
+    return rows <= 16   ? f(SaRun<SaShape<HD, 1, 1, B>>())
+           : rows <= 32 ? f(SaRun<SaShape<HD, 2, 1, B>>()) : f(SaRun<SaShape<HD, 4, 1, B>>());
 }
-
-template <int HD> static cudaError_t sa_pick(const SaArgs &a, bool two, int rt, int dev, cudaStream_t st) {
-    constexpr int B = DS_CUDA_SPEC_BF16, H = DS_CUDA_SPEC_F16, F = DS_CUDA_SPEC_F32;
-    if (a.d.type == F && two) return rt == 16 ? sa_run<SaShape<HD, 1, 2, F>>(a, dev, st) : sa_run<SaShape<HD, 2, 2, F>>(a, dev, st);
-    if (a.d.type == F) return rt == 16 ? sa_run<SaShape<HD, 1, 1, F>>(a, dev, st) : sa_run<SaShape<HD, 2, 1, F>>(a, dev, st);
-    if (a.d.type == H)
-        return rt == 16 ? sa_run<SaShape<HD, 1, 1, H>>(a, dev, st)
-               : rt == 32 ? sa_run<SaShape<HD, 2, 1, H>>(a, dev, st) : sa_run<SaShape<HD, 4, 1, H>>(a, dev, st);
-    return rt == 16 ? sa_run<SaShape<HD, 1, 1, B>>(a, dev, st)
-           : rt == 32 ? sa_run<SaShape<HD, 2, 1, B>>(a, dev, st) : sa_run<SaShape<HD, 4, 1, B>>(a, dev, st);
+template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, F f) {
+    return d->head_dim == 64 ? sa_pick_hd<64>(d, f) : sa_pick_hd<128>(d, f);
 }
+template <class S> static S sa_shape(SaRun<S>) { return S(); }
 
 // One CTA per sequence, one thread per node: a node's word bits are set by
 // walking up its parents (kept in shared memory; at most n_nodes steps).
@@ -757,17 +872,29 @@ static int sa_check(ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
                         d->batch, d->n_nodes, d->n_heads, d->n_kv_heads, d->head_dim, d->kv_max, SA_MAX_NODES);
     if (d->batch > 65535 || d->n_heads > 65535)
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: batch and n_heads are at most 65535");
+    if ((double)d->batch * d->n_heads * d->n_nodes * (d->kv_max / 32.0 + 16) >= 2147483648.0)
+        return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: more than 2^31 tiles");
     return DS_CUDA_OK;
 }
 
-static int sa_ctas(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
-    return c->sm_count * (d->head_dim == 64 ? 2 : 1);
+static SaArgs sa_args(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
+    SaArgs a = {};
+    a.d = *d;
+    a.words = (d->n_nodes + 63) / 64;
+    a.group = d->n_heads / d->n_kv_heads;
+    a.rows = d->n_nodes * a.group;
+    const int rt = sa_pick(d, [](auto r) { return decltype(sa_shape(r))::RT; });
+    a.row_tiles = (a.rows + rt - 1) / rt;
+    a.per_seq = d->n_kv_heads * a.row_tiles;
+    a.sms = c->sm_count;
+    a.scale2 = d->scale * 1.44269504f;
+    return a;
 }
 
 extern "C" size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d) {
     if (!c || !c->ok || sa_check(nullptr, d) < 0) return 0;
-    // two parts a CTA, each of at most 64 rows with their maxima and sums
-    return sa_ctas(c, d) * (size_t)2 * 64 * (d->head_dim * 4 + 8);
+    const SaArgs a = sa_args(c, d);
+    return sa_pick(d, [&](auto r) { return decltype(r)::workspace(a); });
 }
 
 extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d, void *stream) {
@@ -794,24 +921,13 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
         if (t.lo && d->type != DS_CUDA_SPEC_F32)
             return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: %s has a lo plane, which only the F32 type takes", t.name);
     }
-    const size_t need = ds_cuda_tree_attention_workspace(c, d);
-    if (!d->workspace || d->workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->workspace) & 255))
+    const SaArgs a = sa_args(c, d);
+    const size_t need = sa_pick(d, [&](auto r) { return decltype(r)::workspace(a); });
+    if (need && (!d->workspace || d->workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->workspace) & 255)))
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: workspace of %zu bytes, 256-byte aligned, wanted", need);
-    const bool two = d->type == DS_CUDA_SPEC_F32 && (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo);
-    const int rt = sa_row_tile(d);
-    SaArgs a = {};
-    a.d = *d;
-    a.words = (d->n_nodes + 63) / 64;
-    a.group = d->n_heads / d->n_kv_heads;
-    a.rows = d->n_nodes * a.group;
-    a.row_tiles = (a.rows + rt - 1) / rt;
-    a.ctas = sa_ctas(c, d);
-    a.scale2 = d->scale * 1.44269504f;
-    a.part = (float *)d->workspace;
-    a.ml = (float2 *)(a.part + (size_t)a.ctas * 2 * rt * d->head_dim);
     cudaSetDevice(c->device);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    const cudaError_t e = d->head_dim == 64 ? sa_pick<64>(a, two, rt, c->device, st) : sa_pick<128>(a, two, rt, c->device, st);
+    const cudaError_t e = sa_pick(d, [&](auto r) { return decltype(r)::run(a, c->device, st); });
     return ctx_cuda(c, e, "tree_attention launch");
 }
 

@@ -88,44 +88,51 @@ class Speculative:
         self._index = self.ctx.device
         self._types = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
         self._workspace = {}  # bytes by sizes
+        # the handle alone, without the Stream object (2 us) around it
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
 
     def _stream(self):
         # torch's default stream is the legacy stream (handle 0), which the C
         # ABI would take for the context's own: cudaStreamLegacy is handle 1
-        return self.torch.cuda.current_stream(self.device).cuda_stream or 1
+        return self._raw_stream(self._index) or 1
 
-    def _want(self, name, t, shape, dtype, contiguous=True):
-        """The address of a tensor that has to be as given."""
+    def _refuse(self, name, t, shape, dtype, why):
         if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index:
-            raise ValueError(f"{name}: expected {dtype} {tuple(shape)} on {self.device}, got {t.dtype} "
-                             f"{tuple(t.shape)} on {t.device}")
-        if contiguous and not t.is_contiguous():
-            raise ValueError(f"{name}: must be contiguous")
+            why = f"expected {dtype} {tuple(shape)} on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}"
+        raise ValueError(f"{name}: {why}")
+
+    def _want(self, name, t, shape, dtype):
+        """The address of a contiguous tensor that has to be as given."""
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index or not t.is_contiguous():
+            self._refuse(name, t, shape, dtype, "must be contiguous")
         return t.data_ptr()
 
     def _strided(self, name, t, shape, dtype):
-        """(address, strides without the last, which is 1)."""
-        p = self._want(name, t, shape, dtype, False)
-        *st, last = t.stride()
-        if last != 1 and shape[-1] > 1:
-            raise ValueError(f"{name}: the last dimension must be contiguous")
-        return p, st
+        """Address and strides but the last, which is 1."""
+        st = t.stride()
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index or (st[-1] != 1 and shape[-1] > 1):
+            self._refuse(name, t, shape, dtype, "the last dimension must be contiguous")
+        return t.data_ptr(), *st[:-1]
 
     def _rows(self, name, planes, shape, dtype, pair):
         """Address, lo address, strides of a K or V tensor: one tensor, or
         with F32 queries its BF16 plane and optional lo plane."""
         if isinstance(planes, self.torch.Tensor):
             planes = (planes,)
-        if not 1 <= len(planes) <= (2 if pair else 1):
-            raise ValueError(f"{name}: {len(planes)} planes" + (" (at most 2)" if pair else
-                                                               " (a second plane goes with float32 queries)"))
-        p, st = self._strided(name, planes[0], shape, dtype)
-        if len(planes) == 1:
-            return p, 0, *st
-        lo, lst = self._strided(name + " lo plane", planes[1], shape, dtype)
-        if lst != st:
-            raise ValueError(f"{name}: the planes must have the same strides")
-        return p, lo, *st
+        t, n = planes[0], len(planes)
+        st = t.stride()
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index or st[-1] != 1:
+            self._refuse(name, t, shape, dtype, "the last dimension must be contiguous")
+        if n == 1:
+            return t.data_ptr(), 0, *st[:3]
+        if n != 2 or not pair:
+            raise ValueError(f"{name}: {n} planes" + (" (at most 2)" if pair else
+                                                     " (a second plane goes with float32 queries)"))
+        lo = planes[1]
+        if lo.dtype is not dtype or lo.shape != shape or lo.get_device() != self._index or lo.stride() != st:
+            self._refuse(name + " lo plane", lo, shape, dtype, "the planes must have the same strides")
+        return t.data_ptr(), lo.data_ptr(), *st[:3]
 
     def tree_mask(self, parents, counts=None):
         """Mask words [batch x n_nodes x ceil(n_nodes / 64)] (int64 bits) and
@@ -163,24 +170,25 @@ class Speculative:
             raise ValueError("k: expected [batch x n_kv_heads x kv_max x head_dim]")
         _, kv, cap, _ = k0.shape
         if out is None:
-            out = torch.empty((b, n, heads, hd), dtype=qt, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         cache, tree, i32 = (b, kv, cap, hd), (b, kv, n, hd), torch.int32
-        qp, qs = self._strided("q", q, (b, n, heads, hd), qt)
-        op, os = self._strided("out", out, (b, n, heads, hd), qt)
         head = (ty, b, n, heads, kv, hd, cap)
-        fields = (*head, hd ** -0.5 if scale is None else scale, qp, *qs,
+        fields = (*head, hd ** -0.5 if scale is None else scale,
+                  *self._strided("q", q, (b, n, heads, hd), qt),
                   *self._rows("k", k, cache, kt, pair), *self._rows("v", v, cache, kt, pair),
                   *self._rows("tree_k", tree_k, tree, kt, pair), *self._rows("tree_v", tree_v, tree, kt, pair),
                   self._want("lens", lens, (b,), i32), 0 if counts is None else self._want("counts", counts, (b,), i32),
-                  self._want("mask", mask, (b, n, (n + 63) // 64), torch.int64), op, *os,
+                  self._want("mask", mask, (b, n, (n + 63) // 64), torch.int64),
+                  *self._strided("out", out, (b, n, heads, hd), qt),
                   0 if lse is None else self._want("lse", lse, (b, n, heads), torch.float32))
-        need = self._workspace.get(head)
+        key = (head, pair and any(fields[13:29:5]))  # a lo plane's presence
+        need = self._workspace.get(key)
         if need is None:
-            need = self._workspace[head] = self.lib.ds_cuda_tree_attention_workspace(self.ctx.h,
-                                                                                     _pack_attention(*fields, 0, 0))
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        self.ctx.check(self.lib.ds_cuda_tree_attention_dev(self.ctx.h, _pack_attention(*fields, ws.data_ptr(), need),
-                                                           self._stream()), "tree_attention")
+            need = self._workspace[key] = self.lib.ds_cuda_tree_attention_workspace(self.ctx.h,
+                                                                                    _pack_attention(*fields, 0, 0))
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self.ctx.check(self.lib.ds_cuda_tree_attention_dev(
+            self.ctx.h, _pack_attention(*fields, ws.data_ptr() if need else 0, need), self._stream()), "tree_attention")
         return out
 
     def token_probs(self, logits, temperature=None, out=None):
@@ -196,7 +204,7 @@ class Speculative:
         tp = None if temperature is None else self._want("temperature", temperature, (rows,), torch.float32)
         if out is None:
             out = torch.empty((rows, vocab), dtype=torch.float32, device=self.device)
-        self.ctx.check(self.lib.ds_cuda_token_probs_dev(self.ctx.h, ty, lp, rows, vocab, st[0], tp,
+        self.ctx.check(self.lib.ds_cuda_token_probs_dev(self.ctx.h, ty, lp, rows, vocab, st, tp,
                                                         self._want("out", out, (rows, vocab), torch.float32),
                                                         self._stream()), "token_probs")
         return out
@@ -215,21 +223,20 @@ class Speculative:
             raise ValueError("target: expected [batch x n_nodes x vocab]")
         vocab = target.shape[2]
         i32, f32, shape = torch.int32, torch.float32, (b, n, vocab)
-        tp, ts = self._strided("target", target, shape, f32)
-        dp, ds = (0, (0, 0)) if draft is None else self._strided("draft", draft, shape, f32)
-        res = self._results(b, n)
+        res = self._results(tokens)
         d = _pack_verify(b, n, vocab, self._want("tokens", tokens, (b, n), i32),
                          self._want("parents", parents, (b, n), i32),
-                         0 if counts is None else self._want("counts", counts, (b,), i32), tp, *ts, dp, *ds,
+                         0 if counts is None else self._want("counts", counts, (b,), i32),
+                         *self._strided("target", target, shape, f32),
+                         *((0, 0, 0) if draft is None else self._strided("draft", draft, shape, f32)),
                          self._want("accept_u", accept_u, (b, n), f32), self._want("sample_u", sample_u, (b,), f32),
                          *(t.data_ptr() for t in res))
         self.ctx.check(self.lib.ds_cuda_tree_verify_dev(self.ctx.h, d, self._stream()), "tree_verify")
         return res
 
-    def _results(self, b, n):
-        torch = self.torch
-        r = torch.empty(b * (n + 2), dtype=torch.int32, device=self.device)
-        return r[:b * n].view(b, n), r[b * n:b * n + b], r[b * n + b:]
+    def _results(self, tokens):
+        accepted, token = tokens.new_empty((2, tokens.shape[0]))
+        return self.torch.empty_like(tokens), accepted, token
 
     def verify_greedy(self, tokens, parents, target_tokens, counts=None):
         """The greedy rule on the target's argmax tokens [batch x n_nodes]
@@ -241,7 +248,7 @@ class Speculative:
         pp = self._want("parents", parents, (b, n), torch.int32)
         wp = self._want("target_tokens", target_tokens, (b, n), torch.int32)
         cp = None if counts is None else self._want("counts", counts, (b,), torch.int32)
-        res = self._results(b, n)
+        res = self._results(tokens)
         self.ctx.check(self.lib.ds_cuda_tree_verify_greedy_dev(self.ctx.h, tp, pp, cp, wp, b, n,
                                                                *(t.data_ptr() for t in res), self._stream()),
                        "tree_verify_greedy")
@@ -266,9 +273,9 @@ class Speculative:
         i32 = torch.int32
         cp, cs, tp, ts = [0] * 8, [0] * 32, [0] * 8, [0] * 32
         for i in range(m):
-            cp[i], cs[4 * i:4 * i + 4] = self._strided("cache", caches[i], shape, dt)
-            tp[i], ts[4 * i:4 * i + 4] = self._strided("tree", trees[i], rows, dt)
-        new = torch.empty(b, dtype=i32, device=self.device)
+            cp[i], *cs[4 * i:4 * i + 4] = self._strided("cache", caches[i], shape, dt)
+            tp[i], *ts[4 * i:4 * i + 4] = self._strided("tree", trees[i], rows, dt)
+        new = torch.empty_like(lens)
         d = _pack_commit(m, layers, b, n, kv, hd, cap, *cp, *cs, *tp, *ts, self._want("lens", lens, (b,), i32),
                          self._want("path", path, (b, n), i32), self._want("accepted", accepted, (b,), i32),
                          new.data_ptr())

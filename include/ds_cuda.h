@@ -582,8 +582,8 @@ typedef struct {
     float *lse;                             /* optional [batch x n_nodes x n_heads]: log of the sum of exp(scale q k) */
     void *workspace; size_t workspace_bytes; /* 256-byte aligned; not shared by calls that may overlap */
 } ds_cuda_tree_attention_t;
-/* Bytes of workspace a call with these sizes needs (pointers not read); 0
- * also where the sizes are refused. */
+/* Bytes of workspace a call with these sizes needs (0 for some, and where the
+ * sizes are refused); of the pointers only the lo planes' presence matters. */
 size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *ctx, const ds_cuda_tree_attention_t *d);
 int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *ctx, const ds_cuda_tree_attention_t *d, void *stream);
 
