@@ -24,7 +24,7 @@ constexpr int SA_MAX_NODES = 256;
 constexpr int SA_THREADS = 128;
 constexpr int SA_WARPS = SA_THREADS / 32;
 constexpr int SA_STAGES = 3;
-constexpr int SA_MAX_CTAS = 4;  // resident CTAs an SM
+constexpr int SA_MAX_CTAS = 4;  // of an SM
 
 struct SaArgs {
     ds_cuda_tree_attention_t d;
@@ -55,7 +55,7 @@ __device__ __forceinline__ SaSeq sa_seq(const ds_cuda_tree_attention_t &d, int b
 // Sums the sequences' tiles over the batch: returns the total, *mine the
 // tiles before this thread's run of sequences [b0, b1). (The host refuses
 // what could pass 2^31 tiles.)
-template <int KT, int WARPS>
+template <int KT>
 __device__ __forceinline__ int sa_scan(const SaArgs &a, int b0, int b1, int *sh, int *mine) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int s = 0;
@@ -70,7 +70,7 @@ __device__ __forceinline__ int sa_scan(const SaArgs &a, int b0, int b1, int *sh,
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; w++) {
+    for (int w = 0; w < SA_WARPS; w++) {
         if (w < warp) before += sh[w];
         total += sh[w];
     }
@@ -97,6 +97,9 @@ struct SaCut {
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -118,10 +121,11 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 8 keys at a time (BF16).
-__device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5},{%6},{%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b0));
+// An 8 x 8 block of 16-bit values, two a thread, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 template <bool F16> __device__ __forceinline__ uint32_t pack2(float x, float y) {
     uint32_t r;
@@ -212,6 +216,536 @@ __device__ __forceinline__ float4 cluster_ld4(const float4 *p, int k) {
     return v;
 }
 
+// ---- a CTA's run of the list -------------------------------------------------
+struct SaCursor {
+    int b, g, rt, t;  // sequence, key head, row tile, tile of the item
+    SaSeq s;
+};
+// The run's first tile and length. CLUSTER: an item is shared by one cluster,
+// its tiles cut into the CTAs' runs. False: nothing to do (list only).
+template <int KT, bool CLUSTER>
+__device__ __forceinline__ bool sa_begin(const SaArgs &a, SaCursor &c, int &tiles) {
+    __shared__ int sh_scan[SA_WARPS], sh_off, sh_b;
+    const int tid = threadIdx.x;
+    if (CLUSTER) {
+        cluster_arrive();
+        const int item = blockIdx.x / cluster_ctas(), rank = cluster_rank();
+        c.b = item / a.per_seq;
+        c.rt = item % a.row_tiles;
+        c.g = item % a.per_seq / a.row_tiles;
+        c.s = sa_seq<KT>(a.d, c.b);
+        const SaCut cut(c.s.tiles, cluster_ctas());
+        c.t = rank < cut.ctas ? cut.start(rank) : 0;
+        tiles = rank < cut.ctas ? cut.start(rank + 1) - c.t : 0;
+        return true;
+    }
+    pdl_launch();
+    const int chunk = (a.d.batch + SA_THREADS - 1) / SA_THREADS;
+    const int b0 = min(a.d.batch, tid * chunk), b1 = min(a.d.batch, b0 + chunk);
+    int at;
+    const int total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
+    const SaCut cut(total, a.ctas);
+    if ((int)blockIdx.x >= cut.ctas) return false;
+    const int first = cut.start(blockIdx.x);
+    tiles = cut.start(blockIdx.x + 1) - first;
+    for (int b = b0; b < b1; b++) {
+        const int n = sa_seq<KT>(a.d, b).tiles * a.per_seq;
+        if (at <= first && first < at + n) {
+            sh_b = b;
+            sh_off = first - at;
+        }
+        at += n;
+    }
+    __syncthreads();
+    c.b = sh_b;
+    c.s = sa_seq<KT>(a.d, c.b);
+    const int off = sh_off / c.s.tiles;
+    c.t = sh_off - off * c.s.tiles;
+    c.rt = off % a.row_tiles;
+    c.g = off / a.row_tiles;
+    return true;
+}
+template <int KT> __device__ __forceinline__ void sa_next(const SaArgs &a, SaCursor &c) {
+    if (++c.t < c.s.tiles) return;
+    c.t = 0;
+    if (++c.rt < a.row_tiles) return;
+    c.rt = 0;
+    if (++c.g < a.d.n_kv_heads) return;
+    c.g = 0;
+    if (++c.b < a.d.batch) c.s = sa_seq<KT>(a.d, c.b);
+}
+// Where a tile's rows are: K and V planes, row strides, the valid rows (may
+// be none or more than the tile's).
+struct SaTile {
+    bool node;
+    int r0, valid;
+    const uint16_t *base[2][2];
+    int64_t step[2];
+    bool lo[2];
+};
+template <int KT> __device__ __forceinline__ SaTile sa_tile(const ds_cuda_tree_attention_t &d, const SaCursor &c) {
+    SaTile s;
+    s.node = c.t >= c.s.cache_tiles;
+    s.r0 = (s.node ? c.t - c.s.cache_tiles : c.t) * KT;
+    s.valid = (s.node ? c.s.cnt : c.s.len) - s.r0;
+    const int64_t *ks = s.node ? d.tree_k_stride : d.k_stride, *vs = s.node ? d.tree_v_stride : d.v_stride;
+    const int64_t ko = c.b * ks[0] + c.g * ks[1] + (int64_t)s.r0 * ks[2], vo = c.b * vs[0] + c.g * vs[1] + (int64_t)s.r0 * vs[2];
+    const void *k_lo = s.node ? d.tree_k_lo : d.k_lo, *v_lo = s.node ? d.tree_v_lo : d.v_lo;
+    s.base[0][0] = (const uint16_t *)(s.node ? d.tree_k : d.k) + ko;
+    s.base[0][1] = (const uint16_t *)k_lo + ko;
+    s.base[1][0] = (const uint16_t *)(s.node ? d.tree_v : d.v) + vo;
+    s.base[1][1] = (const uint16_t *)v_lo + vo;
+    s.step[0] = ks[2];
+    s.step[1] = vs[2];
+    s.lo[0] = k_lo != nullptr;
+    s.lo[1] = v_lo != nullptr;
+    return s;
+}
+// Dimension c of row r of a part in shared memory is at c ^ sa_swz(r).
+__device__ __forceinline__ int sa_swz(int r) { return ((r >> 1) & 3) << 3; }
+// A CTA's part of an item, from KS warps' parts of each row: given to
+// put(row, c, max, sum, values of dimensions [c, c + 4)).
+template <int RT, int HD, int KS, class ML, class PART, class PUT>
+__device__ __forceinline__ void sa_merge(ML ml_of, PART part_of, PUT put) {
+    for (int x = threadIdx.x; x < RT * (HD / 4); x += SA_THREADS) {
+        const int r = x / (HD / 4), c = 4 * (x % (HD / 4));
+        float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < KS; w++) mm = fmaxf(mm, ml_of(w, r).x);
+#pragma unroll
+        for (int w = 0; w < KS; w++) {
+            const float2 ml = ml_of(w, r);
+            sa_add(v, ll, *reinterpret_cast<const float4 *>(part_of(w, r, c)), ml.y, ex2(ml.x - mm));
+        }
+        put(r, c, mm, ll, v);
+    }
+}
+// What a CTA does with its part of an item: keep it for the cluster, write
+// the result, or leave it in the workspace (slot 0: a run's first item,
+// begun by an earlier CTA; 1: its last).
+template <int RT, int HD, bool CLUSTER>
+__device__ __forceinline__ void sa_put(const SaArgs &a, const SaCursor &c, bool first, bool last, float4 *sh_part,
+                                       float2 *sh_pml, int r, int col, float m, float l, float (&v)[4]) {
+    const int row = c.rt * RT + r;
+    if (row >= a.rows) return;
+    if (CLUSTER) {
+        sh_part[r * (HD / 4) + col / 4] = make_float4(v[0], v[1], v[2], v[3]);
+        if (col == 0) sh_pml[r] = make_float2(m, l);
+    } else if (first && last) {
+        sa_finish(a, c.b, c.g, row, c.s.cnt, col, m, l, v);
+    } else {
+        const size_t pr = ((size_t)blockIdx.x * 2 + first) * RT + r;
+        *reinterpret_cast<float4 *>(a.part + pr * HD + col) = make_float4(v[0], v[1], v[2], v[3]);
+        if (col == 0) a.ml[pr] = make_float2(m, l);
+    }
+}
+// The cluster's parts joined, each CTA a share of the rows and dimensions.
+template <int RT, int HD>
+__device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor &c, const float4 *sh_part,
+                                                const float2 *sh_pml) {
+    __syncwarp();
+    cluster_wait();  // (the arrival at the start)
+    cluster_arrive();
+    cluster_wait();  // every CTA's part is in its shared memory
+    const int n = cluster_ctas(), used = min(n, c.s.tiles), left = min(RT, a.rows - c.rt * RT);
+    for (int x = cluster_rank() * SA_THREADS + threadIdx.x; x < left * (HD / 4); x += n * SA_THREADS) {
+        const int r = x / (HD / 4);
+        float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < used; k++) mm = fmaxf(mm, cluster_ld2(&sh_pml[r], k).x);
+        for (int k = 0; k < used; k++) {
+            const float2 ml = cluster_ld2(&sh_pml[r], k);
+            sa_add(v, ll, cluster_ld4(&sh_part[x], k), ml.y, ex2(ml.x - mm));
+        }
+        sa_finish(a, c.b, c.g, c.rt * RT + r, c.s.cnt, 4 * (x % (HD / 4)), mm, ll, v);
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();  // no CTA leaves while another reads its part
+}
+
+// ---- up to 16 rows -------------------------------------------------------------
+// Keys take the 16-row side of the matrix instructions and the query rows the
+// 8-column side (S^T = K Q^T, O^T = V^T P^T), so up to 8 rows waste nothing and
+// K and V fragments serve all rows. A tile is 64 keys, 16 per warp; a warp
+// loads, multiplies and sums its own keys, with no barrier but at an item's
+// end. Its K and V rows of a tile are a unit each in a ring of three: while
+// one is used, two are in flight, with eight warps an SM 128 KB of them. The
+// queries stay in registers.
+template <int HD_, int NG_, int PL_, int QT_> struct SaFew {
+    static constexpr int HD = HD_, NG = NG_, PL = PL_, QT = QT_;
+    static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
+    static constexpr int RT = 8 * NG, KT = 64;
+    static constexpr int PLANE = 16 * HD * 2, UNIT = PL * PLANE;  // of a warp
+    static constexpr int SMEM = SA_WARPS * 3 * UNIT;
+    static constexpr int PHASES = RT * HD * 4 > UNIT ? RT * HD * 4 / UNIT : 1;  // of a join through one unit a warp
+    static constexpr int FIT = (226 << 10) / (SMEM + 3072);
+    static constexpr int MOST = HD == 128 && QP == 3 && NG == 2 ? 2 : HD == 128 || QP == 3 ? 3 : 4;  // by registers
+    static constexpr int PER_SM = FIT < MOST ? FIT : MOST;
+    static_assert(RT * HD * 4 <= 2 * UNIT, "a CTA's part takes two units at most");
+};
+
+template <class S, bool CLUSTER>
+__global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __grid_constant__ SaArgs a) {
+    constexpr int HD = S::HD, NG = S::NG, CH = HD / 8, KK = HD / 16, NL = NG == 1 ? 4 : 2;
+    constexpr int RS = 32 / CH;  // rows a warp's 16-byte lanes cover at once
+    constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16, F32 = S::QT == DS_CUDA_SPEC_F32;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ float2 sh_ml[SA_WARPS][S::RT], sh_pml[S::RT];
+    // a cluster's part: over the first warp's last unit and the second's first
+    float4 *const sh_part = reinterpret_cast<float4 *>(smem + 2 * S::UNIT);
+    const ds_cuda_tree_attention_t &d = a.d;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = lane & 3;
+    SaCursor ld;
+    int tiles;
+    if (!sa_begin<S::KT, CLUSTER>(a, ld, tiles)) return;
+    SaCursor cu = ld;
+    const SaCursor item = ld;  // CLUSTER's one item
+    uint8_t *const mine = smem + warp * 3 * S::UNIT;
+    auto wrap = [](int x) { return x >= 3 ? x - 3 : x; };
+
+    // Loads: this warp's 16 rows of the cursor's tile, K or V. The pointers
+    // (of this lane's first row and 16 bytes) step from tile to tile and are
+    // set anew where an item or its tree begins.
+    const int cc = lane % CH, rr = lane / CH;
+    const uint16_t *from[2][2];
+    int64_t step[2];
+    bool lo[2];
+    int left = 0;  // valid rows from this warp's first on
+    auto aim = [&]() {
+        const SaTile src = sa_tile<S::KT>(d, ld);
+        left = src.valid - 16 * warp;
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+            step[kv] = src.step[kv] * RS;
+            lo[kv] = src.lo[kv];
+#pragma unroll
+            for (int p = 0; p < S::PL; p++) from[kv][p] = src.base[kv][p] + (16 * warp + rr) * src.step[kv] + 8 * cc;
+        }
+    };
+    auto load = [&](int kv, int slot) {
+        const uint32_t dst = smem_u32(mine) + slot * S::UNIT;
+        if (left >= 16 && (S::PL == 1 || lo[kv])) {
+#pragma unroll
+            for (int p = 0; p < S::PL; p++) {
+                const uint16_t *x = from[kv][p];
+#pragma unroll
+                for (int r = 0; r < 16; r += RS, x += step[kv]) cp16(dst + p * S::PLANE + sw<HD>(rr + r, cc), x);
+            }
+        } else if (left > 0) {  // rows past the valid ones are zeros, and so is a plane that is not there
+#pragma unroll
+            for (int p = 0; p < S::PL; p++) {
+                const uint16_t *x = from[kv][p];
+#pragma unroll
+                for (int r = 0; r < 16; r += RS, x += step[kv]) {
+                    const bool ok = rr + r < left && (p == 0 || lo[kv]);
+                    cp16(dst + p * S::PLANE + sw<HD>(rr + r, cc), ok ? x : d.q, ok);
+                }
+            }
+        }
+        cp_commit();
+    };
+    auto advance = [&]() {
+        const int was = ld.t;
+        const bool tree = was + 1 == ld.s.cache_tiles;
+        sa_next<S::KT>(a, ld);
+        if (ld.t == 0 || tree || was >= ld.s.cache_tiles) {
+            if (ld.b < d.batch) aim();
+            return;
+        }
+        left -= S::KT;
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++)
+#pragma unroll
+            for (int p = 0; p < S::PL; p++) from[kv][p] += step[kv] * (S::KT / RS);
+    };
+    if (tiles > 0) {
+        aim();
+        load(0, 0);
+        load(1, 1);
+        advance();
+    }
+
+    uint32_t qf[NG][S::QP][KK][2];
+    uint64_t bits[NG][2];                 // of rows 2 gc and 2 gc + 1 of each group
+    float o[KK][NG][4], m[NG][2], l[NG][2];
+    bool fresh = true, whole = cu.t == 0;
+    int slot = 0;  // of K; V's follows it, then the next tile's
+    for (int i = 0; i < tiles; i++, slot = wrap(slot + 2)) {
+        if (fresh) {
+            fresh = false;
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+                const int row = cu.rt * S::RT + 8 * n + gr;
+                const bool ok = row < a.rows;
+                const int64_t qo = ok ? cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
+                                            (cu.g * a.group + row % a.group) * d.q_stride[2] + 2 * gc : 0;
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (F32) {
+                            float2 u = make_float2(0.f, 0.f);
+                            if (ok) u = *reinterpret_cast<const float2 *>((const float *)d.q + qo + 16 * kk + 8 * h);
+                            uint32_t p[3];
+                            split3(u.x, u.y, p);
+#pragma unroll
+                            for (int k = 0; k < S::QP; k++) qf[n][k][kk][h] = p[k];
+                        } else {
+                            qf[n][0][kk][h] = ok ? *reinterpret_cast<const uint32_t *>((const uint16_t *)d.q + qo + 16 * kk + 8 * h) : 0;
+                        }
+                    }
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int r2 = cu.rt * S::RT + 8 * n + 2 * gc + e, nd = r2 / a.group;
+                    // rows <= 16, so at most 16 nodes: one word
+                    bits[n][e] = r2 < a.rows && nd < cu.s.cnt ? d.mask[(size_t)cu.b * d.n_nodes + nd] & ((1ull << cu.s.cnt) - 1) : 0;
+                    m[n][e] = -__FLT_MAX__;
+                    l[n][e] = 0.f;
+                }
+#pragma unroll
+                for (int t = 0; t < KK; t++) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+            }
+        }
+        cp_wait<1>();
+        __syncwarp();
+        const bool more = i + 1 < tiles;
+        if (more) load(0, wrap(slot + 2));
+        else cp_commit();
+
+        const bool node = cu.t >= cu.s.cache_tiles;
+        const int valid = (node ? cu.s.cnt : cu.s.len - cu.t * S::KT) - 16 * warp;  // of this warp's keys
+        uint32_t pf[NG][S::QP][2];
+        if (valid > 0) {
+            const uint32_t k_s = smem_u32(mine) + slot * S::UNIT;
+            // scores of 16 keys and 8 NG rows; the planes' products of lower
+            // orders apart (shorter chains, smaller rounding)
+            float s[NG][4], low[F32 ? NG : 1][NL][4];
+#pragma unroll
+            for (int n = 0; n < NG; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[n][e] = 0.f;
+                    if (F32)
+#pragma unroll
+                        for (int x = 0; x < NL; x++) low[n][x][e] = 0.f;
+                }
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                uint32_t kf[S::PL][4];
+#pragma unroll
+                for (int p = 0; p < S::PL; p++) ldsm4(kf[p], k_s + p * S::PLANE + sw<HD>(lane & 15, 2 * kk + (lane >> 4)));
+#pragma unroll
+                for (int pk = 0; pk < S::PL; pk++)
+#pragma unroll
+                    for (int pq = 0; pq < S::QP; pq++)
+                        if (pq + pk < 3)
+#pragma unroll
+                            for (int n = 0; n < NG; n++) {
+                                const int x = NG == 1 ? (pq == 0 ? 0 : pq == 2 ? 3 : pk + 1) : pq + pk - 1;
+                                mma16<F16>(pq + pk ? low[F32 ? n : 0][x & (NL - 1)] : s[n], kf[pk], qf[n][pq][kk][0], qf[n][pq][kk][1]);
+                            }
+            }
+            if (F32)
+#pragma unroll
+                for (int n = 0; n < NG; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float x = low[n][0][e] + low[n][1][e];
+                        if (NL == 4) x += low[n][2 & (NL - 1)][e] + low[n][3 & (NL - 1)][e];
+                        s[n][e] += x;
+                    }
+            // element e: key gr + 8 (e >> 1), row 2 gc + (e & 1) of group n
+            const bool masked = node || valid < 16;
+            uint32_t see = ~0u;  // 4 bits per group
+            if (masked) {
+                see = 0;
+#pragma unroll
+                for (int n = 0; n < NG; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int key = gr + 8 * (e >> 1);
+                        const bool ok = node ? (bits[n][e & 1] >> (16 * warp + key)) & 1 : key < valid;
+                        see |= (uint32_t)ok << (4 * n + e);
+                    }
+            }
+            float mx[NG][2];
+            bool grew = false;
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    mx[n][e] = m[n][e];
+                    if (see >> (4 * n + e) & 1) mx[n][e] = fmaxf(mx[n][e], s[n][e] * a.scale2);
+                    if (see >> (4 * n + e + 2) & 1) mx[n][e] = fmaxf(mx[n][e], s[n][e + 2] * a.scale2);
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(DS_FULL, mx[n][e], w));
+                    grew |= mx[n][e] > m[n][e];
+                }
+            }
+            if (__any_sync(DS_FULL, grew)) {
+#pragma unroll
+                for (int n = 0; n < NG; n++) {
+                    const float f0 = ex2(m[n][0] - mx[n][0]), f1 = ex2(m[n][1] - mx[n][1]);
+                    m[n][0] = mx[n][0];
+                    m[n][1] = mx[n][1];
+                    l[n][0] *= f0;
+                    l[n][1] *= f1;
+#pragma unroll
+                    for (int t = 0; t < KK; t++) {
+                        o[t][n][0] *= f0;
+                        o[t][n][1] *= f1;
+                        o[t][n][2] *= f0;
+                        o[t][n][3] *= f1;
+                    }
+                }
+            }
+            // the weights, and their fragments: the score fragment's 8 x 8
+            // blocks [key][row] transposed are those of P^T [key] for the rows
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[n][e] = see >> (4 * n + e) & 1 ? ex2(__fmaf_rn(s[n][e], a.scale2, -m[n][e & 1])) : 0.f;
+                    l[n][e & 1] += s[n][e];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t p[3];
+                    if (F32) split3(s[n][2 * h], s[n][2 * h + 1], p);
+                    else p[0] = pack2<F16>(s[n][2 * h], s[n][2 * h + 1]);
+#pragma unroll
+                    for (int k = 0; k < S::QP; k++) pf[n][k][h] = transpose8(p[k]);
+                }
+            }
+        }
+        cp_wait<1>();
+        __syncwarp();
+        if (more) {
+            load(1, slot);
+            advance();
+        } else {
+            cp_commit();
+        }
+        if (valid > 0) {
+            uint8_t *const vs = mine + wrap(slot + 1) * S::UNIT;
+            const uint32_t v_s = smem_u32(vs);
+            if (node) {
+                // A node's V may hold NaN or infinities that some rows must not
+                // see, and 0 * NaN would spread through the product: such values
+                // are added here to the rows that attend them, then zeroed.
+                constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u;
+                bool bad = false;
+                for (int x = lane; x < S::UNIT / 16; x += 32) {
+                    const uint4 u = reinterpret_cast<const uint4 *>(vs)[x];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t e = ((&u.x)[k] & E) ^ E;
+                        bad |= !(e & 0xffffu) || !(e >> 16);
+                    }
+                }
+                if (__any_sync(DS_FULL, bad)) {
+                    for (int key = 0; key < 16; key++)
+#pragma unroll
+                        for (int t = 0; t < KK; t++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                float v = 0.f;
+#pragma unroll
+                                for (int p = 0; p < S::PL; p++) {
+                                    const uint16_t w = *reinterpret_cast<const uint16_t *>(vs + p * S::PLANE + sw<HD>(key, 2 * t + h) + 2 * gr);
+                                    v += F16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
+                                }
+                                if (!isfinite(v))
+#pragma unroll
+                                    for (int n = 0; n < NG; n++)
+#pragma unroll
+                                        for (int e = 0; e < 2; e++)
+                                            if (bits[n][e] >> (16 * warp + key) & 1) o[t][n][2 * h + e] += v;
+                            }
+                    __syncwarp();
+                    for (int x = lane; x < 16 * HD; x += 32) {
+                        const uint32_t off = sw<HD>(x / HD, x % HD / 8) + 2 * (x % 8);
+                        bool nf = false;
+#pragma unroll
+                        for (int p = 0; p < S::PL; p++)
+                            nf |= (*reinterpret_cast<uint16_t *>(vs + p * S::PLANE + off) & (E & 0xffff)) == (E & 0xffff);
+                        if (nf)
+#pragma unroll
+                            for (int p = 0; p < S::PL; p++) *reinterpret_cast<uint16_t *>(vs + p * S::PLANE + off) = 0;
+                    }
+                    __syncwarp();
+                }
+            }
+            // O^T += V^T P^T
+#pragma unroll
+            for (int t = 0; t < KK; t++) {
+                uint32_t vf[S::PL][4];
+#pragma unroll
+                for (int p = 0; p < S::PL; p++)
+                    ldsm4t(vf[p], v_s + p * S::PLANE + sw<HD>((lane & 7) + ((lane >> 4) << 3), 2 * t + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int pk = 0; pk < S::PL; pk++)
+#pragma unroll
+                    for (int pq = 0; pq < S::QP; pq++)
+                        if (pq + pk < 3)
+#pragma unroll
+                            for (int n = 0; n < NG; n++) mma16<F16>(o[t][n], vf[pk], pf[n][pq][0], pf[n][pq][1]);
+            }
+        }
+
+        const bool end = cu.t + 1 == cu.s.tiles;
+        if (end || i + 1 == tiles) {
+            // the item, or this CTA's part of it, is done: the warps' parts are
+            // joined through V's units, which are free (a cluster's run ends
+            // here, with every unit free: through the second ones), in phases
+            // where they are smaller than a part
+            constexpr int STEP = 3 * S::UNIT / 4, COLS = HD / S::PHASES;
+            const int js = CLUSTER ? 1 : wrap(slot + 1);
+            float *const so = reinterpret_cast<float *>(mine + js * S::UNIT);
+            const float *const parts = reinterpret_cast<const float *>(smem + js * S::UNIT);
+#pragma unroll
+            for (int n = 0; n < NG; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+#pragma unroll
+                    for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(DS_FULL, l[n][e], w);
+                    if (gr == 0) sh_ml[warp][8 * n + 2 * gc + e] = make_float2(m[n][e], l[n][e]);
+                }
+#pragma unroll
+            for (int ph = 0; ph < S::PHASES; ph++) {
+                // (a cluster's other units may still be read by slower warps)
+                if (CLUSTER && ph == 0) __syncthreads();
+                else __syncwarp();
+#pragma unroll
+                for (int n = 0; n < NG; n++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int t = 0; t < KK / S::PHASES; t++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const int r = 8 * n + 2 * gc + e;
+                                so[r * COLS + ((16 * t + 8 * h + gr) ^ sa_swz(r))] = o[t + ph * (KK / S::PHASES)][n][2 * h + e];
+                            }
+                __syncthreads();
+                sa_merge<S::RT, COLS, SA_WARPS>(
+                    [&](int w, int r) { return sh_ml[w][r]; },
+                    [&](int w, int r, int c) { return parts + w * STEP + r * COLS + (c ^ sa_swz(r)); },
+                    [&](int r, int c, float mm, float ll, float (&v)[4]) {
+                        sa_put<S::RT, HD, CLUSTER>(a, cu, whole, end, sh_part, sh_pml, r, c + ph * COLS, mm, ll, v);
+                    });
+                __syncthreads();  // the join's readers are done: the units may be refilled
+            }
+            fresh = true;
+            whole = true;
+        }
+        sa_next<S::KT>(a, cu);
+    }
+    cp_wait<0>();
+    if (CLUSTER) sa_cluster_join<S::RT, HD>(a, item, sh_part, sh_pml);
+}
+
+// ---- more rows -----------------------------------------------------------------
 // Shapes of one instantiation. QP planes of the queries and of the weights
 // (F32: three, all 24 bits; 16-bit types: one), PL planes of K and V. Four
 // warps: MT row tiles of 16 times KS slices of KW keys. The CTAs are small,
@@ -237,7 +771,6 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
     constexpr int HD = S::HD, KT = S::KT, NT = S::NT, KW = S::KW, CH = HD / 8;
     constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16, F32 = S::QT == DS_CUDA_SPEC_F32;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ int sh_scan[SA_WARPS], sh_off, sh_b;
     __shared__ float2 sh_ml[SA_WARPS][16];
     __shared__ uint64_t sh_mask[2][S::RT];  // by tile parity
     // a cluster's part: over the first stage, unused by then
@@ -248,80 +781,14 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
     const int mt = warp % S::MT, ks = warp / S::MT;
     const uint32_t q_s = smem_u32(smem) + SA_STAGES * S::STAGE;
 
-    struct Cursor {
-        int b, g, rt, t;
-        SaSeq s;
-    } ld, cu;
+    SaCursor ld;
     int tiles;  // of this CTA's run
-    if (CLUSTER) {
-        cluster_arrive();
-        const int item = blockIdx.x / cluster_ctas(), rank = cluster_rank();
-        ld.b = item / a.per_seq;
-        ld.rt = item % a.row_tiles;
-        ld.g = item % a.per_seq / a.row_tiles;
-        ld.s = sa_seq<KT>(d, ld.b);
-        const SaCut cut(ld.s.tiles, cluster_ctas());
-        ld.t = rank < cut.ctas ? cut.start(rank) : 0;
-        tiles = rank < cut.ctas ? cut.start(rank + 1) - ld.t : 0;
-    } else {
-        pdl_launch();
-        const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
-        const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
-        int at;
-        const int total = sa_scan<KT, SA_WARPS>(a, b0, b1, sh_scan, &at);
-        const SaCut cut(total, a.ctas);
-        if ((int)blockIdx.x >= cut.ctas) return;
-        const int first = cut.start(blockIdx.x);
-        tiles = cut.start(blockIdx.x + 1) - first;
-        for (int b = b0; b < b1; b++) {
-            const int n = sa_seq<KT>(d, b).tiles * a.per_seq;
-            if (at <= first && first < at + n) {
-                sh_b = b;
-                sh_off = first - at;
-            }
-            at += n;
-        }
-        __syncthreads();
-        ld.b = sh_b;
-        ld.s = sa_seq<KT>(d, ld.b);
-        const int off = sh_off / ld.s.tiles;
-        ld.t = sh_off - off * ld.s.tiles;
-        ld.rt = off % a.row_tiles;
-        ld.g = off / a.row_tiles;
-    }
-    cu = ld;
-    const int item_b = ld.b, item_g = ld.g, item_rt = ld.rt, item_tiles = ld.s.tiles, cnt = ld.s.cnt;  // CLUSTER's one item
-    auto next = [&](Cursor &c) {
-        if (++c.t < c.s.tiles) return;
-        c.t = 0;
-        if (++c.rt < a.row_tiles) return;
-        c.rt = 0;
-        if (++c.g < d.n_kv_heads) return;
-        c.g = 0;
-        if (++c.b < d.batch) c.s = sa_seq<KT>(d, c.b);
-    };
+    if (!sa_begin<KT, CLUSTER>(a, ld, tiles)) return;
+    SaCursor cu = ld;
+    const SaCursor item = ld;  // CLUSTER's one item
     // the rows of tile c into stage st; rows past the valid ones are zeros
-    auto load = [&](const Cursor &c, int st) {
-        const bool node = c.t >= c.s.cache_tiles;
-        const int r0 = (node ? c.t - c.s.cache_tiles : c.t) * KT;
-        const int valid = (node ? c.s.cnt : c.s.len) - r0;
-        const void *base[4];
-        int64_t step[2];
-        {
-            const int64_t *s = node ? d.tree_k_stride : d.k_stride;
-            const int64_t o = c.b * s[0] + c.g * s[1] + (int64_t)r0 * s[2];
-            base[0] = (const uint16_t *)(node ? d.tree_k : d.k) + o;
-            base[1] = (const uint16_t *)(node ? d.tree_k_lo : d.k_lo) + o;
-            step[0] = s[2];
-        }
-        {
-            const int64_t *s = node ? d.tree_v_stride : d.v_stride;
-            const int64_t o = c.b * s[0] + c.g * s[1] + (int64_t)r0 * s[2];
-            base[2] = (const uint16_t *)(node ? d.tree_v : d.v) + o;
-            base[3] = (const uint16_t *)(node ? d.tree_v_lo : d.v_lo) + o;
-            step[1] = s[2];
-        }
-        const bool lo[2] = {(node ? d.tree_k_lo : d.k_lo) != nullptr, (node ? d.tree_v_lo : d.v_lo) != nullptr};
+    auto load = [&](const SaCursor &c, int st) {
+        const SaTile src = sa_tile<KT>(d, c);
         const uint32_t dst = smem_u32(smem) + st * S::STAGE;
         const int cc = tid % CH, rr = tid / CH;
 #pragma unroll
@@ -331,9 +798,9 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
 #pragma unroll
                 for (int x = 0; x < KT / (SA_THREADS / CH); x++) {
                     const int r = rr + x * (SA_THREADS / CH);
-                    const bool ok = r < valid && (p == 0 || lo[kv]);
+                    const bool ok = r < src.valid && (p == 0 || src.lo[kv]);
                     cp16(dst + (kv * S::PL + p) * S::PLANE + sw<HD>(r, cc),
-                         ok ? (const uint16_t *)base[2 * kv + p] + r * step[kv] + 8 * cc : d.q, ok);
+                         ok ? src.base[kv][p] + r * src.step[kv] + 8 * cc : d.q, ok);
                 }
     };
 
@@ -341,7 +808,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
     for (int i = 0; i < SA_STAGES - 1; i++) {
         if (i < tiles) {
             load(ld, i);
-            next(ld);
+            sa_next<KT>(a, ld);
         }
         cp_commit();
     }
@@ -400,7 +867,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
         __syncthreads();
         if (i + SA_STAGES - 1 < tiles) {
             load(ld, fill);
-            next(ld);
+            sa_next<KT>(a, ld);
         }
         cp_commit();
         fill = fill + 1 == SA_STAGES ? 0 : fill + 1;
@@ -417,26 +884,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
                 if (F32) low[n][0][e] = low[n][1][e] = 0.f;
             }
         const int qr = 16 * mt + (lane & 15), qc = lane >> 4;
-        if (NT == 1) {
-            const int kr = ks * KW + (lane & 7), kc = lane >> 3;
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; kk += 2) {
-                uint32_t qf[2][S::QP][4], kf[S::PL][4];
-#pragma unroll
-                for (int p = 0; p < S::PL; p++) ldsm4(kf[p], k_s + p * S::PLANE + sw<HD>(kr, 2 * kk + kc));
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-#pragma unroll
-                    for (int p = 0; p < S::QP; p++) ldsm4(qf[h][p], q_s + p * S::QPLANE + sw<HD>(qr, 2 * kk + 2 * h + qc));
-#pragma unroll
-                    for (int pq = 0; pq < S::QP; pq++)
-#pragma unroll
-                        for (int pk = 0; pk < S::PL; pk++)
-                            if (pq + pk < 3)
-                                mma16<F16>(pq + pk ? low[0][(pq + pk + 1) & 1] : s[0], qf[h][pq], kf[pk][2 * h], kf[pk][2 * h + 1]);
-                }
-            }
-        } else {
+        {
             const int kr = ks * KW + (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk++) {
@@ -571,25 +1019,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
         }
 
         // O += P V
-        if (NT == 1) {
-            uint32_t p0[3], p1[3];
-            split3(s[0][0], s[0][1], p0);
-            split3(s[0][2], s[0][3], p1);
-            const int vr = ks * KW + (lane & 7), vc = lane >> 3;
-#pragma unroll
-            for (int c = 0; c < CH; c += 4) {
-                uint32_t vf[S::PL][4];
-#pragma unroll
-                for (int p = 0; p < S::PL; p++) ldsm4t(vf[p], v_s + p * S::PLANE + sw<HD>(vr, c + vc));
-#pragma unroll
-                for (int pq = 0; pq < S::QP; pq++)
-#pragma unroll
-                    for (int pk = 0; pk < S::PL; pk++)
-                        if (pq + pk < 3)
-#pragma unroll
-                            for (int x = 0; x < 4; x++) mma8(o[c + x], p0[pq], p1[pq], vf[pk][x]);
-            }
-        } else {
+        {
             const int vr = ks * KW + (lane & 15), vc = lane >> 4;
 #pragma unroll
             for (int n = 0; n < NT; n += 2) {
@@ -645,61 +1075,22 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
                 }
             }
             __syncthreads();
-            const bool alone = end && whole && !CLUSTER;
-            const int slot = whole ? 1 : 0;
-            for (int x = tid; x < S::RT * (HD / 4); x += SA_THREADS) {
-                const int r = x / (HD / 4), c = 4 * (x % (HD / 4)), t16 = r >> 4, rr = r & 15;
-                float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < S::KS; w++) mm = fmaxf(mm, sh_ml[w * S::MT + t16][rr].x);
-#pragma unroll
-                for (int w = 0; w < S::KS; w++) {
-                    const float2 ml = sh_ml[w * S::MT + t16][rr];
-                    const float4 u = *reinterpret_cast<const float4 *>(parts + ((w * S::MT + t16) * 16 + rr) * HD +
-                                                                       (c ^ ((rr & 3) << 3)));
-                    sa_add(v, ll, u, ml.y, ex2(ml.x - mm));
-                }
-                const int row = cu.rt * S::RT + r;
-                if (row >= a.rows) continue;
-                if (CLUSTER) {
-                    sh_part[r * (HD / 4) + c / 4] = make_float4(v[0], v[1], v[2], v[3]);
-                    if (c == 0) sh_pml[r] = make_float2(mm, ll);
-                } else if (alone) {
-                    sa_finish(a, cu.b, cu.g, row, cu.s.cnt, c, mm, ll, v);
-                } else {
-                    const size_t pr = ((size_t)blockIdx.x * 2 + slot) * S::RT + r;
-                    *reinterpret_cast<float4 *>(a.part + pr * HD + c) = make_float4(v[0], v[1], v[2], v[3]);
-                    if (c == 0) a.ml[pr] = make_float2(mm, ll);
-                }
-            }
+            sa_merge<S::RT, HD, S::KS>([&](int w, int r) { return sh_ml[w * S::MT + (r >> 4)][r & 15]; },
+                                       [&](int w, int r, int c) {
+                                           return parts + ((w * S::MT + (r >> 4)) * 16 + (r & 15)) * HD + (c ^ ((r & 3) << 3));
+                                       },
+                                       [&](int r, int c, float mm, float ll, float (&v)[4]) {
+                                           sa_put<S::RT, HD, CLUSTER>(a, cu, whole, end, sh_part, sh_pml, r, c, mm, ll, v);
+                                       });
             fresh = true;
             whole = true;
             __syncthreads();  // the join's readers are done: the stage and the queries may be refilled
         }
-        next(cu);
+        sa_next<KT>(a, cu);
         st = st + 1 == SA_STAGES ? 0 : st + 1;
     }
     cp_wait<0>();
-    if (CLUSTER) {
-        __syncwarp();
-        cluster_wait();  // (the arrival at the start)
-        cluster_arrive();
-        cluster_wait();  // every CTA's part is in its shared memory
-        const int n = cluster_ctas(), used = min(n, item_tiles), left = min(S::RT, a.rows - item_rt * S::RT);
-        for (int x = cluster_rank() * SA_THREADS + tid; x < left * (HD / 4); x += n * SA_THREADS) {
-            const int r = x / (HD / 4);
-            float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < used; k++) mm = fmaxf(mm, cluster_ld2(&sh_pml[r], k).x);
-            for (int k = 0; k < used; k++) {
-                const float2 ml = cluster_ld2(&sh_pml[r], k);
-                sa_add(v, ll, cluster_ld4(&sh_part[x], k), ml.y, ex2(ml.x - mm));
-            }
-            sa_finish(a, item_b, item_g, item_rt * S::RT + r, cnt, 4 * (x % (HD / 4)), mm, ll, v);
-        }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();  // no CTA leaves while another reads its part
-    }
+    if (CLUSTER) sa_cluster_join<S::RT, HD>(a, item, sh_part, sh_pml);
 }
 
 // The items that several CTAs had parts of: HD / 4 threads per row, the parts
@@ -714,7 +1105,7 @@ __global__ void __launch_bounds__(SA_THREADS) sa_join_kernel(const __grid_consta
     const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
     const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
     int at;
-    const int total = sa_scan<KT, SA_WARPS>(a, b0, b1, sh_scan, &at);
+    const int total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
     if (b0 <= b && b < b1) {
         for (int y = b0; y < b; y++) at += sa_seq<KT>(d, y).tiles * a.per_seq;
         sh_off = at;
@@ -762,6 +1153,13 @@ template <class S> static bool sa_clusters(const ds_cuda_tree_attention_t *d, in
     return (long long)items * SA_CLUSTER <= sms * S::PER_SM && tiles <= 8 * SA_CLUSTER;
 }
 
+template <class S, bool CLUSTER> struct SaKernel {
+    static constexpr auto kernel = sa_kernel<S, CLUSTER>;
+};
+template <int HD, int NG, int PL, int QT, bool CLUSTER> struct SaKernel<SaFew<HD, NG, PL, QT>, CLUSTER> {
+    static constexpr auto kernel = sa_few_kernel<SaFew<HD, NG, PL, QT>, CLUSTER>;
+};
+
 template <class S> struct SaRun {
     static bool clusters(const SaArgs &a) { return sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
     static size_t workspace(const SaArgs &a) {
@@ -771,9 +1169,9 @@ template <class S> struct SaRun {
     template <bool CLUSTER> static cudaError_t attributes(int device) {
         static std::atomic<uint64_t> ready;  // devices (of the first 64) that have them
         if (device < 64 && ready.load() >> device & 1) return cudaSuccess;
-        cudaError_t e = cudaFuncSetAttribute(sa_kernel<S, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(SaKernel<S, CLUSTER>::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
         if (e == cudaSuccess && CLUSTER)
-            e = cudaFuncSetAttribute(sa_kernel<S, CLUSTER>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            e = cudaFuncSetAttribute(SaKernel<S, CLUSTER>::kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess && device < 64) ready.fetch_or(1ull << device);
         return e;
     }
@@ -793,14 +1191,14 @@ template <class S> struct SaRun {
             attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            return cudaLaunchKernelExC(&cfg, (const void *)sa_kernel<S, true>, args);
+            return cudaLaunchKernelExC(&cfg, (const void *)SaKernel<S, true>::kernel, args);
         }
         a.ctas = a.sms * S::PER_SM;
         a.part = (float *)a.d.workspace;
         a.ml = (float2 *)(a.part + (size_t)a.ctas * 2 * S::RT * S::HD);
         cudaError_t e = attributes<false>(device);
         if (e != cudaSuccess) return e;
-        sa_kernel<S, false><<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
+        SaKernel<S, false>::kernel<<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
         return launch_ex((const void *)sa_join_kernel<S>, dim3(a.per_seq * (S::RT * (S::HD / 4) / SA_THREADS), a.d.batch),
@@ -808,20 +1206,25 @@ template <class S> struct SaRun {
     }
 };
 
-// f(instantiation) for a call. The row tile: up to 64 rows, or 32 with F32
-// queries, whose three planes take the shared memory.
+// f(instantiation) for a call, by its rows: 8, 16, 32, 64, or 32 at most with
+// F32 queries, whose three planes take the shared memory.
 template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, F f) {
     constexpr int B = DS_CUDA_SPEC_BF16, H = DS_CUDA_SPEC_F16, P = DS_CUDA_SPEC_F32;
     const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
     if (d->type == P) {
         const bool two = d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo;
-        if (two) return rows <= 16 ? f(SaRun<SaShape<HD, 1, 2, P>>()) : f(SaRun<SaShape<HD, 2, 2, P>>());
-        return rows <= 16 ? f(SaRun<SaShape<HD, 1, 1, P>>()) : f(SaRun<SaShape<HD, 2, 1, P>>());
+        if (two)
+            return rows <= 8    ? f(SaRun<SaFew<HD, 1, 2, P>>())
+                   : rows <= 16 ? f(SaRun<SaFew<HD, 2, 2, P>>()) : f(SaRun<SaShape<HD, 2, 2, P>>());
+        return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, P>>())
+               : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, P>>()) : f(SaRun<SaShape<HD, 2, 1, P>>());
     }
     if (d->type == H)
-        return rows <= 16   ? f(SaRun<SaShape<HD, 1, 1, H>>())
+        return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, H>>())
+               : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, H>>())
                : rows <= 32 ? f(SaRun<SaShape<HD, 2, 1, H>>()) : f(SaRun<SaShape<HD, 4, 1, H>>());
-    return rows <= 16   ? f(SaRun<SaShape<HD, 1, 1, B>>())
+    return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, B>>())
+           : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, B>>())
            : rows <= 32 ? f(SaRun<SaShape<HD, 2, 1, B>>()) : f(SaRun<SaShape<HD, 4, 1, B>>());
 }
 template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, F f) {
