@@ -97,6 +97,7 @@ SIGNATURES = {
     "ds_cuda_prefill_stage_ms": (c_int, [P, P]),
     "ds_cuda_tree_attention_workspace": (c_size_t, [P, P]),
     "ds_cuda_tree_attention_dev": (c_int, [P, P, P]),
+    "ds_cuda_tree_attention_check": (c_int, [P, P]),
     "ds_cuda_tree_mask_dev": (c_int, [P, P, P, c_int, c_int, P, P, P]),
     "ds_cuda_token_probs_dev": (c_int, [P, c_int, P, c_int, c_int, c_int64, P, P, P]),
     "ds_cuda_tree_verify_dev": (c_int, [P, P, P]),

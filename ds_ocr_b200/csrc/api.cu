@@ -160,9 +160,11 @@ extern "C" ds_cuda_ctx_t *ds_cuda_init(int device) {
               cudaMalloc(&c->d_val, 512 * sizeof(float)) == cudaSuccess &&
               cudaMalloc(&c->d_scores, 256 * sizeof(float)) == cudaSuccess &&
               cudaMalloc(&c->d_idx, 64 * sizeof(int)) == cudaSuccess &&
-              cudaMalloc(&c->d_wt, 64 * sizeof(float)) == cudaSuccess;
+              cudaMalloc(&c->d_wt, 64 * sizeof(float)) == cudaSuccess &&
+              cudaMalloc(&c->d_spec_err, sizeof(unsigned)) == cudaSuccess;
     if (ok) {
-        ok = cudaMemset(c->d_tickets, 0, 64 * sizeof(unsigned)) == cudaSuccess &&
+        ok = cudaMemset(c->d_spec_err, 0, sizeof(unsigned)) == cudaSuccess &&
+             cudaMemset(c->d_tickets, 0, 64 * sizeof(unsigned)) == cudaSuccess &&
              cudaMemset(c->d_slots, 0, 512 * sizeof(unsigned long long)) == cudaSuccess;
     }
     if (!ok) {
@@ -186,7 +188,8 @@ extern "C" void ds_cuda_free(ds_cuda_ctx_t *c) {
     for (auto &kv : c->regs) cudaFree(kv.second.dev);
     for (auto &r : c->key_ranges) munmap(r.first, r.second);
     void *bufs[] = {c->d_tickets, c->d_slots, c->d_tok, c->d_val, c->d_scores, c->d_idx, c->d_wt,
-                    c->d_x, c->d_out, c->d_h, c->d_tmp, c->d_lt_planes, c->d_lt_err, c->d_sk_scratch};
+                    c->d_x, c->d_out, c->d_h, c->d_tmp, c->d_lt_planes, c->d_lt_err, c->d_sk_scratch,
+                    c->d_spec_err};
     for (void *b : bufs)
         if (b) cudaFree(b);
     if (c->pin) cudaFreeHost(c->pin);

@@ -44,6 +44,7 @@ struct ds_cuda_ctx {
     // multi-stream GEMM standalone entry: planes + tile list
     void *d_sk_scratch = nullptr;
     size_t sk_scratch_cap = 0;
+    unsigned *d_spec_err = nullptr;         // tree attention: a bounded wait gave up
     // pinned staging
     void *pin = nullptr;
     size_t pin_cap = 0;

@@ -17,6 +17,7 @@
 
 #include "common.cuh"
 #include "ctx.h"
+#include "umma.cuh"
 
 namespace ds {
 
@@ -35,6 +36,7 @@ struct SaArgs {
     int per_seq;    // n_kv_heads * row_tiles: items of a sequence
     int sms, ctas;  // SMs; runs the tile list is cut into, at most
     float scale2;   // scale * log2(e)
+    unsigned *err;  // set where a bounded wait gave up
     float *part;    // workspace: [ctas][2][row tile][head_dim], then ...
     float2 *ml;     // ... [ctas][2][row tile] (max in log2 units, sum)
 };
@@ -55,7 +57,7 @@ __device__ __forceinline__ SaSeq sa_seq(const ds_cuda_tree_attention_t &d, int b
 // Sums the sequences' tiles over the batch: returns the total, *mine the
 // tiles before this thread's run of sequences [b0, b1). (The host refuses
 // what could pass 2^31 tiles.)
-template <int KT>
+template <int KT, int THREADS>
 __device__ __forceinline__ int sa_scan(const SaArgs &a, int b0, int b1, int *sh, int *mine) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int s = 0;
@@ -70,7 +72,7 @@ __device__ __forceinline__ int sa_scan(const SaArgs &a, int b0, int b1, int *sh,
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < SA_WARPS; w++) {
+    for (int w = 0; w < THREADS / 32; w++) {
         if (w < warp) before += sh[w];
         total += sh[w];
     }
@@ -223,9 +225,9 @@ struct SaCursor {
 };
 // The run's first tile and length. CLUSTER: an item is shared by one cluster,
 // its tiles cut into the CTAs' runs. False: nothing to do (list only).
-template <int KT, bool CLUSTER>
+template <int KT, bool CLUSTER, int THREADS = SA_THREADS>
 __device__ __forceinline__ bool sa_begin(const SaArgs &a, SaCursor &c, int &tiles) {
-    __shared__ int sh_scan[SA_WARPS], sh_off, sh_b;
+    __shared__ int sh_scan[THREADS / 32], sh_off, sh_b;
     const int tid = threadIdx.x;
     if (CLUSTER) {
         cluster_arrive();
@@ -240,10 +242,10 @@ __device__ __forceinline__ bool sa_begin(const SaArgs &a, SaCursor &c, int &tile
         return true;
     }
     pdl_launch();
-    const int chunk = (a.d.batch + SA_THREADS - 1) / SA_THREADS;
+    const int chunk = (a.d.batch + THREADS - 1) / THREADS;
     const int b0 = min(a.d.batch, tid * chunk), b1 = min(a.d.batch, b0 + chunk);
     int at;
-    const int total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
+    const int total = sa_scan<KT, THREADS>(a, b0, b1, sh_scan, &at);
     const SaCut cut(total, a.ctas);
     if ((int)blockIdx.x >= cut.ctas) return false;
     const int first = cut.start(blockIdx.x);
@@ -1093,6 +1095,459 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
     if (CLUSTER) sa_cluster_join<S::RT, HD>(a, item, sh_part, sh_pml);
 }
 
+// ---- many rows: tcgen05 ----------------------------------------------------------
+// 16-bit types with more than 32 rows. The 128 query rows of a block are the
+// rows of tcgen05.mma (M = 128, accumulators in tensor memory); two softmax
+// groups of 128 threads, a row each, work on two streams in turn, so that the
+// tensor cores serve one while the other takes its exponentials:
+//   DUAL (more than 128 rows): the streams are two blocks of rows that share
+//        every K and V tile;
+//   else: one block of rows, the streams take the even and the odd tiles, and
+//        their results are joined where they are written.
+// Per stream and tile: S = Q K^T (both from shared memory) into tensor memory;
+// a thread reads its row of S, takes 2^(S - m) and stores it as P in tensor
+// memory; O += P V with P as the A operand. m is the row's maximum when it
+// last grew by more than 2^8 (the weights stay below 2^8, and O is rarely
+// rescaled). Two producer warps copy K and V rows into a ring of 16 KB units
+// in the 128-byte swizzle, in the order the products take them.
+constexpr int TC_SOFTMAX = 256, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 32;
+constexpr uint32_t TC_DHI = 64u | (1u << 14) | (2u << 29);  // descriptors' high word: 1024 B between 8-row atoms, 128-byte swizzle
+template <int HD_, bool DUAL_, int QT_> struct SaMany {
+    static constexpr int HD = HD_, QT = QT_, PL = 1;
+    static constexpr bool DUAL = DUAL_;
+    static constexpr int RT = DUAL ? 256 : 128;
+    static constexpr int KT = HD == 128 ? 64 : 128;
+    static constexpr int SUB = KT * 128;           // 64 dimensions of a unit
+    static constexpr int UNIT = KT * HD * 2;       // 16 KB
+    static constexpr int QSUB = 128 * 128, QBLOCK = QSUB * (HD / 64);
+    static constexpr int UNITS = HD == 128 ? (DUAL ? 9 : 10) : 10;
+    static constexpr int SMEM = RT / 128 * QBLOCK + UNITS * UNIT + 1024;
+    static constexpr int PER_SM = 1;
+    // tensor-memory columns: S of each stream, P (16-bit pairs), O
+    static constexpr uint32_t TS = 0, TP = 2 * KT, TO = HD == 128 ? 256 : 384;
+    static_assert(TP + KT <= TO && TO + 2 * HD <= 512, "tensor memory");
+};
+
+__device__ __forceinline__ void cp_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(n) : "memory"); }
+// ... returning whether all of them passed `ok`.
+__device__ __forceinline__ bool bar_and(int id, int n, bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((uint32_t)ok), "r"(id), "r"(n) : "memory");
+    return r != 0;
+}
+
+template <class S>
+__global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_constant__ SaArgs a) {
+    constexpr int HD = S::HD, KT = S::KT, CH = HD / 8, NU = S::UNITS, KS = HD / 16, LEAD = S::DUAL ? 1 : 2;
+    constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *const ring = smem + S::RT / 128 * S::QBLOCK;
+    __shared__ uint64_t full[NU], empty[NU], qfull, sfull[2], pfull[2], odone[2], drain;
+    __shared__ uint32_t tmem_base;
+    __shared__ float2 sh_ml[2][128];
+    __shared__ int sh_bad[16];  // by item: a node's V holds NaN or infinities
+    const ds_cuda_tree_attention_t &d = a.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int u = 0; u < NU; u++) {
+            mbar_init(&full[u], TC_PRODUCERS);
+            mbar_init(&empty[u], 1);
+        }
+        mbar_init(&qfull, TC_SOFTMAX / 32);
+        for (int w = 0; w < 2; w++) {
+            mbar_init(&sfull[w], 1);
+            mbar_init(&pfull[w], 4);
+            mbar_init(&odone[w], 1);
+        }
+        mbar_init(&drain, 1);
+        mbar_fence_init();
+    }
+    if (tid < 16) sh_bad[tid] = 0;
+    if (warp == TC_THREADS / 32 - 1) tmem_alloc(&tmem_base, 512);
+    SaCursor cu;
+    int tiles;
+    if (!sa_begin<KT, false, TC_THREADS>(a, cu, tiles)) tiles = 0;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    bool ok = tiles > 0;
+    // tiles of the run's next item that are this CTA's
+    auto here = [&](int left) { return min(left, cu.s.tiles - cu.t); };
+    auto to_next_item = [&]() {
+        cu.t = cu.s.tiles - 1;
+        sa_next<KT>(a, cu);
+    };
+
+    if (warp >= TC_SOFTMAX / 32 && warp < TC_THREADS / 32 - 1) {
+        // ---- producers: K and V rows, 16 bytes a thread at a time ----
+        const int p = tid - TC_SOFTMAX, cc = p % CH, rr = p / CH;
+        constexpr int RS = TC_PRODUCERS / CH;
+        int slot = 0, item = 0;
+        uint32_t phase = 1;
+        auto load = [&](int t, int kv) {
+            if (!ok) return;
+            ok = mbar_wait(&empty[slot], phase, a.err);
+            if (!ok) return;
+            SaCursor c = cu;
+            c.t += t;
+            const SaTile src = sa_tile<KT>(d, c);
+            const uint16_t *x = src.base[kv][0] + rr * src.step[kv] + 8 * cc;
+            uint8_t *const unit = ring + slot * S::UNIT;
+            const uint32_t dst = smem_u32(unit) + (cc >> 3) * S::SUB;
+            auto at = [&](int r) { return (uint32_t)(r * 128 + (((cc & 7) ^ (r & 7)) << 4)); };
+            if (src.valid >= KT) {
+#pragma unroll 8
+                for (int r = rr; r < KT; r += RS, x += RS * src.step[kv]) cp16(dst + at(r), x);
+            } else {
+#pragma unroll 8
+                for (int r = rr; r < KT; r += RS, x += RS * src.step[kv]) cp16(dst + at(r), r < src.valid ? x : d.q, r < src.valid);
+            }
+            if (src.node && kv) {
+                // A node's V may hold NaN or infinities that some rows must not
+                // see, and 0 * NaN would spread through the product: they are
+                // zeroed here, and added to the results of the rows that attend
+                // them when those are written.
+                cp_commit();
+                cp_wait<0>();
+                constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+                for (int r = rr; r < KT; r += RS) {
+                    uint4 *const v = reinterpret_cast<uint4 *>(unit + (cc >> 3) * S::SUB + at(r));
+                    uint4 u = *v;
+                    bool bad = false;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        uint32_t &w = (&u.x)[k];
+                        if ((w & E) == E) w &= 0xffff0000u, bad = true;
+                        if ((w >> 16 & E) == E) w &= 0xffffu, bad = true;
+                    }
+                    if (bad) {
+                        *v = u;
+                        *reinterpret_cast<volatile int *>(&sh_bad[item & 15]) = 1;
+                    }
+                }
+                fence_proxy_async();
+                mbar_arrive(&full[slot]);
+            } else {
+                cp_arrive(&full[slot]);
+            }
+            if (++slot == NU) {
+                slot = 0;
+                phase ^= 1;
+            }
+        };
+        for (int left = tiles; left > 0 && ok; item++) {
+            const int n = here(left);
+            for (int t = 0; t < min(LEAD, n); t++) load(t, 0);
+            for (int t = 0; t < n; t++) {
+                load(t, 1);
+                if (t + LEAD < n) load(t + LEAD, 0);
+            }
+            left -= n;
+            if (left > 0) to_next_item();
+        }
+        cp_commit();
+        cp_wait<0>();
+    } else if (warp == TC_THREADS / 32 - 1) {
+        // ---- one thread issues the products ----
+        if (lane == 0 && ok) {
+            constexpr uint32_t is = F16 ? idesc_f16_f32(128, KT) : idesc_bf16_f32(128, KT);
+            constexpr uint32_t ip = (F16 ? idesc_f16_f32(128, HD) : idesc_bf16_f32(128, HD)) | (1u << 16);  // V is MN-major
+            int slot = 0, items = 0;
+            uint32_t phase = 0, pp[2] = {0, 0};
+            auto wait = [&](uint64_t *bar, uint32_t ph) { ok = ok && mbar_wait(bar, ph, a.err); };
+            // the ring's next unit
+            auto take = [&]() {
+                wait(&full[slot], phase);
+                fence_proxy_async();  // the copies are ordinary writes, the products' reads are not
+                const int s = slot;
+                if (++slot == NU) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+                return s;
+            };
+            auto qk = [&](int w, int s) {
+                if (!ok) return;
+                const uint32_t k = ((smem_u32(ring + s * S::UNIT) >> 4) & 0x3fffu) | (1u << 16);
+                const uint32_t q = ((smem_u32(smem + (S::DUAL ? w * S::QBLOCK : 0)) >> 4) & 0x3fffu) | (1u << 16);
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    const uint64_t qd = ((uint64_t)TC_DHI << 32) | (q + (j / 4) * (S::QSUB >> 4) + 2 * (j % 4));
+                    const uint64_t kd = ((uint64_t)TC_DHI << 32) | (k + (j / 4) * (S::SUB >> 4) + 2 * (j % 4));
+                    umma_bf16(tmem + S::TS + w * KT, qd, kd, is, j > 0);
+                }
+                umma_commit(&sfull[w]);
+            };
+            auto pv = [&](int w, int s, bool first) {
+                wait(&pfull[w], pp[w]);
+                pp[w] ^= 1;
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t v = ((smem_u32(ring + s * S::UNIT) >> 4) & 0x3fffu) | ((S::SUB >> 4) << 16);
+#pragma unroll
+                for (int j = 0; j < KT / 16; j++) {
+                    if (first && j == 0) umma_ts<0>(tmem + S::TO + w * HD, tmem + S::TP + w * (KT / 2), v, TC_DHI, ip);
+                    else umma_ts<1>(tmem + S::TO + w * HD, tmem + S::TP + w * (KT / 2) + 8 * j, v + 128 * j, TC_DHI, ip);
+                }
+            };
+            for (int left = tiles; left > 0 && ok; items++) {
+                const int n = here(left);
+                wait(&qfull, items & 1);
+                tc_fence_after();
+                if (S::DUAL) {
+                    int k = take();
+                    qk(0, k);
+                    qk(1, k);
+                    umma_commit(&empty[k]);
+                    for (int t = 0; t < n && ok; t++) {
+                        const int v = take();
+                        pv(0, v, t == 0);
+                        if (t + 1 < n) {
+                            k = take();
+                            qk(0, k);
+                        } else {
+                            umma_commit(&odone[0]);
+                        }
+                        pv(1, v, t == 0);
+                        umma_commit(&empty[v]);
+                        if (t + 1 < n) {
+                            qk(1, k);
+                            umma_commit(&empty[k]);
+                        } else {
+                            umma_commit(&odone[1]);
+                        }
+                    }
+                } else {
+                    for (int t = 0; t < min(2, n); t++) {
+                        const int k = take();
+                        qk(t, k);
+                        umma_commit(&empty[k]);
+                    }
+                    for (int t = 0; t < n && ok; t++) {
+                        const int v = take();
+                        pv(t & 1, v, t < 2);
+                        umma_commit(&empty[v]);
+                        if (t + 2 < n) {
+                            const int k = take();
+                            qk(t & 1, k);
+                            umma_commit(&empty[k]);
+                        } else {
+                            umma_commit(&odone[t & 1]);
+                        }
+                    }
+                }
+                left -= n;
+                if (left > 0) to_next_item();
+            }
+            if (!ok) {  // a wait gave up: what was issued ends before the memory goes
+                umma_commit(&drain);
+                mbar_wait(&drain, 0, nullptr);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: row i of stream w ----
+        const int w = warp >> 2, i = tid & 127;
+        const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t ts = tl + S::TS + w * KT, tp = tl + S::TP + w * (KT / 2), to = tl + S::TO + w * HD;
+        const float c = fabsf(a.scale2);
+        const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // the sign goes to the queries
+        uint32_t sp = 0, dp[2] = {0, 0};
+        int item = 0;
+        for (int left = tiles; left > 0 && ok; item++) {
+            const int n = here(left);
+            const bool whole = cu.t == 0, end = cu.t + n == cu.s.tiles;
+            // the queries of the item's rows, swizzled as K is
+            for (int x = tid; x < S::RT * CH; x += TC_SOFTMAX) {
+                const int r = x / CH, ch = x % CH, row = cu.rt * S::RT + r;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (row < a.rows) {
+                    u = *reinterpret_cast<const uint4 *>((const uint16_t *)d.q + cu.b * d.q_stride[0] +
+                                                         (row / a.group) * d.q_stride[1] +
+                                                         (cu.g * a.group + row % a.group) * d.q_stride[2] + 8 * ch);
+                    u.x ^= flip, u.y ^= flip, u.z ^= flip, u.w ^= flip;
+                }
+                *reinterpret_cast<uint4 *>(smem + (r >> 7) * S::QBLOCK + (ch >> 3) * S::QSUB + (r & 127) * 128 +
+                                           (((ch & 7) ^ (r & 7)) << 4)) = u;
+            }
+            fence_proxy_async();
+            tc_fence_before();  // (the last item's results have been read)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&qfull);
+            const int row = cu.rt * S::RT + (S::DUAL ? w * 128 : 0) + i, nd = row / a.group;
+            const bool used = row < a.rows && nd < cu.s.cnt;
+            const uint64_t *const words = d.mask + ((size_t)cu.b * d.n_nodes + (used ? nd : 0)) * a.words;
+            float m = -__FLT_MAX__, l = 0.f;
+            for (int t = S::DUAL ? 0 : w; t < n && ok; t += LEAD) {
+                const bool node = cu.t + t >= cu.s.cache_tiles;
+                const int r0 = (node ? cu.t + t - cu.s.cache_tiles : cu.t + t) * KT;
+                const int valid = (node ? cu.s.cnt : cu.s.len) - r0;
+                const bool masked = node || valid < KT;
+                uint64_t see[KT / 64];
+                if (masked)
+#pragma unroll
+                    for (int k = 0; k < KT / 64; k++) {
+                        const int v = valid - 64 * k;
+                        see[k] = v >= 64 ? ~0ull : v > 0 ? (1ull << v) - 1 : 0;
+                        if (node) see[k] = used && v > 0 ? see[k] & words[r0 / 64 + k] : 0;
+                    }
+                ok = mbar_wait(&sfull[w], sp, a.err);
+                ok = __all_sync(DS_FULL, ok);
+                sp ^= 1;
+                if (!ok) break;
+                tc_fence_after();
+                const bool first = t < LEAD;
+                float mt = -__FLT_MAX__, v[32];
+#pragma unroll
+                for (int k = 0; k < KT / 32; k++) {
+                    tmem_ld32(ts + 32 * k, v);
+                    if (masked) {
+                        const uint32_t b = (uint32_t)(see[k >> 1] >> (32 * (k & 1)));
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (b >> e & 1) mt = fmaxf(mt, v[e]);
+                    } else {
+#pragma unroll
+                        for (int h = 16; h >= 1; h >>= 1)
+#pragma unroll
+                            for (int e = 0; e < h; e++) v[e] = fmaxf(v[e], v[e + h]);
+                        mt = fmaxf(mt, v[0]);
+                    }
+                }
+                const bool grow = first ? mt > m : (mt - m) * c > 8.f;
+                if (__any_sync(DS_FULL, grow)) {
+                    if (!first) {
+                        const float f = grow ? ex2((m - mt) * c) : 1.f;
+                        l *= f;
+#pragma unroll
+                        for (int k = 0; k < HD / 32; k++) {
+                            tmem_ld32(to + 32 * k, v);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) v[e] *= f;
+                            tmem_st32(to + 32 * k, v);
+                        }
+                    }
+                    if (grow) m = mt;
+                }
+                const float mc = fmaxf(m * c, -__FLT_MAX__);
+#pragma unroll
+                for (int k = 0; k < KT / 32; k++) {
+                    tmem_ld32(ts + 32 * k, v);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = ex2(__fmaf_rn(v[e], c, -mc));
+                    if (masked) {
+                        const uint32_t b = (uint32_t)(see[k >> 1] >> (32 * (k & 1)));
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = b >> e & 1 ? v[e] : 0.f;
+                    }
+                    float s[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        s[e & 3] += v[2 * e] + v[2 * e + 1];
+                        pk[e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
+                    }
+                    l += (s[0] + s[1]) + (s[2] + s[3]);
+                    tmem_st16(tp + 16 * k, pk);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[w]);
+            }
+            // the results: a stream's own rows, or the streams' joined, each
+            // group half of the dimensions
+            const bool both = S::DUAL || n > 1;
+            if (ok) ok = mbar_wait(&odone[0], dp[0], a.err);
+            dp[0] ^= 1;
+            if (ok && both) ok = mbar_wait(&odone[1], dp[1], a.err);
+            if (both) dp[1] ^= 1;
+            ok = __all_sync(DS_FULL, ok);
+            tc_fence_after();
+            float mm = fmaxf(m * c, -__FLT_MAX__), ll = l, f0 = 1.f, f1 = 0.f;
+            if (!S::DUAL) {
+                sh_ml[w][i] = make_float2(mm, l);
+                bar_sync(1, TC_SOFTMAX);
+                const float2 x = sh_ml[0][i], y = both ? sh_ml[1][i] : make_float2(-__FLT_MAX__, 0.f);
+                mm = fmaxf(x.x, y.x);
+                f0 = ex2(x.x - mm);
+                f1 = ex2(y.x - mm);
+                ll = x.y * f0 + y.y * f1;
+            }
+            if (ok) {
+                const bool alone = whole && end, none = !used || ll == 0.f;
+                const int head = cu.g * a.group + row % a.group;
+                const float inv = alone ? (none ? 0.f : 1.f / ll) : 1.f;
+                const bool bad = *reinterpret_cast<volatile int *>(&sh_bad[item & 15]) != 0;
+                const size_t pr = ((size_t)blockIdx.x * 2 + whole) * S::RT + (S::DUAL ? w * 128 : 0) + i;
+#pragma unroll 1
+                for (int k = 0; k < HD / 32 / LEAD; k++) {
+                    const int c0 = 32 * (k + (S::DUAL ? 0 : w * (HD / 64)));
+                    __syncwarp();
+                    float v[32];
+                    if (S::DUAL) {
+                        tmem_ld32(to + c0, v);
+                    } else {
+                        tmem_ld32(tl + S::TO + c0, v);
+                        if (both) {
+                            float y[32];
+                            tmem_ld32(tl + S::TO + HD + c0, y);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) v[e] = v[e] * f0 + y[e] * f1;
+                        }
+                    }
+                    if (bad && used)  // see the producers
+                        for (int j = 0; j < cu.s.cnt; j++)
+                            if (words[j >> 6] >> (j & 63) & 1) {
+                                const uint16_t *x = (const uint16_t *)d.tree_v + cu.b * d.tree_v_stride[0] +
+                                                    cu.g * d.tree_v_stride[1] + j * d.tree_v_stride[2] + c0;
+#pragma unroll
+                                for (int e = 0; e < 32; e++) {
+                                    const float y = F16 ? __half2float(__ushort_as_half(x[e])) : __uint_as_float((uint32_t)x[e] << 16);
+                                    if (!isfinite(y)) v[e] += y;
+                                }
+                            }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = alone && none ? 0.f : v[e] * inv;
+                    if (row < a.rows) {
+                        if (alone) {
+                            uint16_t *o = (uint16_t *)d.out + cu.b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c0;
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8)
+                                *reinterpret_cast<uint4 *>(o + e) = make_uint4(pack2<F16>(v[e], v[e + 1]), pack2<F16>(v[e + 2], v[e + 3]),
+                                                                               pack2<F16>(v[e + 4], v[e + 5]), pack2<F16>(v[e + 6], v[e + 7]));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                *reinterpret_cast<float4 *>(a.part + pr * HD + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        }
+                    }
+                }
+                if (row < a.rows && (S::DUAL || w == 0)) {
+                    if (!alone) a.ml[pr] = make_float2(mm, ll);
+                    else if (d.lse)
+                        d.lse[((size_t)cu.b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (mm + log2f(ll)) * 0.69314718f;
+                }
+            }
+            // every reader of sh_ml, sh_bad and O is done; all go on or none
+            ok = bar_and(1, TC_SOFTMAX, ok);
+            if (tid == 0) sh_bad[item & 15] = 0;
+            left -= n;
+            if (left > 0) to_next_item();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == TC_THREADS / 32 - 1) tmem_dealloc(tmem, 512);
+}
+
 // The items that several CTAs had parts of: HD / 4 threads per row, the parts
 // in list order.
 template <class S>
@@ -1105,7 +1560,7 @@ __global__ void __launch_bounds__(SA_THREADS) sa_join_kernel(const __grid_consta
     const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
     const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
     int at;
-    const int total = sa_scan<KT>(a, b0, b1, sh_scan, &at);
+    const int total = sa_scan<KT, SA_THREADS>(a, b0, b1, sh_scan, &at);
     if (b0 <= b && b < b1) {
         for (int y = b0; y < b; y++) at += sa_seq<KT>(d, y).tiles * a.per_seq;
         sh_off = at;
@@ -1160,8 +1615,20 @@ template <int HD, int NG, int PL, int QT, bool CLUSTER> struct SaKernel<SaFew<HD
     static constexpr auto kernel = sa_few_kernel<SaFew<HD, NG, PL, QT>, CLUSTER>;
 };
 
+template <int HD, bool DUAL, int QT> struct SaKernel<SaMany<HD, DUAL, QT>, false> {
+    static constexpr auto kernel = sa_many_kernel<SaMany<HD, DUAL, QT>>;
+};
+template <class S> struct SaThreads {
+    static constexpr int value = SA_THREADS;
+    static constexpr bool clusters = true;
+};
+template <int HD, bool DUAL, int QT> struct SaThreads<SaMany<HD, DUAL, QT>> {
+    static constexpr int value = TC_THREADS;
+    static constexpr bool clusters = false;
+};
+
 template <class S> struct SaRun {
-    static bool clusters(const SaArgs &a) { return sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
+    static bool clusters(const SaArgs &a) { return SaThreads<S>::clusters && sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
     static size_t workspace(const SaArgs &a) {
         // two parts a CTA, then their maxima and sums
         return clusters(a) ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
@@ -1177,7 +1644,7 @@ template <class S> struct SaRun {
     }
     static cudaError_t run(SaArgs a, int device, cudaStream_t st) {
         void *args[] = {&a};
-        if (clusters(a)) {
+        if constexpr (SaThreads<S>::clusters) if (clusters(a)) {
             const cudaError_t e = attributes<true>(device);
             if (e != cudaSuccess) return e;
             cudaLaunchConfig_t cfg = {};
@@ -1198,7 +1665,7 @@ template <class S> struct SaRun {
         a.ml = (float2 *)(a.part + (size_t)a.ctas * 2 * S::RT * S::HD);
         cudaError_t e = attributes<false>(device);
         if (e != cudaSuccess) return e;
-        SaKernel<S, false>::kernel<<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
+        SaKernel<S, false>::kernel<<<a.ctas, SaThreads<S>::value, S::SMEM, st>>>(a);
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
         return launch_ex((const void *)sa_join_kernel<S>, dim3(a.per_seq * (S::RT * (S::HD / 4) / SA_THREADS), a.d.batch),
@@ -1206,26 +1673,24 @@ template <class S> struct SaRun {
     }
 };
 
-// f(instantiation) for a call, by its rows: 8, 16, 32, 64, or 32 at most with
-// F32 queries, whose three planes take the shared memory.
+// f(instantiation) for a call, by its rows. F32 queries take at most 32 at a
+// time: their three planes fill the shared memory.
+template <int HD, int QT, class F> static auto sa_pick16(int rows, F f) {
+    return rows <= 8     ? f(SaRun<SaFew<HD, 1, 1, QT>>())
+           : rows <= 16  ? f(SaRun<SaFew<HD, 2, 1, QT>>())
+           : rows <= 32  ? f(SaRun<SaShape<HD, 2, 1, QT>>())
+           : rows <= 128 ? f(SaRun<SaMany<HD, false, QT>>()) : f(SaRun<SaMany<HD, true, QT>>());
+}
 template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, F f) {
-    constexpr int B = DS_CUDA_SPEC_BF16, H = DS_CUDA_SPEC_F16, P = DS_CUDA_SPEC_F32;
+    constexpr int P = DS_CUDA_SPEC_F32;
     const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
-    if (d->type == P) {
-        const bool two = d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo;
-        if (two)
-            return rows <= 8    ? f(SaRun<SaFew<HD, 1, 2, P>>())
-                   : rows <= 16 ? f(SaRun<SaFew<HD, 2, 2, P>>()) : f(SaRun<SaShape<HD, 2, 2, P>>());
-        return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, P>>())
-               : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, P>>()) : f(SaRun<SaShape<HD, 2, 1, P>>());
-    }
-    if (d->type == H)
-        return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, H>>())
-               : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, H>>())
-               : rows <= 32 ? f(SaRun<SaShape<HD, 2, 1, H>>()) : f(SaRun<SaShape<HD, 4, 1, H>>());
-    return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, B>>())
-           : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, B>>())
-           : rows <= 32 ? f(SaRun<SaShape<HD, 2, 1, B>>()) : f(SaRun<SaShape<HD, 4, 1, B>>());
+    if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, f);
+    if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, f);
+    if (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo)
+        return rows <= 8    ? f(SaRun<SaFew<HD, 1, 2, P>>())
+               : rows <= 16 ? f(SaRun<SaFew<HD, 2, 2, P>>()) : f(SaRun<SaShape<HD, 2, 2, P>>());
+    return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, P>>())
+           : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, P>>()) : f(SaRun<SaShape<HD, 2, 1, P>>());
 }
 template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, F f) {
     return d->head_dim == 64 ? sa_pick_hd<64>(d, f) : sa_pick_hd<128>(d, f);
@@ -1290,6 +1755,7 @@ static SaArgs sa_args(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
     a.row_tiles = (a.rows + rt - 1) / rt;
     a.per_seq = d->n_kv_heads * a.row_tiles;
     a.sms = c->sm_count;
+    a.err = c->d_spec_err;
     a.scale2 = d->scale * 1.44269504f;
     return a;
 }
@@ -1332,6 +1798,19 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     const cudaError_t e = sa_pick(d, [&](auto r) { return decltype(r)::run(a, c->device, st); });
     return ctx_cuda(c, e, "tree_attention launch");
+}
+
+extern "C" int ds_cuda_tree_attention_check(ds_cuda_ctx_t *c, void *stream) {
+    if (!c || !c->ok) return DS_CUDA_EINVAL;
+    cudaSetDevice(c->device);
+    cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
+    unsigned err = 0;
+    cudaError_t e = cudaMemcpyAsync(&err, c->d_spec_err, sizeof err, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) return ctx_cuda(c, e, "tree_attention_check");
+    if (!err) return DS_CUDA_OK;
+    cudaMemsetAsync(c->d_spec_err, 0, sizeof err, st);
+    return ctx_fail(c, DS_CUDA_ETIMEOUT, "tree_attention: a bounded wait gave up");
 }
 
 extern "C" int ds_cuda_tree_mask_dev(ds_cuda_ctx_t *c, const int *parents, const int *nodes, int batch, int n_nodes,

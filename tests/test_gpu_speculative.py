@@ -110,6 +110,24 @@ def test_attention_lengths(spec, kind, length):
     Case(kind, [length], [11], 11, 3, 1, 128, seed=length).check(spec)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,group", [(33, 1), (25, 5), (16, 8), (43, 3), (64, 4), (37, 9), (200, 1)])
+def test_attention_many_rows_long(spec, kind, hd, n, group):
+    Case(kind, [5003, 0, 517], [n, max(1, n - 9), n], n, 2, group, hd, seed=hd + n).check(spec)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+@pytest.mark.parametrize("kind,n", [("pair", 7), ("pair", 20), ("f16", 12), ("bf16", 20), ("bf16", 50)])
+def test_attention_scales(spec, kind, n, scale):
+    # scores up to 60 with the largest scale: |s| 2^-23 stays below the bound
+    c = Case(kind, [150, 1], [n, n], n, 2, 1, 64, seed=21)
+    c.scale = scale
+    c.q = (c.q * (0.25 if scale == 3.0 else 1)).to(c.q.dtype)
+    out = c.run(spec, scale=scale)
+    assert rel(out, c.want()[0]) < max(TOL[kind], 1e-5 if scale == 3.0 else 0)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_attention_ragged_batch(spec, kind):
     lens = [0, 2000, 3, 700, 64, 0, 1, 128, 129, 513, 1500, 17]
@@ -136,9 +154,10 @@ def test_attention_without_cache_rows(spec, kind):
     c.check(spec)
 
 
+@pytest.mark.parametrize("group", [1, 2, 7])
 @pytest.mark.parametrize("kind", KINDS)
-def test_attention_nan_in_a_node_reaches_only_its_readers(spec, kind):
-    c = Case(kind, [70, 3], [10, 10], 10, 2, 2, 128, seed=9)
+def test_attention_nan_in_a_node_reaches_only_its_readers(spec, kind, group):
+    c = Case(kind, [70, 3], [10, 10], 10, 2, group, 128, seed=9)
     ks, vs = (c.tk, c.tv) if isinstance(c.tk, tuple) else ((c.tk,), (c.tv,))
     ks[0][0, :, 7] = float("nan")
     vs[0][1, :, 8] = float("inf")
