@@ -13,10 +13,12 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
 #include "ctx.h"
+#include "tmap.h"
 #include "umma.cuh"
 
 namespace ds {
@@ -823,30 +825,36 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
         cp_wait<SA_STAGES - 2>();
         if (fresh) {  // (the previous item's readers of these are past the last barrier of its end)
             fresh = false;
-            for (int x = tid; x < S::RT * CH; x += SA_THREADS) {
-                const int r = x / CH, c = x % CH, row = cu.rt * S::RT + r;
-                const bool ok = row < a.rows;
-                const int64_t qo = ok ? cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
-                                            (cu.g * a.group + row % a.group) * d.q_stride[2] + 8 * c : 0;
-                if (F32) {
-                    float4 u = make_float4(0, 0, 0, 0), v = u;
-                    if (ok) {
-                        u = *reinterpret_cast<const float4 *>((const float *)d.q + qo);
-                        v = *reinterpret_cast<const float4 *>((const float *)d.q + qo + 4);
-                    }
-                    uint32_t p[4][3];
-                    split3(u.x, u.y, p[0]);
-                    split3(u.z, u.w, p[1]);
-                    split3(v.x, v.y, p[2]);
-                    split3(v.z, v.w, p[3]);
+            // (all loads first: stores in between would hold them up)
+            constexpr int QN = S::RT * CH / SA_THREADS;
+            uint4 u[QN][F32 ? 2 : 1];
 #pragma unroll
-                    for (int k = 0; k < S::QP; k++)
-                        *reinterpret_cast<uint4 *>(smem + SA_STAGES * S::STAGE + k * S::QPLANE + sw<HD>(r, c)) =
-                            make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+            for (int k = 0; k < QN; k++) {
+                const int x = tid + k * SA_THREADS, row = cu.rt * S::RT + x / CH;
+                const int64_t qo = cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
+                                   (cu.g * a.group + row % a.group) * d.q_stride[2] + 8 * (x % CH);
+#pragma unroll
+                for (int h = 0; h < (F32 ? 2 : 1); h++)
+                    u[k][h] = row >= a.rows ? make_uint4(0, 0, 0, 0)
+                              : F32         ? *reinterpret_cast<const uint4 *>((const float *)d.q + qo + 4 * h)
+                                            : *reinterpret_cast<const uint4 *>((const uint16_t *)d.q + qo);
+            }
+#pragma unroll
+            for (int k = 0; k < QN; k++) {
+                const int x = tid + k * SA_THREADS;
+                uint8_t *const q = smem + SA_STAGES * S::STAGE + sw<HD>(x / CH, x % CH);
+                if (F32) {
+                    uint32_t p[4][3];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint4 &y = u[k][F32 ? e >> 1 : 0];
+                        split3(__uint_as_float(e & 1 ? y.z : y.x), __uint_as_float(e & 1 ? y.w : y.y), p[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < S::QP; e++)
+                        *reinterpret_cast<uint4 *>(q + e * S::QPLANE) = make_uint4(p[0][e], p[1][e], p[2][e], p[3][e]);
                 } else {
-                    uint4 u = make_uint4(0, 0, 0, 0);
-                    if (ok) u = *reinterpret_cast<const uint4 *>((const uint16_t *)d.q + qo);
-                    *reinterpret_cast<uint4 *>(smem + SA_STAGES * S::STAGE + sw<HD>(r, c)) = u;
+                    *reinterpret_cast<uint4 *>(q) = u[k][0];
                 }
             }
 #pragma unroll
@@ -1106,9 +1114,9 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
 //        their results are joined where they are written.
 // Per stream and tile: S = Q K^T (both from shared memory) into tensor memory;
 // a thread reads its row of S, takes 2^(S - m) and stores it as P in tensor
-// memory; O += P V with P as the A operand. m is the row's maximum when it
-// last grew by more than 2^8 (the weights stay below 2^8, and O is rarely
-// rescaled). Two producer warps copy K and V rows into a ring of 16 KB units
+// memory; O += P V with P as the A operand. m is the row's maximum of its
+// first tile, or of a later one whose weights passed 2^10, so that O is rarely
+// rescaled. Two producer warps bring K and V rows into a ring of 16 KB units
 // in the 128-byte swizzle, in the order the products take them.
 constexpr int TC_SOFTMAX = 256, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 32;
 constexpr uint32_t TC_DHI = 64u | (1u << 14) | (2u << 29);  // descriptors' high word: 1024 B between 8-row atoms, 128-byte swizzle
@@ -1141,8 +1149,25 @@ __device__ __forceinline__ bool bar_and(int id, int n, bool ok) {
     return r != 0;
 }
 
+// Tensor maps of the cache's K and V (64-dimension boxes of KT rows): whole
+// tiles are one thread's TMA loads, where the strides allow a map; partial
+// ones and the nodes' are copied with zeros past their rows.
+struct SaManyArgs {
+    CUtensorMap map[2];
+    SaArgs a;
+    int mapped;
+    int dim[2][3];  // the map's dimension (1, 2, 3) of row, head, sequence
+};
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        :: "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
 template <class S>
-__global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_constant__ SaArgs a) {
+__global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_constant__ SaManyArgs args) {
+    const SaArgs &a = args.a;
     constexpr int HD = S::HD, KT = S::KT, CH = HD / 8, NU = S::UNITS, KS = HD / 16, LEAD = S::DUAL ? 1 : 2;
     constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16;
     extern __shared__ uint8_t smem_raw[];
@@ -1189,17 +1214,36 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         // ---- producers: K and V rows, 16 bytes a thread at a time ----
         const int p = tid - TC_SOFTMAX, cc = p % CH, rr = p / CH;
         constexpr int RS = TC_PRODUCERS / CH;
-        int slot = 0, item = 0;
+        int slot = 0, item = 0, issued = 0;
         uint32_t phase = 1;
         auto load = [&](int t, int kv) {
             if (!ok) return;
             ok = mbar_wait(&empty[slot], phase, a.err);
             if (!ok) return;
+            issued++;
             SaCursor c = cu;
             c.t += t;
+            uint8_t *const unit = ring + slot * S::UNIT;
+            if (args.mapped && (c.t + 1) * KT <= c.s.len) {
+                if (p == 0) {
+                    const int *const dim = args.dim[kv];
+                    auto at = [&](int k) { return dim[0] == k ? c.t * KT : dim[1] == k ? c.g : c.b; };
+                    const int y = at(1), z = at(2), v = at(3);
+                    mbar_expect_tx(&full[slot], S::UNIT);
+#pragma unroll
+                    for (int k = 0; k < HD / 64; k++)
+                        tma_load_4d(unit + k * S::SUB, &args.map[kv], 64 * k, y, z, v, &full[slot]);
+                } else {
+                    mbar_arrive(&full[slot]);
+                }
+                if (++slot == NU) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+                return;
+            }
             const SaTile src = sa_tile<KT>(d, c);
             const uint16_t *x = src.base[kv][0] + rr * src.step[kv] + 8 * cc;
-            uint8_t *const unit = ring + slot * S::UNIT;
             const uint32_t dst = smem_u32(unit) + (cc >> 3) * S::SUB;
             auto at = [&](int r) { return (uint32_t)(r * 128 + (((cc & 7) ^ (r & 7)) << 4)); };
             if (src.valid >= KT) {
@@ -1217,7 +1261,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 cp_commit();
                 cp_wait<0>();
                 constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-                for (int r = rr; r < KT; r += RS) {
+                for (int r = rr; r < min(KT, src.valid); r += RS) {
                     uint4 *const v = reinterpret_cast<uint4 *>(unit + (cc >> 3) * S::SUB + at(r));
                     uint4 u = *v;
                     bool bad = false;
@@ -1254,6 +1298,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         }
         cp_commit();
         cp_wait<0>();
+        if (!ok && p == 0)  // a wait gave up: what was issued arrives before the memory goes
+            for (int u = max(0, issued - NU); u < issued; u++) mbar_wait(&full[u % NU], u / NU & 1, nullptr);
     } else if (warp == TC_THREADS / 32 - 1) {
         // ---- one thread issues the products ----
         if (lane == 0 && ok) {
@@ -1364,25 +1410,34 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         for (int left = tiles; left > 0 && ok; item++) {
             const int n = here(left);
             const bool whole = cu.t == 0, end = cu.t + n == cu.s.tiles;
-            // the queries of the item's rows, swizzled as K is
-            for (int x = tid; x < S::RT * CH; x += TC_SOFTMAX) {
-                const int r = x / CH, ch = x % CH, row = cu.rt * S::RT + r;
-                uint4 u = make_uint4(0, 0, 0, 0);
-                if (row < a.rows) {
-                    u = *reinterpret_cast<const uint4 *>((const uint16_t *)d.q + cu.b * d.q_stride[0] +
-                                                         (row / a.group) * d.q_stride[1] +
-                                                         (cu.g * a.group + row % a.group) * d.q_stride[2] + 8 * ch);
-                    u.x ^= flip, u.y ^= flip, u.z ^= flip, u.w ^= flip;
+            // the queries of the item's rows, swizzled as K is: a row a thread,
+            // or half a row (all loads first: stores in between would hold
+            // them up)
+            const int row = cu.rt * S::RT + (S::DUAL ? w * 128 : 0) + i, nd = row / a.group, head = cu.g * a.group + row % a.group;
+            const bool used = row < a.rows && nd < cu.s.cnt;
+            {
+                constexpr int QN = CH / LEAD, BATCH = QN < 8 ? QN : 8;
+                const int c0 = S::DUAL ? 0 : w * QN;
+                const uint4 *const q = reinterpret_cast<const uint4 *>((const uint16_t *)d.q + cu.b * d.q_stride[0] +
+                                                                       nd * d.q_stride[1] + head * d.q_stride[2]) + c0;
+                uint8_t *const to_s = smem + (S::DUAL ? w * S::QBLOCK : 0) + i * 128;
+#pragma unroll
+                for (int k0 = 0; k0 < QN; k0 += BATCH) {
+                    uint4 u[BATCH];
+#pragma unroll
+                    for (int k = 0; k < BATCH; k++) u[k] = row < a.rows ? q[k0 + k] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < BATCH; k++) {
+                        const int ch = c0 + k0 + k;
+                        u[k].x ^= flip, u[k].y ^= flip, u[k].z ^= flip, u[k].w ^= flip;
+                        *reinterpret_cast<uint4 *>(to_s + (ch >> 3) * S::QSUB + (((ch & 7) ^ (i & 7)) << 4)) = u[k];
+                    }
                 }
-                *reinterpret_cast<uint4 *>(smem + (r >> 7) * S::QBLOCK + (ch >> 3) * S::QSUB + (r & 127) * 128 +
-                                           (((ch & 7) ^ (r & 7)) << 4)) = u;
             }
             fence_proxy_async();
             tc_fence_before();  // (the last item's results have been read)
             __syncwarp();
             if (lane == 0) mbar_arrive(&qfull);
-            const int row = cu.rt * S::RT + (S::DUAL ? w * 128 : 0) + i, nd = row / a.group;
-            const bool used = row < a.rows && nd < cu.s.cnt;
             const uint64_t *const words = d.mask + ((size_t)cu.b * d.n_nodes + (used ? nd : 0)) * a.words;
             float m = -__FLT_MAX__, l = 0.f;
             for (int t = S::DUAL ? 0 : w; t < n && ok; t += LEAD) {
@@ -1403,60 +1458,75 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 sp ^= 1;
                 if (!ok) break;
                 tc_fence_after();
-                const bool first = t < LEAD;
-                float mt = -__FLT_MAX__, v[32];
+                // The weights of the tile with the row's m so far. Their sum
+                // tells whether m still serves: only a tile that starts a row or
+                // passes 2^10 is done again with its true maximum. (A weight is
+                // at most 2^10, and m is never above the row's maximum.)
+                bool again = t < LEAD;
+                float lt;
+                for (int pass = 0;; pass++) {
+                    const bool look = __any_sync(DS_FULL, again);
+                    if (pass == 1 && !look) break;
+                    if (look) {
+                        float mt = -__FLT_MAX__, v[32];
+#pragma unroll 1
+                        for (int k = 0; k < KT / 32; k++) {
+                            tmem_ld32(ts + 32 * k, v);
+                            const uint32_t b = masked ? (uint32_t)(see[k >> 1] >> (32 * (k & 1))) : ~0u;
 #pragma unroll
-                for (int k = 0; k < KT / 32; k++) {
-                    tmem_ld32(ts + 32 * k, v);
-                    if (masked) {
-                        const uint32_t b = (uint32_t)(see[k >> 1] >> (32 * (k & 1)));
-#pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (b >> e & 1) mt = fmaxf(mt, v[e]);
-                    } else {
-#pragma unroll
-                        for (int h = 16; h >= 1; h >>= 1)
-#pragma unroll
-                            for (int e = 0; e < h; e++) v[e] = fmaxf(v[e], v[e + h]);
-                        mt = fmaxf(mt, v[0]);
-                    }
-                }
-                const bool grow = first ? mt > m : (mt - m) * c > 8.f;
-                if (__any_sync(DS_FULL, grow)) {
-                    if (!first) {
-                        const float f = grow ? ex2((m - mt) * c) : 1.f;
-                        l *= f;
-#pragma unroll
-                        for (int k = 0; k < HD / 32; k++) {
-                            tmem_ld32(to + 32 * k, v);
-#pragma unroll
-                            for (int e = 0; e < 32; e++) v[e] *= f;
-                            tmem_st32(to + 32 * k, v);
+                            for (int e = 0; e < 32; e++)
+                                if (b >> e & 1) mt = fmaxf(mt, v[e]);
                         }
+                        const float f = again && mt > m ? ex2((m - mt) * c) : 1.f;
+                        if (again && mt > m) m = mt;
+                        l *= f;
+                        if (t >= LEAD)
+#pragma unroll 1
+                            for (int k = 0; k < HD / 32; k++) {
+                                tmem_ld32(to + 32 * k, v);
+#pragma unroll
+                                for (int e = 0; e < 32; e++) v[e] *= f;
+                                tmem_st32(to + 32 * k, v);
+                            }
+                        again = false;
+                        pass = 1;
                     }
-                    if (grow) m = mt;
-                }
-                const float mc = fmaxf(m * c, -__FLT_MAX__);
-#pragma unroll
-                for (int k = 0; k < KT / 32; k++) {
-                    tmem_ld32(ts + 32 * k, v);
-#pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = ex2(__fmaf_rn(v[e], c, -mc));
-                    if (masked) {
-                        const uint32_t b = (uint32_t)(see[k >> 1] >> (32 * (k & 1)));
-#pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = b >> e & 1 ? v[e] : 0.f;
-                    }
+                    const float mc = fmaxf(m * c, -__FLT_MAX__);
                     float s[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t pk[16];
+                    // 16 columns while the next are read
+                    auto weigh = [&](float (&v)[16], int k) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        s[e & 3] += v[2 * e] + v[2 * e + 1];
-                        pk[e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
+                        for (int e = 0; e < 16; e++) v[e] = ex2(__fmaf_rn(v[e], c, -mc));
+                        if (masked) {
+                            const uint32_t b = (uint32_t)(see[k >> 2] >> (16 * (k & 3)));
+#pragma unroll
+                            for (int e = 0; e < 16; e++) v[e] = b >> e & 1 ? v[e] : 0.f;
+                        }
+                        uint32_t pk[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            s[e & 3] += v[2 * e] + v[2 * e + 1];
+                            pk[e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
+                        }
+                        tmem_st8_start(tp + 8 * k, pk);
+                    };
+                    float x[16], y[16];
+                    tmem_ld16_start(ts, x);
+#pragma unroll
+                    for (int k = 0; k < KT / 16; k += 2) {
+                        tmem_ld16_wait(x);
+                        tmem_ld16_start(ts + 16 * k + 16, y);
+                        weigh(x, k);
+                        tmem_ld16_wait(y);
+                        if (k + 2 < KT / 16) tmem_ld16_start(ts + 16 * k + 32, x);
+                        weigh(y, k + 1);
                     }
-                    l += (s[0] + s[1]) + (s[2] + s[3]);
-                    tmem_st16(tp + 16 * k, pk);
+                    tmem_st_wait();
+                    lt = (s[0] + s[1]) + (s[2] + s[3]);
+                    if (pass == 1) break;
+                    again = !(lt <= 1024.f);
                 }
+                l += lt;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&pfull[w]);
@@ -1482,10 +1552,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             }
             if (ok) {
                 const bool alone = whole && end, none = !used || ll == 0.f;
-                const int head = cu.g * a.group + row % a.group;
                 const float inv = alone ? (none ? 0.f : 1.f / ll) : 1.f;
                 const bool bad = *reinterpret_cast<volatile int *>(&sh_bad[item & 15]) != 0;
-                const size_t pr = ((size_t)blockIdx.x * 2 + whole) * S::RT + (S::DUAL ? w * 128 : 0) + i;
+                const size_t slot = (size_t)blockIdx.x * 2 + whole;
+                const int r = (S::DUAL ? w * 128 : 0) + i;
 #pragma unroll 1
                 for (int k = 0; k < HD / 32 / LEAD; k++) {
                     const int c0 = 32 * (k + (S::DUAL ? 0 : w * (HD / 64)));
@@ -1524,13 +1594,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                                                                                pack2<F16>(v[e + 4], v[e + 5]), pack2<F16>(v[e + 6], v[e + 7]));
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4)
-                                *reinterpret_cast<float4 *>(a.part + pr * HD + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                            for (int e = 0; e < 32; e++) a.part[(slot * HD + c0 + e) * S::RT + r] = v[e];  // [dimension][row]
                         }
                     }
                 }
                 if (row < a.rows && (S::DUAL || w == 0)) {
-                    if (!alone) a.ml[pr] = make_float2(mm, ll);
+                    if (!alone) a.ml[slot * S::RT + r] = make_float2(mm, ll);
                     else if (d.lse)
                         d.lse[((size_t)cu.b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (mm + log2f(ll)) * 0.69314718f;
                 }
@@ -1548,19 +1617,33 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
     if (warp == TC_THREADS / 32 - 1) tmem_dealloc(tmem, 512);
 }
 
-// The items that several CTAs had parts of: HD / 4 threads per row, the parts
-// in list order.
-template <class S>
-__global__ void __launch_bounds__(SA_THREADS) sa_join_kernel(const __grid_constant__ SaArgs a) {
-    constexpr int HD = S::HD, KT = S::KT;
-    __shared__ int sh_scan[SA_WARPS], sh_off;
+// The items that several CTAs had parts of. Parts are [row][dimension] with
+// HD / 4 threads a row, one row each, or (WIDE) all on one row, where rows are
+// few and parts may be many. The parts of sa_many_kernel are [dimension][row]:
+// a CTA takes 32 rows and 32 dimensions, a warp every eighth part.
+constexpr int SJ_THREADS = 256, SJ_WARPS = SJ_THREADS / 32;
+template <class S> struct SaMade {
+    static constexpr bool by_dimension = false;
+};
+template <int HD, bool DUAL, int QT> struct SaMade<SaMany<HD, DUAL, QT>> {
+    static constexpr bool by_dimension = true;
+};
+// Rows (or, by dimension, 32 x 32 blocks) a CTA takes.
+template <class S> constexpr int sj_rows(bool wide) {
+    return SaMade<S>::by_dimension || wide ? 1 : std::min(S::RT, SJ_THREADS / (S::HD / 4));
+}
+
+template <class S, bool WIDE>
+__global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_constant__ SaArgs a) {
+    constexpr int HD = S::HD, KT = S::KT, RT = S::RT;
+    constexpr bool BYD = SaMade<S>::by_dimension;
+    __shared__ int sh_scan[SJ_WARPS], sh_off;
     const ds_cuda_tree_attention_t &d = a.d;
-    const int tid = threadIdx.x, b = blockIdx.y;
-    const int x = blockIdx.x * SA_THREADS + tid, item = x / (S::RT * (HD / 4)), r = x / (HD / 4) % S::RT, c = 4 * (x % (HD / 4));
-    const int chunk = (d.batch + SA_THREADS - 1) / SA_THREADS;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.y;
+    const int chunk = (d.batch + SJ_THREADS - 1) / SJ_THREADS;
     const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
     int at;
-    const int total = sa_scan<KT, SA_THREADS>(a, b0, b1, sh_scan, &at);
+    const int total = sa_scan<KT, SJ_THREADS>(a, b0, b1, sh_scan, &at);
     if (b0 <= b && b < b1) {
         for (int y = b0; y < b; y++) at += sa_seq<KT>(d, y).tiles * a.per_seq;
         sh_off = at;
@@ -1568,33 +1651,93 @@ __global__ void __launch_bounds__(SA_THREADS) sa_join_kernel(const __grid_consta
     const SaSeq s = sa_seq<KT>(d, b);
     __syncthreads();
     const SaCut cut(total, a.ctas);
+    // this thread's row and first dimension, and the parts it takes
+    constexpr int PER_ITEM = BYD ? (RT / 32) * (HD / 32) : RT / sj_rows<S>(WIDE);
+    const int item = blockIdx.x / PER_ITEM, in = blockIdx.x % PER_ITEM;
+    const int grp = BYD ? warp : tid / (HD / 4), groups = BYD ? SJ_WARPS : SJ_THREADS / (HD / 4);
+    const int r = BYD ? in / (HD / 32) * 32 + lane : WIDE ? in : in * sj_rows<S>(false) + grp;  // (>= RT: none)
+    const int c = BYD ? in % (HD / 32) * 32 : 4 * (tid % (HD / 4));
     const int x0 = sh_off + item * s.tiles, c0 = cut.cta_of(x0), c1 = cut.cta_of(x0 + s.tiles - 1);
-    const int row = item % a.row_tiles * S::RT + r;
+    const int row = r < RT ? item % a.row_tiles * RT + r : a.rows, g = item / a.row_tiles;
     pdl_wait();
-    if (c0 == c1 || row >= a.rows) return;
-    float m = -__FLT_MAX__, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = c0; k0 <= c1; k0 += 8) {
-        float2 ml[8];
-        float4 v[8];
+    if (c0 == c1) return;
+    constexpr int VN = BYD ? 32 : 4;
+    float m = -__FLT_MAX__, l = 0.f, o[VN] = {};
+    const bool split = BYD || WIDE;
+    if (row < a.rows) {
+        constexpr int AHEAD = BYD ? 1 : 4;
+        const int step = split ? groups : 1;
+        for (int k0 = c0 + (split ? grp : 0); k0 <= c1; k0 += AHEAD * step) {
+            float2 ml[AHEAD];
+            float v[AHEAD][VN];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int cc = min(k0 + k, c1);
-            const size_t pr = ((size_t)cc * 2 + (cc == c0)) * S::RT + r;
-            ml[k] = a.ml[pr];
-            v[k] = *reinterpret_cast<const float4 *>(a.part + pr * HD + c);
-        }
+            for (int k = 0; k < AHEAD; k++) {
+                const int cc = min(k0 + k * step, c1);
+                const size_t slot = (size_t)cc * 2 + (cc == c0);
+                ml[k] = a.ml[slot * RT + r];
+                if (BYD) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            if (k0 + k > c1) break;
-            const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn);
-            m = mn;
-            l *= f;
+                    for (int e = 0; e < VN; e++) v[k][e] = a.part[(slot * HD + c + e) * RT + r];
+                } else {
+                    const float4 u = *reinterpret_cast<const float4 *>(a.part + (slot * RT + r) * HD + c);
+                    v[k][0] = u.x, v[k][1] = u.y, v[k][2] = u.z, v[k][3] = u.w;
+                }
+            }
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] *= f;
-            sa_add(o, l, v[k], ml[k].y, ex2(ml[k].x - mn));
+            for (int k = 0; k < AHEAD; k++) {
+                if (k0 + k * step > c1) break;
+                const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn), e2 = ex2(ml[k].x - mn);
+                m = mn;
+                l = l * f + ml[k].y * e2;
+#pragma unroll
+                for (int e = 0; e < VN; e++) o[e] = o[e] * f + v[k][e] * e2;
+            }
         }
     }
-    sa_finish(a, b, item / a.row_tiles, row, s.cnt, c, m, l, o);
+    if (!split) {
+        if (row < a.rows) {
+            float v[4] = {o[0], o[1], o[2], o[3]};
+            sa_finish(a, b, g, row, s.cnt, c, m, l, v);
+        }
+        return;
+    }
+    // the groups' results, in order
+    const int n = min(groups, c1 - c0 + 1);
+    if (BYD) {
+        __shared__ float sh_o[BYD ? SJ_WARPS : 1][32][33];
+        __shared__ float2 sh_ml[BYD ? SJ_WARPS : 1][32];
+        if (warp < n) {
+            sh_ml[BYD ? warp : 0][lane] = make_float2(m, l);
+#pragma unroll
+            for (int e = 0; e < VN; e++) sh_o[BYD ? warp : 0][lane][e % 32] = o[e];
+        }
+        __syncthreads();
+        const int rr = tid >> 3, cc = 4 * (tid & 7), out = row - lane + rr;
+        if (out >= a.rows) return;
+        float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < n; k++) mm = fmaxf(mm, sh_ml[k][rr].x);
+        for (int k = 0; k < n; k++) {
+            const float f = ex2(sh_ml[k][rr].x - mm);
+            ll += sh_ml[k][rr].y * f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += sh_o[k][rr][cc + e] * f;
+        }
+        sa_finish(a, b, g, out, s.cnt, c + cc, mm, ll, v);
+    } else {
+        __shared__ float4 sh_o[SJ_THREADS];
+        __shared__ float2 sh_ml[SJ_THREADS];
+        sh_o[tid] = make_float4(o[0], o[1], o[2], o[3]);
+        sh_ml[tid] = make_float2(m, l);
+        __syncthreads();
+        if (grp || row >= a.rows) return;
+        float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < n; k++) mm = fmaxf(mm, sh_ml[k * (HD / 4) + tid].x);
+        for (int k = 0; k < n; k++) {
+            const float2 ml = sh_ml[k * (HD / 4) + tid];
+            sa_add(v, ll, sh_o[k * (HD / 4) + tid], ml.y, ex2(ml.x - mm));
+        }
+        sa_finish(a, b, g, row, s.cnt, c, mm, ll, v);
+    }
 }
 
 constexpr int SA_CLUSTER = 16;
@@ -1608,6 +1751,35 @@ template <class S> static bool sa_clusters(const ds_cuda_tree_attention_t *d, in
     return (long long)items * SA_CLUSTER <= sms * S::PER_SM && tiles <= 8 * SA_CLUSTER;
 }
 
+// The cache's K or V as a tensor map: the dimensions after the head's own in
+// the order of their strides. False where the strides allow none.
+static bool sa_map(const ds_cuda_tree_attention_t &d, int kv, int kt, CUtensorMap *map, int (&dim)[3]) {
+    const int64_t *const s = kv ? d.v_stride : d.k_stride;
+    const int64_t step[3] = {s[2], s[1], s[0]};
+    const int extent[3] = {d.kv_max, d.n_kv_heads, d.batch};
+    if (d.kv_max < kt) return false;
+    int order[3] = {0, 1, 2};
+    auto key = [&](int i) { return extent[i] > 1 ? step[i] : INT64_MAX; };  // a stride that is never used goes last
+    std::sort(order, order + 3, [&](int x, int y) { return key(x) < key(y); });
+    cuuint64_t dims[4] = {(cuuint64_t)d.head_dim}, strides[3];
+    cuuint32_t box[4] = {64, 1, 1, 1}, one[4] = {1, 1, 1, 1};
+    for (int k = 0; k < 3; k++) {
+        const int i = order[k];
+        const int64_t most = k ? (int64_t)(strides[k - 1] * dims[k]) : 2 * d.head_dim;
+        if (extent[i] > 1 && (step[i] <= 0 || 2 * step[i] >= (int64_t)1 << 40)) return false;
+        strides[k] = extent[i] > 1 ? 2 * step[i] : (most + 15) / 16 * 16;
+        if (strides[k] >= (cuuint64_t)1 << 40) return false;
+        dims[k + 1] = extent[i];
+        dim[i] = k + 1;
+        if (i == 0) box[k + 1] = kt;
+    }
+    const EncodeTiledFn enc = encode_tiled();
+    return enc && enc(map, d.type == DS_CUDA_SPEC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                      const_cast<void *>(kv ? d.v : d.k), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class S, bool CLUSTER> struct SaKernel {
     static constexpr auto kernel = sa_kernel<S, CLUSTER>;
 };
@@ -1618,17 +1790,8 @@ template <int HD, int NG, int PL, int QT, bool CLUSTER> struct SaKernel<SaFew<HD
 template <int HD, bool DUAL, int QT> struct SaKernel<SaMany<HD, DUAL, QT>, false> {
     static constexpr auto kernel = sa_many_kernel<SaMany<HD, DUAL, QT>>;
 };
-template <class S> struct SaThreads {
-    static constexpr int value = SA_THREADS;
-    static constexpr bool clusters = true;
-};
-template <int HD, bool DUAL, int QT> struct SaThreads<SaMany<HD, DUAL, QT>> {
-    static constexpr int value = TC_THREADS;
-    static constexpr bool clusters = false;
-};
-
 template <class S> struct SaRun {
-    static bool clusters(const SaArgs &a) { return SaThreads<S>::clusters && sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
+    static bool clusters(const SaArgs &a) { return !SaMade<S>::by_dimension && sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
     static size_t workspace(const SaArgs &a) {
         // two parts a CTA, then their maxima and sums
         return clusters(a) ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
@@ -1644,7 +1807,7 @@ template <class S> struct SaRun {
     }
     static cudaError_t run(SaArgs a, int device, cudaStream_t st) {
         void *args[] = {&a};
-        if constexpr (SaThreads<S>::clusters) if (clusters(a)) {
+        if constexpr (!SaMade<S>::by_dimension) if (clusters(a)) {
             const cudaError_t e = attributes<true>(device);
             if (e != cudaSuccess) return e;
             cudaLaunchConfig_t cfg = {};
@@ -1665,11 +1828,20 @@ template <class S> struct SaRun {
         a.ml = (float2 *)(a.part + (size_t)a.ctas * 2 * S::RT * S::HD);
         cudaError_t e = attributes<false>(device);
         if (e != cudaSuccess) return e;
-        SaKernel<S, false>::kernel<<<a.ctas, SaThreads<S>::value, S::SMEM, st>>>(a);
+        if constexpr (SaMade<S>::by_dimension) {
+            SaManyArgs many = {};
+            many.a = a;
+            many.mapped = sa_map(a.d, 0, S::KT, &many.map[0], many.dim[0]) && sa_map(a.d, 1, S::KT, &many.map[1], many.dim[1]);
+            sa_many_kernel<S><<<a.ctas, TC_THREADS, S::SMEM, st>>>(many);
+        } else {
+            SaKernel<S, false>::kernel<<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
+        }
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
-        return launch_ex((const void *)sa_join_kernel<S>, dim3(a.per_seq * (S::RT * (S::HD / 4) / SA_THREADS), a.d.batch),
-                         dim3(SA_THREADS), 0, st, true, args);
+        const bool wide = (long long)a.d.batch * a.per_seq * S::RT <= a.sms * 8;
+        const int per_item = SaMade<S>::by_dimension ? (S::RT / 32) * (S::HD / 32) : S::RT / sj_rows<S>(wide);
+        return launch_ex(wide ? (const void *)sa_join_kernel<S, true> : (const void *)sa_join_kernel<S, false>,
+                         dim3(a.per_seq * per_item, a.d.batch), dim3(SJ_THREADS), 0, st, true, args);
     }
 };
 
@@ -1797,6 +1969,7 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
     cudaSetDevice(c->device);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     const cudaError_t e = sa_pick(d, [&](auto r) { return decltype(r)::run(a, c->device, st); });
+    if (e != cudaSuccess) cudaGetLastError();  // reported here, not by whoever asks next
     return ctx_cuda(c, e, "tree_attention launch");
 }
 
