@@ -1106,36 +1106,74 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
 // ---- many rows: tcgen05 ----------------------------------------------------------
 // 16-bit types with more than 32 rows. The 128 query rows of a block are the
 // rows of tcgen05.mma (M = 128, accumulators in tensor memory); two softmax
-// groups of 128 threads, a row each, work on two streams in turn, so that the
-// tensor cores serve one while the other takes its exponentials:
+// groups of 128 threads, a row each, work on two streams:
 //   DUAL (more than 128 rows): the streams are two blocks of rows that share
 //        every K and V tile;
 //   else: one block of rows, the streams take the even and the odd tiles, and
 //        their results are joined where they are written.
-// Per stream and tile: S = Q K^T (both from shared memory) into tensor memory;
-// a thread reads its row of S, takes 2^(S - m) and stores it as P in tensor
-// memory; O += P V with P as the A operand. m is the row's maximum of its
-// first tile, or of a later one whose weights passed 2^10, so that O is rarely
-// rescaled. Two producer warps bring K and V rows into a ring of 16 KB units
-// in the 128-byte swizzle, in the order the products take them.
-constexpr int TC_SOFTMAX = 256, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 32;
+// Per stream and tile of 64 keys: S = Q K^T (both from shared memory) into one
+// of two buffers in tensor memory; a thread reads its row of S, takes
+// 2^(S - m) and stores it, in the place of S, as P; O += P V with P as the A
+// operand. A warp of its own issues a stream's products (issuing takes about
+// 60 cycles a product, which one warp could not do for both), the next tile's
+// S before this one's P is there. m is the row's maximum of its first tile,
+// or of a later one whose weights passed 2^10, so that O is rarely rescaled.
+// Two producer warps bring K and V rows into a ring of units in the 128-byte
+// swizzle, in the order the products take them.
+constexpr int TC_SOFTMAX = 256, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 64;
 constexpr uint32_t TC_DHI = 64u | (1u << 14) | (2u << 29);  // descriptors' high word: 1024 B between 8-row atoms, 128-byte swizzle
 template <int HD_, bool DUAL_, int QT_> struct SaMany {
     static constexpr int HD = HD_, QT = QT_, PL = 1;
     static constexpr bool DUAL = DUAL_;
     static constexpr int RT = DUAL ? 256 : 128;
-    static constexpr int KT = HD == 128 ? 64 : 128;
+    static constexpr int KT = 64;
     static constexpr int SUB = KT * 128;           // 64 dimensions of a unit
-    static constexpr int UNIT = KT * HD * 2;       // 16 KB
+    static constexpr int UNIT = KT * HD * 2;       // 16 KB, 8 KB for head_dim 64
     static constexpr int QSUB = 128 * 128, QBLOCK = QSUB * (HD / 64);
-    static constexpr int UNITS = HD == 128 ? (DUAL ? 9 : 10) : 10;
+    static constexpr int UNITS = HD == 64 ? 16 : DUAL ? 9 : 10;
+    static constexpr int RING = DUAL ? UNITS : UNITS / 2;  // units of a ring: one ring, or one a stream
     static constexpr int SMEM = RT / 128 * QBLOCK + UNITS * UNIT + 1024;
     static constexpr int PER_SM = 1;
-    // tensor-memory columns: S of each stream, P (16-bit pairs), O
-    static constexpr uint32_t TS = 0, TP = 2 * KT, TO = HD == 128 ? 256 : 384;
-    static_assert(TP + KT <= TO && TO + 2 * HD <= 512, "tensor memory");
+    // tensor-memory columns: S (two buffers a stream, P in the first half of each), O
+    static constexpr uint32_t TS = 0, TO = 4 * KT;
+    static_assert(TO + 2 * HD <= 512, "tensor memory");
+    // a ring's units of an item with n tiles: K of two tiles, then V and K in
+    // turn. The place of K and V of tile t, and what is at a place.
+    static __device__ __forceinline__ int place_k(int t) { return t < 2 ? t : 2 * t - 1; }
+    static __device__ __forceinline__ int place_v(int t, int n) { return min(2, n) + t + min(t, max(0, n - 2)); }
+    static __device__ __forceinline__ int at(int place, int n, int &kv) {
+        const int r = place - min(2, n), m = max(0, n - 2);
+        kv = r >= 0 && (r >= 2 * m || !(r & 1));
+        return r < 0 ? place : r >= 2 * m ? r - m : kv ? r / 2 : 2 + r / 2;
+    }
 };
 
+// A wait that gives up after two seconds: the failure is recorded in *err (if
+// given) and everyone leaves.
+__device__ __forceinline__ bool tc_wait(uint64_t *bar, uint32_t parity, unsigned *err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = ds_gtime();
+    do {
+        for (int i = 0; i < 64; i++)
+            if (mbar_try_wait(bar, parity)) return true;
+    } while (ds_gtime() - t0 < 2000000000ull);
+    if (err) atomicExch(err, 1u);
+    return false;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) :: "memory");
+    return r != 0;
+}
+// tcgen05.mma with both operands in shared memory, the descriptors given as
+// low words and a common high word.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t alo, uint32_t blo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .b64 ad, bd;\n\t.reg .pred p;\n\t"
+        "mov.b64 ad, {%1, %3};\n\tmov.b64 bd, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, p;\n\t}"
+        :: "r"(d), "r"(alo), "r"(blo), "r"(hi), "r"(idesc), "r"(accumulate) : "memory");
+}
 __device__ __forceinline__ void cp_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
@@ -1168,12 +1206,12 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
 template <class S>
 __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_constant__ SaManyArgs args) {
     const SaArgs &a = args.a;
-    constexpr int HD = S::HD, KT = S::KT, CH = HD / 8, NU = S::UNITS, KS = HD / 16, LEAD = S::DUAL ? 1 : 2;
+    constexpr int HD = S::HD, KT = S::KT, CH = HD / 8, NU = S::UNITS, STEP = S::DUAL ? 1 : 2;
     constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *const ring = smem + S::RT / 128 * S::QBLOCK;
-    __shared__ uint64_t full[NU], empty[NU], qfull, sfull[2], pfull[2], odone[2], drain;
+    __shared__ uint64_t full[NU], empty[NU], qfull, sfull[2][2], pfull[2][2], pvdone[2], odone[2], drain[2];
     __shared__ uint32_t tmem_base;
     __shared__ float2 sh_ml[2][128];
     __shared__ int sh_bad[16];  // by item: a node's V holds NaN or infinities
@@ -1182,26 +1220,29 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
     if (tid == 0) {
         for (int u = 0; u < NU; u++) {
             mbar_init(&full[u], TC_PRODUCERS);
-            mbar_init(&empty[u], 1);
+            mbar_init(&empty[u], S::DUAL ? 2 : 1);
         }
         mbar_init(&qfull, TC_SOFTMAX / 32);
         for (int w = 0; w < 2; w++) {
-            mbar_init(&sfull[w], 1);
-            mbar_init(&pfull[w], 4);
+            mbar_init(&sfull[w][0], 1);
+            mbar_init(&sfull[w][1], 1);
+            mbar_init(&pfull[w][0], 4);
+            mbar_init(&pfull[w][1], 4);
+            mbar_init(&pvdone[w], 1);
             mbar_init(&odone[w], 1);
+            mbar_init(&drain[w], 1);
         }
-        mbar_init(&drain, 1);
         mbar_fence_init();
     }
     if (tid < 16) sh_bad[tid] = 0;
-    if (warp == TC_THREADS / 32 - 1) tmem_alloc(&tmem_base, 512);
+    if (warp == (TC_SOFTMAX + TC_PRODUCERS) / 32) tmem_alloc(&tmem_base, 512);
     SaCursor cu;
     int tiles;
     if (!sa_begin<KT, false, TC_THREADS>(a, cu, tiles)) tiles = 0;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base;
+    const uint32_t tmem = __shfl_sync(DS_FULL, tmem_base, 0);
     bool ok = tiles > 0;
     // tiles of the run's next item that are this CTA's
     auto here = [&](int left) { return min(left, cu.s.tiles - cu.t); };
@@ -1210,17 +1251,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         sa_next<KT>(a, cu);
     };
 
-    if (warp >= TC_SOFTMAX / 32 && warp < TC_THREADS / 32 - 1) {
+    constexpr int MMA_WARP = (TC_SOFTMAX + TC_PRODUCERS) / 32;
+    if (warp >= TC_SOFTMAX / 32 && warp < MMA_WARP) {
         // ---- producers: K and V rows, 16 bytes a thread at a time ----
         const int p = tid - TC_SOFTMAX, cc = p % CH, rr = p / CH;
         constexpr int RS = TC_PRODUCERS / CH;
-        int slot = 0, item = 0, issued = 0;
-        uint32_t phase = 1;
-        auto load = [&](int t, int kv) {
+        constexpr int RINGS = S::DUAL ? 1 : 2;
+        int item = 0, units[RINGS] = {};  // units so far
+        auto load = [&](int ring_, int t, int kv) {
             if (!ok) return;
-            ok = mbar_wait(&empty[slot], phase, a.err);
+            const int u = units[ring_], slot = ring_ * S::RING + u % S::RING;
+            ok = tc_wait(&empty[slot], (u / S::RING & 1) ^ 1, a.err);
             if (!ok) return;
-            issued++;
+            units[ring_]++;
             SaCursor c = cu;
             c.t += t;
             uint8_t *const unit = ring + slot * S::UNIT;
@@ -1235,10 +1278,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                         tma_load_4d(unit + k * S::SUB, &args.map[kv], 64 * k, y, z, v, &full[slot]);
                 } else {
                     mbar_arrive(&full[slot]);
-                }
-                if (++slot == NU) {
-                    slot = 0;
-                    phase ^= 1;
                 }
                 return;
             }
@@ -1281,132 +1320,107 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             } else {
                 cp_arrive(&full[slot]);
             }
-            if (++slot == NU) {
-                slot = 0;
-                phase ^= 1;
-            }
         };
         for (int left = tiles; left > 0 && ok; item++) {
             const int n = here(left);
-            for (int t = 0; t < min(LEAD, n); t++) load(t, 0);
-            for (int t = 0; t < n; t++) {
-                load(t, 1);
-                if (t + LEAD < n) load(t + LEAD, 0);
-            }
+            const int steps = S::DUAL ? n : (n + 1) >> 1;
+            for (int place = 0; place < 2 * steps; place++)
+#pragma unroll
+                for (int w = 0; w < RINGS; w++) {
+                    const int mine = w ? n >> 1 : steps;
+                    if (place >= 2 * mine) continue;
+                    int kv;
+                    const int t = S::at(place, mine, kv);
+                    load(w, S::DUAL ? t : 2 * t + w, kv);
+                }
             left -= n;
             if (left > 0) to_next_item();
         }
         cp_commit();
         cp_wait<0>();
         if (!ok && p == 0)  // a wait gave up: what was issued arrives before the memory goes
-            for (int u = max(0, issued - NU); u < issued; u++) mbar_wait(&full[u % NU], u / NU & 1, nullptr);
-    } else if (warp == TC_THREADS / 32 - 1) {
-        // ---- one thread issues the products ----
-        if (lane == 0 && ok) {
-            constexpr uint32_t is = F16 ? idesc_f16_f32(128, KT) : idesc_bf16_f32(128, KT);
-            constexpr uint32_t ip = (F16 ? idesc_f16_f32(128, HD) : idesc_bf16_f32(128, HD)) | (1u << 16);  // V is MN-major
-            int slot = 0, items = 0;
-            uint32_t phase = 0, pp[2] = {0, 0};
-            auto wait = [&](uint64_t *bar, uint32_t ph) { ok = ok && mbar_wait(bar, ph, a.err); };
-            // the ring's next unit
-            auto take = [&]() {
-                wait(&full[slot], phase);
-                fence_proxy_async();  // the copies are ordinary writes, the products' reads are not
-                const int s = slot;
-                if (++slot == NU) {
-                    slot = 0;
-                    phase ^= 1;
-                }
-                return s;
-            };
-            auto qk = [&](int w, int s) {
-                if (!ok) return;
-                const uint32_t k = ((smem_u32(ring + s * S::UNIT) >> 4) & 0x3fffu) | (1u << 16);
-                const uint32_t q = ((smem_u32(smem + (S::DUAL ? w * S::QBLOCK : 0)) >> 4) & 0x3fffu) | (1u << 16);
-#pragma unroll
-                for (int j = 0; j < KS; j++) {
-                    const uint64_t qd = ((uint64_t)TC_DHI << 32) | (q + (j / 4) * (S::QSUB >> 4) + 2 * (j % 4));
-                    const uint64_t kd = ((uint64_t)TC_DHI << 32) | (k + (j / 4) * (S::SUB >> 4) + 2 * (j % 4));
-                    umma_bf16(tmem + S::TS + w * KT, qd, kd, is, j > 0);
-                }
-                umma_commit(&sfull[w]);
-            };
-            auto pv = [&](int w, int s, bool first) {
-                wait(&pfull[w], pp[w]);
-                pp[w] ^= 1;
+            for (int w = 0; w < RINGS; w++)
+                for (int u = max(0, units[w] - S::RING); u < units[w]; u++)
+                    tc_wait(&full[w * S::RING + u % S::RING], u / S::RING & 1, nullptr);
+    } else if (warp >= MMA_WARP) {
+        // ---- stream w's products: the warp waits, one lane issues ----
+        const int w = __shfl_sync(DS_FULL, warp - MMA_WARP, 0);
+        constexpr uint32_t is = F16 ? idesc_f16_f32(128, KT) : idesc_bf16_f32(128, KT);
+        constexpr uint32_t ip = (F16 ? idesc_f16_f32(128, HD) : idesc_bf16_f32(128, HD)) | (1u << 16);  // V is MN-major
+        const uint32_t ring_k = (((smem_u32(ring) >> 4) & 0x3fffu) | (1u << 16));
+        const uint32_t ring_v = (((smem_u32(ring) >> 4) & 0x3fffu) | ((S::SUB >> 4) << 16));
+        const uint32_t q = ((smem_u32(smem + (S::DUAL ? w * S::QBLOCK : 0)) >> 4) & 0x3fffu) | (1u << 16);
+        const uint32_t ts = tmem + S::TS + w * 2 * KT, to = tmem + S::TO + w * HD;
+        int done = 0;  // this stream's tiles before the item (two units of its ring each)
+        auto wait = [&](uint64_t *bar, uint32_t ph) { ok = __all_sync(DS_FULL, ok && tc_wait(bar, ph, a.err)); };
+        // a unit of the ring, of the item's tile t
+        auto take = [&](int place, int t) {
+            const int u = 2 * done + place, s = (S::DUAL ? 0 : w * S::RING) + u % S::RING;
+            wait(&full[s], u / S::RING & 1);
+            // copies that are not TMA's are ordinary writes, the products'
+            // reads are not
+            if (!args.mapped || (cu.t + t + 1) * KT > cu.s.len) fence_proxy_async();
+            return s;
+        };
+        for (int left = tiles, item = 0; left > 0 && ok; item++) {
+            const int n = here(left), steps = S::DUAL ? n : (n - w + 1) >> 1;
+            auto qk = [&](int j) {
+                const int t = S::DUAL ? j : 2 * j + w, s = take(S::place_k(j), t), buf = (done + j) & 1;
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t v = ((smem_u32(ring + s * S::UNIT) >> 4) & 0x3fffu) | ((S::SUB >> 4) << 16);
+                const uint32_t k = ring_k + s * (S::UNIT >> 4);
+                if (elect_one()) {
 #pragma unroll
-                for (int j = 0; j < KT / 16; j++) {
-                    if (first && j == 0) umma_ts<0>(tmem + S::TO + w * HD, tmem + S::TP + w * (KT / 2), v, TC_DHI, ip);
-                    else umma_ts<1>(tmem + S::TO + w * HD, tmem + S::TP + w * (KT / 2) + 8 * j, v + 128 * j, TC_DHI, ip);
+                    for (int x = 0; x < HD / 16; x++)
+                        umma_ss(ts + buf * KT, q + (x / 4) * (S::QSUB >> 4) + 2 * (x % 4), k + (x / 4) * (S::SUB >> 4) + 2 * (x % 4),
+                                TC_DHI, is, x > 0);
+                    umma_commit(&sfull[w][buf]);
+                    umma_commit(&empty[s]);
                 }
+                __syncwarp();
             };
-            for (int left = tiles; left > 0 && ok; items++) {
-                const int n = here(left);
-                wait(&qfull, items & 1);
+            wait(&qfull, item & 1);
+            for (int j = 0; j < min(2, steps) && ok; j++) qk(j);
+            for (int j = 0; j < steps && ok; j++) {
+                const int t = S::DUAL ? j : 2 * j + w, s = take(S::place_v(j, steps), t), buf = (done + j) & 1;
+                wait(&pfull[w][buf], (done + j) >> 1 & 1);
+                if (!ok) break;
                 tc_fence_after();
-                if (S::DUAL) {
-                    int k = take();
-                    qk(0, k);
-                    qk(1, k);
-                    umma_commit(&empty[k]);
-                    for (int t = 0; t < n && ok; t++) {
-                        const int v = take();
-                        pv(0, v, t == 0);
-                        if (t + 1 < n) {
-                            k = take();
-                            qk(0, k);
-                        } else {
-                            umma_commit(&odone[0]);
-                        }
-                        pv(1, v, t == 0);
-                        umma_commit(&empty[v]);
-                        if (t + 1 < n) {
-                            qk(1, k);
-                            umma_commit(&empty[k]);
-                        } else {
-                            umma_commit(&odone[1]);
-                        }
-                    }
-                } else {
-                    for (int t = 0; t < min(2, n); t++) {
-                        const int k = take();
-                        qk(t, k);
-                        umma_commit(&empty[k]);
-                    }
-                    for (int t = 0; t < n && ok; t++) {
-                        const int v = take();
-                        pv(t & 1, v, t < 2);
-                        umma_commit(&empty[v]);
-                        if (t + 2 < n) {
-                            const int k = take();
-                            qk(t & 1, k);
-                            umma_commit(&empty[k]);
-                        } else {
-                            umma_commit(&odone[t & 1]);
-                        }
-                    }
+                const uint32_t v = ring_v + s * (S::UNIT >> 4);
+                if (elect_one()) {
+                    if (j == 0) umma_ts<0>(to, ts + buf * KT, v, TC_DHI, ip);
+                    else umma_ts<1>(to, ts + buf * KT, v, TC_DHI, ip);
+#pragma unroll
+                    for (int x = 1; x < KT / 16; x++) umma_ts<1>(to, ts + buf * KT + 8 * x, v + 128 * x, TC_DHI, ip);
+                    umma_commit(&pvdone[w]);
+                    umma_commit(&empty[s]);
+                    if (j + 1 == steps) umma_commit(&odone[w]);
                 }
-                left -= n;
-                if (left > 0) to_next_item();
+                __syncwarp();
+                if (j + 2 < steps) {  // S over this P, once the product has read it
+                    wait(&pvdone[w], (done + j) & 1);
+                    if (ok) qk(j + 2);
+                }
             }
-            if (!ok) {  // a wait gave up: what was issued ends before the memory goes
-                umma_commit(&drain);
-                mbar_wait(&drain, 0, nullptr);
-            }
+            // (a stream without a tile says so: the item's end waits for both)
+            if (steps == 0 && lane == 0) mbar_arrive(&odone[w]);
+            done += steps;
+            left -= n;
+            if (left > 0) to_next_item();
         }
-        __syncwarp();
+        if (!ok && tiles > 0) {  // a wait gave up: what was issued ends before the memory goes
+            if (elect_one()) umma_commit(&drain[w]);
+            __syncwarp();
+            tc_wait(&drain[w], 0, nullptr);
+        }
     } else {
         // ---- softmax: row i of stream w ----
         const int w = warp >> 2, i = tid & 127;
         const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t ts = tl + S::TS + w * KT, tp = tl + S::TP + w * (KT / 2), to = tl + S::TO + w * HD;
+        const uint32_t to = tl + S::TO + w * HD;
         const float c = fabsf(a.scale2);
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // the sign goes to the queries
-        uint32_t sp = 0, dp[2] = {0, 0};
-        int item = 0;
+        int item = 0, done = 0;  // this stream's tiles before the item
         for (int left = tiles; left > 0 && ok; item++) {
             const int n = here(left);
             const bool whole = cu.t == 0, end = cu.t + n == cu.s.tiles;
@@ -1416,7 +1430,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             const int row = cu.rt * S::RT + (S::DUAL ? w * 128 : 0) + i, nd = row / a.group, head = cu.g * a.group + row % a.group;
             const bool used = row < a.rows && nd < cu.s.cnt;
             {
-                constexpr int QN = CH / LEAD, BATCH = QN < 8 ? QN : 8;
+                constexpr int QN = CH / STEP, BATCH = QN < 8 ? QN : 8;
                 const int c0 = S::DUAL ? 0 : w * QN;
                 const uint4 *const q = reinterpret_cast<const uint4 *>((const uint16_t *)d.q + cu.b * d.q_stride[0] +
                                                                        nd * d.q_stride[1] + head * d.q_stride[2]) + c0;
@@ -1440,7 +1454,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             if (lane == 0) mbar_arrive(&qfull);
             const uint64_t *const words = d.mask + ((size_t)cu.b * d.n_nodes + (used ? nd : 0)) * a.words;
             float m = -__FLT_MAX__, l = 0.f;
-            for (int t = S::DUAL ? 0 : w; t < n && ok; t += LEAD) {
+            int step = done;
+            for (int t = S::DUAL ? 0 : w; t < n && ok; t += STEP, step++) {
                 const bool node = cu.t + t >= cu.s.cache_tiles;
                 const int r0 = (node ? cu.t + t - cu.s.cache_tiles : cu.t + t) * KT;
                 const int valid = (node ? cu.s.cnt : cu.s.len) - r0;
@@ -1453,16 +1468,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                         see[k] = v >= 64 ? ~0ull : v > 0 ? (1ull << v) - 1 : 0;
                         if (node) see[k] = used && v > 0 ? see[k] & words[r0 / 64 + k] : 0;
                     }
-                ok = mbar_wait(&sfull[w], sp, a.err);
-                ok = __all_sync(DS_FULL, ok);
-                sp ^= 1;
+                ok = __all_sync(DS_FULL, tc_wait(&sfull[w][step & 1], step >> 1 & 1, a.err));
                 if (!ok) break;
                 tc_fence_after();
+                const uint32_t ts = tl + S::TS + (2 * w + (step & 1)) * KT;
+                uint32_t pk[KT / 2];
                 // The weights of the tile with the row's m so far. Their sum
                 // tells whether m still serves: only a tile that starts a row or
                 // passes 2^10 is done again with its true maximum. (A weight is
                 // at most 2^10, and m is never above the row's maximum.)
-                bool again = t < LEAD;
+                bool again = t < STEP;
                 float lt;
                 for (int pass = 0;; pass++) {
                     const bool look = __any_sync(DS_FULL, again);
@@ -1480,7 +1495,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                         const float f = again && mt > m ? ex2((m - mt) * c) : 1.f;
                         if (again && mt > m) m = mt;
                         l *= f;
-                        if (t >= LEAD)
+                        if (t >= STEP) {
+                            // (the last tile's product has to be in O)
+                            ok = __all_sync(DS_FULL, tc_wait(&pvdone[w], (step - 1) & 1, a.err));
+                            tc_fence_after();
 #pragma unroll 1
                             for (int k = 0; k < HD / 32; k++) {
                                 tmem_ld32(to + 32 * k, v);
@@ -1488,6 +1506,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                                 for (int e = 0; e < 32; e++) v[e] *= f;
                                 tmem_st32(to + 32 * k, v);
                             }
+                        }
                         again = false;
                         pass = 1;
                     }
@@ -1502,13 +1521,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
 #pragma unroll
                             for (int e = 0; e < 16; e++) v[e] = b >> e & 1 ? v[e] : 0.f;
                         }
-                        uint32_t pk[8];
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
                             s[e & 3] += v[2 * e] + v[2 * e + 1];
-                            pk[e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
+                            pk[8 * k + e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
                         }
-                        tmem_st8_start(tp + 8 * k, pk);
                     };
                     float x[16], y[16];
                     tmem_ld16_start(ts, x);
@@ -1521,23 +1538,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                         if (k + 2 < KT / 16) tmem_ld16_start(ts + 16 * k + 32, x);
                         weigh(y, k + 1);
                     }
-                    tmem_st_wait();
                     lt = (s[0] + s[1]) + (s[2] + s[3]);
                     if (pass == 1) break;
                     again = !(lt <= 1024.f);
                 }
                 l += lt;
+                tmem_st32u(ts, pk);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&pfull[w]);
+                if (lane == 0) mbar_arrive(&pfull[w][step & 1]);
             }
             // the results: a stream's own rows, or the streams' joined, each
             // group half of the dimensions
             const bool both = S::DUAL || n > 1;
-            if (ok) ok = mbar_wait(&odone[0], dp[0], a.err);
-            dp[0] ^= 1;
-            if (ok && both) ok = mbar_wait(&odone[1], dp[1], a.err);
-            if (both) dp[1] ^= 1;
+            done = step;
+            if (ok) ok = tc_wait(&odone[0], item & 1, a.err);
+            if (ok) ok = tc_wait(&odone[1], item & 1, a.err);
             ok = __all_sync(DS_FULL, ok);
             tc_fence_after();
             float mm = fmaxf(m * c, -__FLT_MAX__), ll = l, f0 = 1.f, f1 = 0.f;
@@ -1557,7 +1573,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 const size_t slot = (size_t)blockIdx.x * 2 + whole;
                 const int r = (S::DUAL ? w * 128 : 0) + i;
 #pragma unroll 1
-                for (int k = 0; k < HD / 32 / LEAD; k++) {
+                for (int k = 0; k < HD / 32 / STEP; k++) {
                     const int c0 = 32 * (k + (S::DUAL ? 0 : w * (HD / 64)));
                     __syncwarp();
                     float v[32];
@@ -1614,7 +1630,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == TC_THREADS / 32 - 1) tmem_dealloc(tmem, 512);
+    if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
 // The items that several CTAs had parts of. Parts are [row][dimension] with
