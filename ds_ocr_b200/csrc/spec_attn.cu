@@ -1118,8 +1118,8 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
 // 60 cycles a product, which one warp could not do for both), the next tile's
 // S before this one's P is there. m is the row's maximum of its first tile,
 // or of a later one whose weights passed 2^10, so that O is rarely rescaled.
-// Two producer warps bring K and V rows into a ring of units in the 128-byte
-// swizzle, in the order the products take them.
+// Two producer warps bring K and V rows into a ring each (of K and of V, or of
+// the streams) in the 128-byte swizzle, in the order the products take them.
 constexpr int TC_SOFTMAX = 256, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 64;
 constexpr uint32_t TC_DHI = 64u | (1u << 14) | (2u << 29);  // descriptors' high word: 1024 B between 8-row atoms, 128-byte swizzle
 template <int HD_, bool DUAL_, int QT_> struct SaMany {
@@ -1130,15 +1130,16 @@ template <int HD_, bool DUAL_, int QT_> struct SaMany {
     static constexpr int SUB = KT * 128;           // 64 dimensions of a unit
     static constexpr int UNIT = KT * HD * 2;       // 16 KB, 8 KB for head_dim 64
     static constexpr int QSUB = 128 * 128, QBLOCK = QSUB * (HD / 64);
-    static constexpr int UNITS = HD == 64 ? 16 : DUAL ? 9 : 10;
-    static constexpr int RING = DUAL ? UNITS : UNITS / 2;  // units of a ring: one ring, or one a stream
+    static constexpr int UNITS = HD == 64 ? 16 : DUAL ? 8 : 10;
+    static constexpr int RING = UNITS / 2;         // two rings: of K and of V (DUAL), or of the streams
     static constexpr int SMEM = RT / 128 * QBLOCK + UNITS * UNIT + 1024;
     static constexpr int PER_SM = 1;
     // tensor-memory columns: S (two buffers a stream, P in the first half of each), O
     static constexpr uint32_t TS = 0, TO = 4 * KT;
     static_assert(TO + 2 * HD <= 512, "tensor memory");
-    // a ring's units of an item with n tiles: K of two tiles, then V and K in
-    // turn. The place of K and V of tile t, and what is at a place.
+    // a stream's ring holds, of an item with n of its tiles, K of two tiles,
+    // then V and K in turn. The place of K and V of tile t, and what is at a
+    // place.
     static __device__ __forceinline__ int place_k(int t) { return t < 2 ? t : 2 * t - 1; }
     static __device__ __forceinline__ int place_v(int t, int n) { return min(2, n) + t + min(t, max(0, n - 2)); }
     static __device__ __forceinline__ int at(int place, int n, int &kv) {
@@ -1148,6 +1149,9 @@ template <int HD_, bool DUAL_, int QT_> struct SaMany {
     }
 };
 
+__device__ __forceinline__ void mbar_arrive_n(uint64_t *bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0], %1;" :: "r"(smem_u32(bar)), "r"(n) : "memory");
+}
 // A wait that gives up after two seconds: the failure is recorded in *err (if
 // given) and everyone leaves.
 __device__ __forceinline__ bool tc_wait(uint64_t *bar, uint32_t parity, unsigned *err) {
@@ -1219,7 +1223,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int u = 0; u < NU; u++) {
-            mbar_init(&full[u], TC_PRODUCERS);
+            mbar_init(&full[u], 32);
             mbar_init(&empty[u], S::DUAL ? 2 : 1);
         }
         mbar_init(&qfull, TC_SOFTMAX / 32);
@@ -1253,34 +1257,34 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
 
     constexpr int MMA_WARP = (TC_SOFTMAX + TC_PRODUCERS) / 32;
     if (warp >= TC_SOFTMAX / 32 && warp < MMA_WARP) {
-        // ---- producers: K and V rows, 16 bytes a thread at a time ----
-        const int p = tid - TC_SOFTMAX, cc = p % CH, rr = p / CH;
-        constexpr int RS = TC_PRODUCERS / CH;
-        constexpr int RINGS = S::DUAL ? 1 : 2;
-        int item = 0, units[RINGS] = {};  // units so far
-        auto load = [&](int ring_, int t, int kv) {
+        // ---- producers: a warp a ring; whole tiles by TMA, others 16 bytes a
+        // lane at a time ----
+        const int rg = __shfl_sync(DS_FULL, warp - TC_SOFTMAX / 32, 0), cc = lane % CH, rr = lane / CH;
+        constexpr int RS = 32 / CH;
+        int item = 0, units = 0;  // units so far
+        auto load = [&](int t, int kv) {
+            const int slot = rg * S::RING + units % S::RING;
+            ok = __all_sync(DS_FULL, ok && tc_wait(&empty[slot], (units / S::RING & 1) ^ 1, a.err));
             if (!ok) return;
-            const int u = units[ring_], slot = ring_ * S::RING + u % S::RING;
-            ok = tc_wait(&empty[slot], (u / S::RING & 1) ^ 1, a.err);
-            if (!ok) return;
-            units[ring_]++;
-            SaCursor c = cu;
-            c.t += t;
+            units++;
             uint8_t *const unit = ring + slot * S::UNIT;
-            if (args.mapped && (c.t + 1) * KT <= c.s.len) {
-                if (p == 0) {
+            if (args.mapped && (cu.t + t + 1) * KT <= cu.s.len) {
+                if (elect_one()) {
                     const int *const dim = args.dim[kv];
-                    auto at = [&](int k) { return dim[0] == k ? c.t * KT : dim[1] == k ? c.g : c.b; };
-                    const int y = at(1), z = at(2), v = at(3);
+                    const int r0 = (cu.t + t) * KT;
+                    const int y = dim[0] == 1 ? r0 : dim[1] == 1 ? cu.g : cu.b, z = dim[0] == 2 ? r0 : dim[1] == 2 ? cu.g : cu.b,
+                              v = dim[0] == 3 ? r0 : dim[1] == 3 ? cu.g : cu.b;
+                    mbar_arrive_n(&full[slot], 31);
                     mbar_expect_tx(&full[slot], S::UNIT);
 #pragma unroll
                     for (int k = 0; k < HD / 64; k++)
                         tma_load_4d(unit + k * S::SUB, &args.map[kv], 64 * k, y, z, v, &full[slot]);
-                } else {
-                    mbar_arrive(&full[slot]);
                 }
+                __syncwarp();
                 return;
             }
+            SaCursor c = cu;
+            c.t += t;
             const SaTile src = sa_tile<KT>(d, c);
             const uint16_t *x = src.base[kv][0] + rr * src.step[kv] + 8 * cc;
             const uint32_t dst = smem_u32(unit) + (cc >> 3) * S::SUB;
@@ -1300,6 +1304,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 cp_commit();
                 cp_wait<0>();
                 constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+#pragma unroll 4
                 for (int r = rr; r < min(KT, src.valid); r += RS) {
                     uint4 *const v = reinterpret_cast<uint4 *>(unit + (cc >> 3) * S::SUB + at(r));
                     uint4 u = *v;
@@ -1323,25 +1328,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         };
         for (int left = tiles; left > 0 && ok; item++) {
             const int n = here(left);
-            const int steps = S::DUAL ? n : (n + 1) >> 1;
-            for (int place = 0; place < 2 * steps; place++)
-#pragma unroll
-                for (int w = 0; w < RINGS; w++) {
-                    const int mine = w ? n >> 1 : steps;
-                    if (place >= 2 * mine) continue;
+            if (S::DUAL) {
+                for (int t = 0; t < n; t++) load(t, rg);
+            } else {
+                const int mine = (n - rg + 1) >> 1;
+                for (int place = 0; place < 2 * mine; place++) {
                     int kv;
                     const int t = S::at(place, mine, kv);
-                    load(w, S::DUAL ? t : 2 * t + w, kv);
+                    load(2 * t + rg, kv);
                 }
+            }
             left -= n;
             if (left > 0) to_next_item();
         }
         cp_commit();
         cp_wait<0>();
-        if (!ok && p == 0)  // a wait gave up: what was issued arrives before the memory goes
-            for (int w = 0; w < RINGS; w++)
-                for (int u = max(0, units[w] - S::RING); u < units[w]; u++)
-                    tc_wait(&full[w * S::RING + u % S::RING], u / S::RING & 1, nullptr);
+        if (!ok)  // a wait gave up: what was issued arrives before the memory goes
+            for (int u = max(0, units - S::RING); u < units; u++) tc_wait(&full[rg * S::RING + u % S::RING], u / S::RING & 1, nullptr);
     } else if (warp >= MMA_WARP) {
         // ---- stream w's products: the warp waits, one lane issues ----
         const int w = __shfl_sync(DS_FULL, warp - MMA_WARP, 0);
@@ -1351,11 +1354,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         const uint32_t ring_v = (((smem_u32(ring) >> 4) & 0x3fffu) | ((S::SUB >> 4) << 16));
         const uint32_t q = ((smem_u32(smem + (S::DUAL ? w * S::QBLOCK : 0)) >> 4) & 0x3fffu) | (1u << 16);
         const uint32_t ts = tmem + S::TS + w * 2 * KT, to = tmem + S::TO + w * HD;
-        int done = 0;  // this stream's tiles before the item (two units of its ring each)
+        int done = 0;  // this stream's tiles before the item
         auto wait = [&](uint64_t *bar, uint32_t ph) { ok = __all_sync(DS_FULL, ok && tc_wait(bar, ph, a.err)); };
-        // a unit of the ring, of the item's tile t
-        auto take = [&](int place, int t) {
-            const int u = 2 * done + place, s = (S::DUAL ? 0 : w * S::RING) + u % S::RING;
+        // unit u of ring rg, of the item's tile t
+        auto take = [&](int rg, int u, int t) {
+            const int s = rg * S::RING + u % S::RING;
             wait(&full[s], u / S::RING & 1);
             // copies that are not TMA's are ordinary writes, the products'
             // reads are not
@@ -1365,7 +1368,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         for (int left = tiles, item = 0; left > 0 && ok; item++) {
             const int n = here(left), steps = S::DUAL ? n : (n - w + 1) >> 1;
             auto qk = [&](int j) {
-                const int t = S::DUAL ? j : 2 * j + w, s = take(S::place_k(j), t), buf = (done + j) & 1;
+                const int t = S::DUAL ? j : 2 * j + w, buf = (done + j) & 1;
+                const int s = S::DUAL ? take(0, done + j, t) : take(w, 2 * done + S::place_k(j), t);
                 if (!ok) return;
                 tc_fence_after();
                 const uint32_t k = ring_k + s * (S::UNIT >> 4);
@@ -1382,7 +1386,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             wait(&qfull, item & 1);
             for (int j = 0; j < min(2, steps) && ok; j++) qk(j);
             for (int j = 0; j < steps && ok; j++) {
-                const int t = S::DUAL ? j : 2 * j + w, s = take(S::place_v(j, steps), t), buf = (done + j) & 1;
+                const int t = S::DUAL ? j : 2 * j + w, buf = (done + j) & 1;
+                const int s = S::DUAL ? take(1, done + j, t) : take(w, 2 * done + S::place_v(j, steps), t);
                 wait(&pfull[w][buf], (done + j) >> 1 & 1);
                 if (!ok) break;
                 tc_fence_after();
@@ -1421,37 +1426,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         const float c = fabsf(a.scale2);
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // the sign goes to the queries
         int item = 0, done = 0;  // this stream's tiles before the item
+        // the queries of an item's rows, swizzled as K is: a row a thread, or
+        // half a row (all loads first: stores in between would hold them up)
+        constexpr int QN = CH / STEP;
+        uint4 qu[QN];
+        auto q_load = [&]() {
+            const int row = cu.rt * S::RT + (S::DUAL ? w * 128 : 0) + i;
+            const uint4 *const q = reinterpret_cast<const uint4 *>((const uint16_t *)d.q + cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
+                                                                   (cu.g * a.group + row % a.group) * d.q_stride[2]) + (S::DUAL ? 0 : w * QN);
+#pragma unroll
+            for (int k = 0; k < QN; k++) qu[k] = row < a.rows ? q[k] : make_uint4(0, 0, 0, 0);
+        };
+        auto q_store = [&]() {
+            uint8_t *const q = smem + (S::DUAL ? w * S::QBLOCK : 0) + i * 128;
+#pragma unroll
+            for (int k = 0; k < QN; k++) {
+                const int ch = (S::DUAL ? 0 : w * QN) + k;
+                qu[k].x ^= flip, qu[k].y ^= flip, qu[k].z ^= flip, qu[k].w ^= flip;
+                *reinterpret_cast<uint4 *>(q + (ch >> 3) * S::QSUB + (((ch & 7) ^ (i & 7)) << 4)) = qu[k];
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&qfull);
+        };
         for (int left = tiles; left > 0 && ok; item++) {
             const int n = here(left);
             const bool whole = cu.t == 0, end = cu.t + n == cu.s.tiles;
-            // the queries of the item's rows, swizzled as K is: a row a thread,
-            // or half a row (all loads first: stores in between would hold
-            // them up)
             const int row = cu.rt * S::RT + (S::DUAL ? w * 128 : 0) + i, nd = row / a.group, head = cu.g * a.group + row % a.group;
             const bool used = row < a.rows && nd < cu.s.cnt;
-            {
-                constexpr int QN = CH / STEP, BATCH = QN < 8 ? QN : 8;
-                const int c0 = S::DUAL ? 0 : w * QN;
-                const uint4 *const q = reinterpret_cast<const uint4 *>((const uint16_t *)d.q + cu.b * d.q_stride[0] +
-                                                                       nd * d.q_stride[1] + head * d.q_stride[2]) + c0;
-                uint8_t *const to_s = smem + (S::DUAL ? w * S::QBLOCK : 0) + i * 128;
-#pragma unroll
-                for (int k0 = 0; k0 < QN; k0 += BATCH) {
-                    uint4 u[BATCH];
-#pragma unroll
-                    for (int k = 0; k < BATCH; k++) u[k] = row < a.rows ? q[k0 + k] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                    for (int k = 0; k < BATCH; k++) {
-                        const int ch = c0 + k0 + k;
-                        u[k].x ^= flip, u[k].y ^= flip, u[k].z ^= flip, u[k].w ^= flip;
-                        *reinterpret_cast<uint4 *>(to_s + (ch >> 3) * S::QSUB + (((ch & 7) ^ (i & 7)) << 4)) = u[k];
-                    }
-                }
+            if (item == 0) {
+                q_load();
+                q_store();
             }
-            fence_proxy_async();
-            tc_fence_before();  // (the last item's results have been read)
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&qfull);
             const uint64_t *const words = d.mask + ((size_t)cu.b * d.n_nodes + (used ? nd : 0)) * a.words;
             float m = -__FLT_MAX__, l = 0.f;
             int step = done;
@@ -1512,31 +1518,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                     }
                     const float mc = fmaxf(m * c, -__FLT_MAX__);
                     float s[4] = {0.f, 0.f, 0.f, 0.f};
-                    // 16 columns while the next are read
-                    auto weigh = [&](float (&v)[16], int k) {
+                    float v[KT];
+                    tmem_ld64(ts, v);
 #pragma unroll
-                        for (int e = 0; e < 16; e++) v[e] = ex2(__fmaf_rn(v[e], c, -mc));
-                        if (masked) {
-                            const uint32_t b = (uint32_t)(see[k >> 2] >> (16 * (k & 3)));
+                    for (int e = 0; e < KT; e++) v[e] = ex2(__fmaf_rn(v[e], c, -mc));
+                    if (masked) {
 #pragma unroll
-                            for (int e = 0; e < 16; e++) v[e] = b >> e & 1 ? v[e] : 0.f;
-                        }
+                        for (int e = 0; e < KT; e++) v[e] = see[0] >> e & 1 ? v[e] : 0.f;
+                    }
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            s[e & 3] += v[2 * e] + v[2 * e + 1];
-                            pk[8 * k + e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
-                        }
-                    };
-                    float x[16], y[16];
-                    tmem_ld16_start(ts, x);
-#pragma unroll
-                    for (int k = 0; k < KT / 16; k += 2) {
-                        tmem_ld16_wait(x);
-                        tmem_ld16_start(ts + 16 * k + 16, y);
-                        weigh(x, k);
-                        tmem_ld16_wait(y);
-                        if (k + 2 < KT / 16) tmem_ld16_start(ts + 16 * k + 32, x);
-                        weigh(y, k + 1);
+                    for (int e = 0; e < KT / 2; e++) {
+                        s[e & 3] += v[2 * e] + v[2 * e + 1];
+                        pk[e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
                     }
                     lt = (s[0] + s[1]) + (s[2] + s[3]);
                     if (pass == 1) break;
@@ -1552,9 +1545,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             // group half of the dimensions
             const bool both = S::DUAL || n > 1;
             done = step;
+            // the next item's queries come in while this one's products end,
+            // and go to shared memory as soon as they have: its first S are
+            // ready when this one's results are written. (Its first O waits
+            // for weights, which come after the barrier below.)
+            const SaCursor it = cu;
+            left -= n;
+            if (left > 0) {
+                to_next_item();
+                q_load();
+            }
             if (ok) ok = tc_wait(&odone[0], item & 1, a.err);
             if (ok) ok = tc_wait(&odone[1], item & 1, a.err);
             ok = __all_sync(DS_FULL, ok);
+            if (ok && left > 0) q_store();
             tc_fence_after();
             float mm = fmaxf(m * c, -__FLT_MAX__), ll = l, f0 = 1.f, f1 = 0.f;
             if (!S::DUAL) {
@@ -1589,10 +1593,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                         }
                     }
                     if (bad && used)  // see the producers
-                        for (int j = 0; j < cu.s.cnt; j++)
+                        for (int j = 0; j < it.s.cnt; j++)
                             if (words[j >> 6] >> (j & 63) & 1) {
-                                const uint16_t *x = (const uint16_t *)d.tree_v + cu.b * d.tree_v_stride[0] +
-                                                    cu.g * d.tree_v_stride[1] + j * d.tree_v_stride[2] + c0;
+                                const uint16_t *x = (const uint16_t *)d.tree_v + it.b * d.tree_v_stride[0] +
+                                                    it.g * d.tree_v_stride[1] + j * d.tree_v_stride[2] + c0;
 #pragma unroll
                                 for (int e = 0; e < 32; e++) {
                                     const float y = F16 ? __half2float(__ushort_as_half(x[e])) : __uint_as_float((uint32_t)x[e] << 16);
@@ -1603,7 +1607,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                     for (int e = 0; e < 32; e++) v[e] = alone && none ? 0.f : v[e] * inv;
                     if (row < a.rows) {
                         if (alone) {
-                            uint16_t *o = (uint16_t *)d.out + cu.b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c0;
+                            uint16_t *o = (uint16_t *)d.out + it.b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c0;
 #pragma unroll
                             for (int e = 0; e < 32; e += 8)
                                 *reinterpret_cast<uint4 *>(o + e) = make_uint4(pack2<F16>(v[e], v[e + 1]), pack2<F16>(v[e + 2], v[e + 3]),
@@ -1617,14 +1621,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 if (row < a.rows && (S::DUAL || w == 0)) {
                     if (!alone) a.ml[slot * S::RT + r] = make_float2(mm, ll);
                     else if (d.lse)
-                        d.lse[((size_t)cu.b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (mm + log2f(ll)) * 0.69314718f;
+                        d.lse[((size_t)it.b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (mm + log2f(ll)) * 0.69314718f;
                 }
             }
             // every reader of sh_ml, sh_bad and O is done; all go on or none
+            tc_fence_before();
             ok = bar_and(1, TC_SOFTMAX, ok);
             if (tid == 0) sh_bad[item & 15] = 0;
-            left -= n;
-            if (left > 0) to_next_item();
         }
     }
     tc_fence_before();
