@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "ctx.h"
@@ -1106,13 +1107,13 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
 // ---- many rows: tcgen05 ----------------------------------------------------------
 // 16-bit types with more than 32 rows. The 128 query rows of a block are the
 // rows of tcgen05.mma (M = 128, accumulators in tensor memory); two softmax
-// groups of 128 threads, a row each, work on two streams:
+// groups of 256 threads, two a row, work on two streams:
 //   DUAL (more than 128 rows): the streams are two blocks of rows that share
 //        every K and V tile;
 //   else: one block of rows, the streams take the even and the odd tiles, and
 //        their results are joined where they are written.
 // Per stream and tile of 64 keys: S = Q K^T (both from shared memory) into one
-// of two buffers in tensor memory; a thread reads its row of S, takes
+// of two buffers in tensor memory; a thread reads half a row of S, takes
 // 2^(S - m) and stores it, in the place of S, as P; O += P V with P as the A
 // operand. A warp of its own issues a stream's products (issuing takes about
 // 60 cycles a product, which one warp could not do for both), the next tile's
@@ -1120,7 +1121,8 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
 // or of a later one whose weights passed 2^10, so that O is rarely rescaled.
 // Two producer warps bring K and V rows into a ring each (of K and of V, or of
 // the streams) in the 128-byte swizzle, in the order the products take them.
-constexpr int TC_SOFTMAX = 256, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 64;
+constexpr int TC_SOFTMAX = 512, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 64;
+constexpr int TC_ALL = 9;  // barrier of the softmax threads (1 .. 8: of the two warps of 32 rows)
 constexpr uint32_t TC_DHI = 64u | (1u << 14) | (2u << 29);  // descriptors' high word: 1024 B between 8-row atoms, 128-byte swizzle
 template <int HD_, bool DUAL_, int QT_> struct SaMany {
     static constexpr int HD = HD_, QT = QT_, PL = 1;
@@ -1182,7 +1184,15 @@ __device__ __forceinline__ void cp_arrive(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(n) : "memory"); }
-// ... returning whether all of them passed `ok`.
+// ... returning whether any of them passed `x`.
+__device__ __forceinline__ bool bar_or(int id, int n, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((uint32_t)x), "r"(id), "r"(n) : "memory");
+    return r != 0;
+}
+// ... whether all of them passed `ok`.
 __device__ __forceinline__ bool bar_and(int id, int n, bool ok) {
     uint32_t r;
     asm volatile(
@@ -1216,8 +1226,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *const ring = smem + S::RT / 128 * S::QBLOCK;
     __shared__ uint64_t full[NU], empty[NU], qfull, sfull[2][2], pfull[2][2], pvdone[2], odone[2], drain[2];
+    __shared__ uint64_t second;  // an item's stream 1 may begin
     __shared__ uint32_t tmem_base;
-    __shared__ float2 sh_ml[2][128];
+    __shared__ float2 sh_ml[2][2][128];  // by stream, half and row: maximum and sum
+    __shared__ float sh_mx[2][2][128];
     __shared__ int sh_bad[16];  // by item: a node's V holds NaN or infinities
     const ds_cuda_tree_attention_t &d = a.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1227,11 +1239,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             mbar_init(&empty[u], S::DUAL ? 2 : 1);
         }
         mbar_init(&qfull, TC_SOFTMAX / 32);
+        mbar_init(&second, 8);
         for (int w = 0; w < 2; w++) {
             mbar_init(&sfull[w][0], 1);
             mbar_init(&sfull[w][1], 1);
-            mbar_init(&pfull[w][0], 4);
-            mbar_init(&pfull[w][1], 4);
+            mbar_init(&pfull[w][0], 8);
+            mbar_init(&pfull[w][1], 8);
             mbar_init(&pvdone[w], 1);
             mbar_init(&odone[w], 1);
             mbar_init(&drain[w], 1);
@@ -1303,22 +1316,29 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 // them when those are written.
                 cp_commit();
                 cp_wait<0>();
-                constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+                // (an exponent of all ones carries into the bit above it)
+                constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
+                auto scan = [&](auto found) {
 #pragma unroll 4
-                for (int r = rr; r < min(KT, src.valid); r += RS) {
-                    uint4 *const v = reinterpret_cast<uint4 *>(unit + (cc >> 3) * S::SUB + at(r));
-                    uint4 u = *v;
-                    bool bad = false;
+                    for (int r = rr; r < min(KT, src.valid); r += RS) {
+                        uint4 *const v = reinterpret_cast<uint4 *>(unit + (cc >> 3) * S::SUB + at(r));
+                        const uint4 u = *v;
+                        if ((((u.x & E) + ONE) | ((u.y & E) + ONE) | ((u.z & E) + ONE) | ((u.w & E) + ONE)) & 0x80008000u) found(v, u);
+                    }
+                };
+                bool bad = false;
+                scan([&](uint4 *, uint4) { bad = true; });
+                if (bad) {
+                    scan([&](uint4 *v, uint4 u) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint32_t &w = (&u.x)[k];
-                        if ((w & E) == E) w &= 0xffff0000u, bad = true;
-                        if ((w >> 16 & E) == E) w &= 0xffffu, bad = true;
-                    }
-                    if (bad) {
+                        for (int k = 0; k < 4; k++) {
+                            uint32_t &x = (&u.x)[k];
+                            const uint32_t top = ((x & E) + ONE) & 0x80008000u;
+                            x &= ~((top >> 15) * 0xffffu);
+                        }
                         *v = u;
-                        *reinterpret_cast<volatile int *>(&sh_bad[item & 15]) = 1;
-                    }
+                    });
+                    *reinterpret_cast<volatile int *>(&sh_bad[item & 15]) = 1;
                 }
                 fence_proxy_async();
                 mbar_arrive(&full[slot]);
@@ -1419,21 +1439,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             tc_wait(&drain[w], 0, nullptr);
         }
     } else {
-        // ---- softmax: row i of stream w ----
-        const int w = warp >> 2, i = tid & 127;
+        // ---- softmax: row i of stream w, keys (and dimensions) of half h ----
+        const int w = warp >> 3, h = warp >> 2 & 1, i = 32 * (warp & 3) + lane, pair = 1 + 4 * w + (warp & 3);
         const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t to = tl + S::TO + w * HD;
         const float c = fabsf(a.scale2);
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;  // the sign goes to the queries
+        constexpr int PARTS = S::DUAL ? 2 : 4;                    // threads of a row
+        const int part = S::DUAL ? h : 2 * w + h;
         int item = 0, done = 0;  // this stream's tiles before the item
-        // the queries of an item's rows, swizzled as K is: a row a thread, or
-        // half a row (all loads first: stores in between would hold them up)
-        constexpr int QN = CH / STEP;
+        // the queries of an item's rows, swizzled as K is (all loads first:
+        // stores in between would hold them up)
+        constexpr int QN = CH / PARTS;
         uint4 qu[QN];
         auto q_load = [&]() {
             const int row = cu.rt * S::RT + (S::DUAL ? w * 128 : 0) + i;
             const uint4 *const q = reinterpret_cast<const uint4 *>((const uint16_t *)d.q + cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
-                                                                   (cu.g * a.group + row % a.group) * d.q_stride[2]) + (S::DUAL ? 0 : w * QN);
+                                                                   (cu.g * a.group + row % a.group) * d.q_stride[2]) + part * QN;
 #pragma unroll
             for (int k = 0; k < QN; k++) qu[k] = row < a.rows ? q[k] : make_uint4(0, 0, 0, 0);
         };
@@ -1441,7 +1463,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             uint8_t *const q = smem + (S::DUAL ? w * S::QBLOCK : 0) + i * 128;
 #pragma unroll
             for (int k = 0; k < QN; k++) {
-                const int ch = (S::DUAL ? 0 : w * QN) + k;
+                const int ch = part * QN + k;
                 qu[k].x ^= flip, qu[k].y ^= flip, qu[k].z ^= flip, qu[k].w ^= flip;
                 *reinterpret_cast<uint4 *>(q + (ch >> 3) * S::QSUB + (((ch & 7) ^ (i & 7)) << 4)) = qu[k];
             }
@@ -1461,88 +1483,101 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             const uint64_t *const words = d.mask + ((size_t)cu.b * d.n_nodes + (used ? nd : 0)) * a.words;
             float m = -__FLT_MAX__, l = 0.f;
             int step = done;
-            for (int t = S::DUAL ? 0 : w; t < n && ok; t += STEP, step++) {
-                const bool node = cu.t + t >= cu.s.cache_tiles;
-                const int r0 = (node ? cu.t + t - cu.s.cache_tiles : cu.t + t) * KT;
-                const int valid = (node ? cu.s.cnt : cu.s.len) - r0;
-                const bool masked = node || valid < KT;
-                uint64_t see[KT / 64];
-                if (masked)
-#pragma unroll
-                    for (int k = 0; k < KT / 64; k++) {
-                        const int v = valid - 64 * k;
-                        see[k] = v >= 64 ? ~0ull : v > 0 ? (1ull << v) - 1 : 0;
-                        if (node) see[k] = used && v > 0 ? see[k] & words[r0 / 64 + k] : 0;
-                    }
-                ok = __all_sync(DS_FULL, tc_wait(&sfull[w][step & 1], step >> 1 & 1, a.err));
-                if (!ok) break;
+            // (after a wait that gave up: on without waiting, through every
+            // barrier, to the item's end)
+            auto tile = [&](auto masks, int t) {
+                constexpr bool MASKED = decltype(masks)::value;
+                const int buf = step & 1;
+                const uint32_t ts = tl + S::TS + (2 * w + buf) * KT;
+                uint32_t see = ~0u;
+                if (MASKED) {
+                    const bool node = cu.t + t >= cu.s.cache_tiles;
+                    const int r0 = (node ? cu.t + t - cu.s.cache_tiles : cu.t + t) * KT;
+                    const int valid = (node ? cu.s.cnt : cu.s.len) - r0 - 32 * h;  // of this half's keys
+                    see = valid >= 32 ? ~0u : valid > 0 ? (1u << valid) - 1 : 0;
+                    if (node) see = used && valid > 0 ? see & (uint32_t)(words[r0 / 64] >> (32 * h)) : 0;
+                }
+                ok = ok && tc_wait(&sfull[w][buf], step >> 1 & 1, a.err);
+                __syncwarp();
                 tc_fence_after();
-                const uint32_t ts = tl + S::TS + (2 * w + (step & 1)) * KT;
-                uint32_t pk[KT / 2];
-                // The weights of the tile with the row's m so far. Their sum
-                // tells whether m still serves: only a tile that starts a row or
-                // passes 2^10 is done again with its true maximum. (A weight is
-                // at most 2^10, and m is never above the row's maximum.)
-                bool again = t < STEP;
-                float lt;
-                for (int pass = 0;; pass++) {
-                    const bool look = __any_sync(DS_FULL, again);
-                    if (pass == 1 && !look) break;
-                    if (look) {
-                        float mt = -__FLT_MAX__, v[32];
-#pragma unroll 1
-                        for (int k = 0; k < KT / 32; k++) {
-                            tmem_ld32(ts + 32 * k, v);
-                            const uint32_t b = masked ? (uint32_t)(see[k >> 1] >> (32 * (k & 1))) : ~0u;
+                float v[32], lt;
+                uint32_t pk[16];
+                tmem_ld32(ts + 32 * h, v);
+                // the row's maximum over both halves (and what m was)
+                auto look = [&]() {
+                    float mt = m;
 #pragma unroll
-                            for (int e = 0; e < 32; e++)
-                                if (b >> e & 1) mt = fmaxf(mt, v[e]);
-                        }
-                        const float f = again && mt > m ? ex2((m - mt) * c) : 1.f;
-                        if (again && mt > m) m = mt;
-                        l *= f;
-                        if (t >= STEP) {
-                            // (the last tile's product has to be in O)
-                            ok = __all_sync(DS_FULL, tc_wait(&pvdone[w], (step - 1) & 1, a.err));
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int k = 0; k < HD / 32; k++) {
-                                tmem_ld32(to + 32 * k, v);
-#pragma unroll
-                                for (int e = 0; e < 32; e++) v[e] *= f;
-                                tmem_st32(to + 32 * k, v);
-                            }
-                        }
-                        again = false;
-                        pass = 1;
-                    }
+                    for (int e = 0; e < 32; e++)
+                        if (!MASKED || (see >> e & 1)) mt = fmaxf(mt, v[e]);
+                    sh_mx[w][h][i] = mt;
+                    bar_sync(pair, 64);
+                    m = fmaxf(mt, sh_mx[w][h ^ 1][i]);
+                };
+                // weights of the row's keys with m, their sum, and packed in pairs
+                auto weigh = [&]() {
                     const float mc = fmaxf(m * c, -__FLT_MAX__);
                     float s[4] = {0.f, 0.f, 0.f, 0.f};
-                    float v[KT];
-                    tmem_ld64(ts, v);
 #pragma unroll
-                    for (int e = 0; e < KT; e++) v[e] = ex2(__fmaf_rn(v[e], c, -mc));
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < KT; e++) v[e] = see[0] >> e & 1 ? v[e] : 0.f;
+                    for (int e = 0; e < 32; e++) {
+                        v[e] = ex2(__fmaf_rn(v[e], c, -mc));
+                        if (MASKED) v[e] = see >> e & 1 ? v[e] : 0.f;
                     }
 #pragma unroll
-                    for (int e = 0; e < KT / 2; e++) {
+                    for (int e = 0; e < 16; e++) {
                         s[e & 3] += v[2 * e] + v[2 * e + 1];
                         pk[e] = pack2<F16>(v[2 * e], v[2 * e + 1]);
                     }
                     lt = (s[0] + s[1]) + (s[2] + s[3]);
-                    if (pass == 1) break;
-                    again = !(lt <= 1024.f);
+                };
+                if (t < STEP) {
+                    // An item's stream 1 begins when stream 0 has its first
+                    // weights: half a step apart, one's waits, loads and stores
+                    // run beside the other's exponentials.
+                    look();
+                    if (w) ok = ok && tc_wait(&second, item & 1, a.err);
+                    __syncwarp();
+                    weigh();
+                    if (!w && lane == 0) mbar_arrive(&second);
+                } else {
+                    // The sum tells whether m still serves: a tile that passes
+                    // 2^10 in either half of any of the 32 rows is done again
+                    // with the true maxima. (So a weight is at most 2^10, and m
+                    // never above the row's maximum.)
+                    weigh();
+                    if (bar_or(pair, 64, !(lt <= 1024.f))) {
+                        const float was = m;
+                        tmem_ld32(ts + 32 * h, v);
+                        look();
+                        const float f = m > was ? ex2((was - m) * c) : 1.f;
+                        weigh();
+                        l *= f;
+                        // (the last tile's product has to be in O)
+                        ok = ok && tc_wait(&pvdone[w], (step - 1) & 1, a.err);
+                        __syncwarp();
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int k = 0; k < HD / 2; k += 16) {
+                            float y[16];
+                            tmem_ld16(to + h * (HD / 2) + k, y);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) y[e] *= f;
+                            tmem_st16f(to + h * (HD / 2) + k, y);
+                        }
+                    }
                 }
                 l += lt;
-                tmem_st32u(ts, pk);
+                tmem_st16(ts + 16 * h, pk);  // over S, which both halves have read
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&pfull[w][step & 1]);
-            }
-            // the results: a stream's own rows, or the streams' joined, each
-            // group half of the dimensions
+                if (lane == 0) mbar_arrive(&pfull[w][buf]);
+                step++;
+            };
+            const int plain = min(n, cu.s.len / KT - cu.t);  // tiles without a mask
+            int t = S::DUAL ? 0 : w;
+            for (; t < plain; t += STEP) tile(std::false_type(), t);
+            for (; t < n; t += STEP) tile(std::true_type(), t);
+            // the results: a stream's own rows, or the streams' joined; a row's
+            // threads take a share of the dimensions each
             const bool both = S::DUAL || n > 1;
             done = step;
             // the next item's queries come in while this one's products end,
@@ -1555,20 +1590,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 to_next_item();
                 q_load();
             }
+            sh_ml[w][h][i] = make_float2(fmaxf(m * c, -__FLT_MAX__), l);
             if (ok) ok = tc_wait(&odone[0], item & 1, a.err);
             if (ok) ok = tc_wait(&odone[1], item & 1, a.err);
             ok = __all_sync(DS_FULL, ok);
             if (ok && left > 0) q_store();
             tc_fence_after();
-            float mm = fmaxf(m * c, -__FLT_MAX__), ll = l, f0 = 1.f, f1 = 0.f;
-            if (!S::DUAL) {
-                sh_ml[w][i] = make_float2(mm, l);
-                bar_sync(1, TC_SOFTMAX);
-                const float2 x = sh_ml[0][i], y = both ? sh_ml[1][i] : make_float2(-__FLT_MAX__, 0.f);
+            bar_sync(TC_ALL, TC_SOFTMAX);
+            float mm, ll, f0 = 1.f, f1 = 0.f;
+            if (S::DUAL) {
+                mm = sh_ml[w][0][i].x;
+                ll = sh_ml[w][0][i].y + sh_ml[w][1][i].y;
+            } else {
+                const float2 x = sh_ml[0][0][i], y = both ? sh_ml[1][0][i] : make_float2(-__FLT_MAX__, 0.f);
                 mm = fmaxf(x.x, y.x);
                 f0 = ex2(x.x - mm);
                 f1 = ex2(y.x - mm);
-                ll = x.y * f0 + y.y * f1;
+                ll = (x.y + sh_ml[0][1][i].y) * f0;
+                if (both) ll += (y.y + sh_ml[1][1][i].y) * f1;
             }
             if (ok) {
                 const bool alone = whole && end, none = !used || ll == 0.f;
@@ -1577,19 +1616,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 const size_t slot = (size_t)blockIdx.x * 2 + whole;
                 const int r = (S::DUAL ? w * 128 : 0) + i;
 #pragma unroll 1
-                for (int k = 0; k < HD / 32 / STEP; k++) {
-                    const int c0 = 32 * (k + (S::DUAL ? 0 : w * (HD / 64)));
+                for (int k = 0; k < HD / PARTS; k += 16) {
+                    const int c0 = part * (HD / PARTS) + k;
                     __syncwarp();
-                    float v[32];
+                    float v[16];
                     if (S::DUAL) {
-                        tmem_ld32(to + c0, v);
+                        tmem_ld16(to + c0, v);
                     } else {
-                        tmem_ld32(tl + S::TO + c0, v);
+                        tmem_ld16(tl + S::TO + c0, v);
                         if (both) {
-                            float y[32];
-                            tmem_ld32(tl + S::TO + HD + c0, y);
+                            float y[16];
+                            tmem_ld16(tl + S::TO + HD + c0, y);
 #pragma unroll
-                            for (int e = 0; e < 32; e++) v[e] = v[e] * f0 + y[e] * f1;
+                            for (int e = 0; e < 16; e++) v[e] = v[e] * f0 + y[e] * f1;
                         }
                     }
                     if (bad && used)  // see the producers
@@ -1598,27 +1637,28 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                                 const uint16_t *x = (const uint16_t *)d.tree_v + it.b * d.tree_v_stride[0] +
                                                     it.g * d.tree_v_stride[1] + j * d.tree_v_stride[2] + c0;
 #pragma unroll
-                                for (int e = 0; e < 32; e++) {
+                                for (int e = 0; e < 16; e++) {
                                     const float y = F16 ? __half2float(__ushort_as_half(x[e])) : __uint_as_float((uint32_t)x[e] << 16);
                                     if (!isfinite(y)) v[e] += y;
                                 }
                             }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = alone && none ? 0.f : v[e] * inv;
+                    for (int e = 0; e < 16; e++) v[e] = alone && none ? 0.f : v[e] * inv;
                     if (row < a.rows) {
                         if (alone) {
                             uint16_t *o = (uint16_t *)d.out + it.b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c0;
 #pragma unroll
-                            for (int e = 0; e < 32; e += 8)
+                            for (int e = 0; e < 16; e += 8)
                                 *reinterpret_cast<uint4 *>(o + e) = make_uint4(pack2<F16>(v[e], v[e + 1]), pack2<F16>(v[e + 2], v[e + 3]),
                                                                                pack2<F16>(v[e + 4], v[e + 5]), pack2<F16>(v[e + 6], v[e + 7]));
                         } else {
+                            float *const o = a.part + (slot * HD + c0) * S::RT + r;  // [dimension][row]
 #pragma unroll
-                            for (int e = 0; e < 32; e++) a.part[(slot * HD + c0 + e) * S::RT + r] = v[e];  // [dimension][row]
+                            for (int e = 0; e < 16; e++) o[e * S::RT] = v[e];
                         }
                     }
                 }
-                if (row < a.rows && (S::DUAL || w == 0)) {
+                if (row < a.rows && (S::DUAL ? h == 0 : part == 0)) {
                     if (!alone) a.ml[slot * S::RT + r] = make_float2(mm, ll);
                     else if (d.lse)
                         d.lse[((size_t)it.b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (mm + log2f(ll)) * 0.69314718f;
@@ -1626,7 +1666,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             }
             // every reader of sh_ml, sh_bad and O is done; all go on or none
             tc_fence_before();
-            ok = bar_and(1, TC_SOFTMAX, ok);
+            ok = bar_and(TC_ALL, TC_SOFTMAX, ok);
             if (tid == 0) sh_bad[item & 15] = 0;
         }
     }
