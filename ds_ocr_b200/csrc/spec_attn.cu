@@ -1679,7 +1679,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
 // The items that several CTAs had parts of. Parts are [row][dimension] with
 // HD / 4 threads a row, one row each, or (WIDE) all on one row, where rows are
 // few and parts may be many. The parts of sa_many_kernel are [dimension][row]:
-// a CTA takes 32 rows and 32 dimensions, a warp every eighth part.
+// a CTA takes 32 rows, a warp an eighth of the dimensions; or (WIDE) 32 rows
+// and 16 dimensions, a warp every eighth part.
 constexpr int SJ_THREADS = 256, SJ_WARPS = SJ_THREADS / 32;
 template <class S> struct SaMade {
     static constexpr bool by_dimension = false;
@@ -1687,9 +1688,12 @@ template <class S> struct SaMade {
 template <int HD, bool DUAL, int QT> struct SaMade<SaMany<HD, DUAL, QT>> {
     static constexpr bool by_dimension = true;
 };
-// Rows (or, by dimension, 32 x 32 blocks) a CTA takes.
+// Rows a CTA takes, and CTAs of an item.
 template <class S> constexpr int sj_rows(bool wide) {
-    return SaMade<S>::by_dimension || wide ? 1 : std::min(S::RT, SJ_THREADS / (S::HD / 4));
+    return SaMade<S>::by_dimension ? 32 : wide ? 1 : std::min(S::RT, SJ_THREADS / (S::HD / 4));
+}
+template <class S> constexpr int sj_ctas(bool wide) {
+    return S::RT / sj_rows<S>(wide) * (SaMade<S>::by_dimension && wide ? S::HD / 16 : 1);
 }
 
 template <class S, bool WIDE>
@@ -1711,27 +1715,24 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
     __syncthreads();
     const SaCut cut(total, a.ctas);
     // this thread's row and first dimension, and the parts it takes
-    constexpr int PER_ITEM = BYD ? (RT / 32) * (HD / 32) : RT / sj_rows<S>(WIDE);
-    const int item = blockIdx.x / PER_ITEM, in = blockIdx.x % PER_ITEM;
-    const int grp = BYD ? warp : tid / (HD / 4), groups = BYD ? SJ_WARPS : SJ_THREADS / (HD / 4);
-    const int r = BYD ? in / (HD / 32) * 32 + lane : WIDE ? in : in * sj_rows<S>(false) + grp;  // (>= RT: none)
-    const int c = BYD ? in % (HD / 32) * 32 : 4 * (tid % (HD / 4));
+    const int item = blockIdx.x / sj_ctas<S>(WIDE), in = blockIdx.x % sj_ctas<S>(WIDE);
+    const int grp = BYD ? warp : tid / (HD / 4), groups = WIDE ? (BYD ? SJ_WARPS : SJ_THREADS / (HD / 4)) : 1;
+    constexpr int VN = BYD ? (WIDE ? 16 : HD / SJ_WARPS) : 4;
+    const int r = BYD ? (WIDE ? in / (HD / 16) : in) * 32 + lane : WIDE ? in : in * sj_rows<S>(false) + grp;  // (>= RT: none)
+    const int c = BYD ? (WIDE ? in % (HD / 16) * 16 : warp * VN) : 4 * (tid % (HD / 4));
     const int x0 = sh_off + item * s.tiles, c0 = cut.cta_of(x0), c1 = cut.cta_of(x0 + s.tiles - 1);
     const int row = r < RT ? item % a.row_tiles * RT + r : a.rows, g = item / a.row_tiles;
     pdl_wait();
     if (c0 == c1) return;
-    constexpr int VN = BYD ? 32 : 4;
     float m = -__FLT_MAX__, l = 0.f, o[VN] = {};
-    const bool split = BYD || WIDE;
     if (row < a.rows) {
-        constexpr int AHEAD = BYD ? 1 : 4;
-        const int step = split ? groups : 1;
-        for (int k0 = c0 + (split ? grp : 0); k0 <= c1; k0 += AHEAD * step) {
+        constexpr int AHEAD = BYD && WIDE ? 2 : 4;
+        for (int k0 = c0 + (WIDE ? grp : 0); k0 <= c1; k0 += AHEAD * groups) {
             float2 ml[AHEAD];
             float v[AHEAD][VN];
 #pragma unroll
             for (int k = 0; k < AHEAD; k++) {
-                const int cc = min(k0 + k * step, c1);
+                const int cc = min(k0 + k * groups, c1);
                 const size_t slot = (size_t)cc * 2 + (cc == c0);
                 ml[k] = a.ml[slot * RT + r];
                 if (BYD) {
@@ -1744,7 +1745,7 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
             }
 #pragma unroll
             for (int k = 0; k < AHEAD; k++) {
-                if (k0 + k * step > c1) break;
+                if (k0 + k * groups > c1) break;
                 const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn), e2 = ex2(ml[k].x - mn);
                 m = mn;
                 l = l * f + ml[k].y * e2;
@@ -1753,26 +1754,40 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
             }
         }
     }
-    if (!split) {
-        if (row < a.rows) {
-            float v[4] = {o[0], o[1], o[2], o[3]};
-            sa_finish(a, b, g, row, s.cnt, c, m, l, v);
+    if (!WIDE) {
+        if (row >= a.rows) return;
+        if constexpr (BYD) {  // 16-bit types: a thread's dimensions in 16-byte stores
+            const int nd = row / a.group, head = g * a.group + row % a.group;
+            const bool none = nd >= s.cnt || l == 0.f;
+            const float inv = 1.f / l;
+            constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16;
+            uint4 *const out = reinterpret_cast<uint4 *>((uint16_t *)d.out + b * d.out_stride[0] + nd * d.out_stride[1] + head * d.out_stride[2] + c);
+#pragma unroll
+            for (int e = 0; e < VN; e++) o[e] = none ? 0.f : o[e] * inv;
+#pragma unroll
+            for (int e = 0; e < VN; e += 8)
+                out[e / 8] = make_uint4(pack2<F16>(o[e], o[e + 1]), pack2<F16>(o[e + 2], o[e + 3]), pack2<F16>(o[e + 4], o[e + 5]),
+                                        pack2<F16>(o[e + 6], o[e + 7]));
+            if (d.lse && c == 0)
+                d.lse[((size_t)b * d.n_nodes + nd) * d.n_heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.69314718f;
+        } else {
+            sa_finish(a, b, g, row, s.cnt, c, m, l, o);
         }
         return;
     }
     // the groups' results, in order
     const int n = min(groups, c1 - c0 + 1);
     if (BYD) {
-        __shared__ float sh_o[BYD ? SJ_WARPS : 1][32][33];
+        __shared__ float sh_o[BYD ? SJ_WARPS : 1][32][17];
         __shared__ float2 sh_ml[BYD ? SJ_WARPS : 1][32];
         if (warp < n) {
             sh_ml[BYD ? warp : 0][lane] = make_float2(m, l);
 #pragma unroll
-            for (int e = 0; e < VN; e++) sh_o[BYD ? warp : 0][lane][e % 32] = o[e];
+            for (int e = 0; e < VN; e++) sh_o[BYD ? warp : 0][lane][e % 16] = o[e];
         }
         __syncthreads();
-        const int rr = tid >> 3, cc = 4 * (tid & 7), out = row - lane + rr;
-        if (out >= a.rows) return;
+        const int rr = tid >> 2, cc = 4 * (tid & 3), out = row - lane + rr;
+        if (rr >= 32 || out >= a.rows) return;
         float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
         for (int k = 0; k < n; k++) mm = fmaxf(mm, sh_ml[k][rr].x);
         for (int k = 0; k < n; k++) {
@@ -1898,9 +1913,8 @@ template <class S> struct SaRun {
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
         const bool wide = (long long)a.d.batch * a.per_seq * S::RT <= a.sms * 8;
-        const int per_item = SaMade<S>::by_dimension ? (S::RT / 32) * (S::HD / 32) : S::RT / sj_rows<S>(wide);
         return launch_ex(wide ? (const void *)sa_join_kernel<S, true> : (const void *)sa_join_kernel<S, false>,
-                         dim3(a.per_seq * per_item, a.d.batch), dim3(SJ_THREADS), 0, st, true, args);
+                         dim3(a.per_seq * sj_ctas<S>(wide), a.d.batch), dim3(SJ_THREADS), 0, st, true, args);
     }
 };
 
