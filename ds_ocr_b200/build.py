@@ -2,7 +2,9 @@
 
 nvcc compiles every .cu under csrc/ (plus the host C file synth.c) with
 -gencode arch=compute_100a,code=sm_100a into one shared library exporting the
-C ABI of include/ds_cuda.h. Runs without a GPU (cross-compilation).
+C ABI of include/ds_cuda.h. Runs without a GPU (cross-compilation). Where
+torch is installed, g++ then builds the module ds_ocr_b200._spec
+(csrc/spec_torch.cpp), the speculative-decoding calls on torch tensors.
 """
 import os
 import subprocess
@@ -12,6 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libds_cuda.so")
+SPEC = os.path.join(HERE, "_spec.so")
 BUILD = os.path.join(ROOT, "_build")
 
 NVCC_FLAGS = [
@@ -78,7 +81,33 @@ def build(verbose=False, force=False):
         if verbose:
             print(" ".join(cmd))
         subprocess.check_call(cmd)
+    build_spec(verbose, force)
     return LIB
+
+
+def build_spec(verbose=False, force=False):
+    """The torch module _spec.so, linked to libds_cuda.so beside it."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    import sysconfig
+    src = os.path.join(CSRC, "spec_torch.cpp")
+    if not (force or _stale(SPEC, [src, os.path.join(ROOT, "include", "ds_cuda.h")])):
+        return SPEC
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())) or "/usr/local/cuda", "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", src, "-o", SPEC,
+           "-I", os.path.join(ROOT, "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-isystem", os.path.join(base, "include"),
+           "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-isystem", cuda,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-L", HERE, "-l:libds_cuda.so",
+           "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.check_call(cmd)
+    return SPEC
 
 
 if __name__ == "__main__":
