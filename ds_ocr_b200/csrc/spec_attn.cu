@@ -688,13 +688,22 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
 #pragma unroll
                 for (int p = 0; p < S::PL; p++)
                     ldsm4t(vf[p], v_s + p * S::PLANE + sw<HD>((lane & 7) + ((lane >> 4) << 3), 2 * t + ((lane >> 3) & 1)));
+                // (F32: a tile's products apart, added with rounding to nearest:
+                // the tensor cores' own sums round towards zero, which adds up
+                // over a long cache)
+                float x[F32 ? NG : 1][4] = {};
 #pragma unroll
-                for (int pk = 0; pk < S::PL; pk++)
+                for (int pk = S::PL - 1; pk >= 0; pk--)
 #pragma unroll
-                    for (int pq = 0; pq < S::QP; pq++)
+                    for (int pq = S::QP - 1; pq >= 0; pq--)
                         if (pq + pk < 3)
 #pragma unroll
-                            for (int n = 0; n < NG; n++) mma16<F16>(o[t][n], vf[pk], pf[n][pq][0], pf[n][pq][1]);
+                            for (int n = 0; n < NG; n++) mma16<F16>(F32 ? x[F32 ? n : 0] : o[t][n], vf[pk], pf[n][pq][0], pf[n][pq][1]);
+                if (F32)
+#pragma unroll
+                    for (int n = 0; n < NG; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[t][n][e] += x[F32 ? n : 0][e];
             }
         }
 
@@ -1050,17 +1059,25 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_
                 }
 #pragma unroll
                 for (int c = 0; c < CH; c += 2) {
+                    // (F32: apart and added, as in sa_few_kernel)
+                    float x[2][4] = {};
 #pragma unroll
-                    for (int pk = 0; pk < S::PL; pk++) {
+                    for (int pk = S::PL - 1; pk >= 0; pk--) {
                         uint32_t vf[4];
                         ldsm4t(vf, v_s + pk * S::PLANE + sw<HD>(vr + 8 * n, c + vc));
 #pragma unroll
-                        for (int pq = 0; pq < S::QP; pq++)
+                        for (int pq = S::QP - 1; pq >= 0; pq--)
                             if (pq + pk < 3) {
-                                mma16<F16>(o[c], pf[pq], vf[0], vf[1]);
-                                mma16<F16>(o[c + 1], pf[pq], vf[2], vf[3]);
+                                mma16<F16>(F32 ? x[0] : o[c], pf[pq], vf[0], vf[1]);
+                                mma16<F16>(F32 ? x[1] : o[c + 1], pf[pq], vf[2], vf[3]);
                             }
                     }
+                    if (F32)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            o[c][e] += x[0][e];
+                            o[c + 1][e] += x[1][e];
+                        }
                 }
             }
         }
