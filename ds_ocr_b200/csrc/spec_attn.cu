@@ -27,8 +27,6 @@ namespace ds {
 constexpr int SA_MAX_NODES = 256;
 constexpr int SA_THREADS = 128;
 constexpr int SA_WARPS = SA_THREADS / 32;
-constexpr int SA_STAGES = 3;
-constexpr int SA_MAX_CTAS = 4;  // of an SM
 
 struct SaArgs {
     ds_cuda_tree_attention_t d;
@@ -368,7 +366,7 @@ __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor 
     cluster_wait();  // no CTA leaves while another reads its part
 }
 
-// ---- up to 16 rows -------------------------------------------------------------
+// ---- few rows: up to 16 at a time ------------------------------------------------
 // Keys take the 16-row side of the matrix instructions and the query rows the
 // 8-column side (S^T = K Q^T, O^T = V^T P^T), so up to 8 rows waste nothing and
 // K and V fragments serve all rows. A tile is 64 keys, 16 per warp; a warp
@@ -471,7 +469,12 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
     }
 
     uint32_t qf[NG][S::QP][KK][2];
-    uint64_t bits[NG][2];                 // of rows 2 gc and 2 gc + 1 of each group
+    uint64_t bits[NG][2];                 // of rows 2 gc and 2 gc + 1 of each group, for the tree's tile at hand
+    auto word = [&](int n, int e, int k) -> uint64_t {
+        const int row = cu.rt * S::RT + 8 * n + 2 * gc + e, nd = row / a.group, left = cu.s.cnt - 64 * k;
+        if (row >= a.rows || nd >= cu.s.cnt || left <= 0) return 0;
+        return d.mask[((size_t)cu.b * d.n_nodes + nd) * a.words + k] & (left < 64 ? (1ull << left) - 1 : ~0ull);
+    };
     float o[KK][NG][4], m[NG][2], l[NG][2];
     bool fresh = true, whole = cu.t == 0;
     int slot = 0;  // of K; V's follows it, then the next tile's
@@ -501,9 +504,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
                     }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const int r2 = cu.rt * S::RT + 8 * n + 2 * gc + e, nd = r2 / a.group;
-                    // rows <= 16, so at most 16 nodes: one word
-                    bits[n][e] = r2 < a.rows && nd < cu.s.cnt ? d.mask[(size_t)cu.b * d.n_nodes + nd] & ((1ull << cu.s.cnt) - 1) : 0;
+                    bits[n][e] = word(n, e, 0);
                     m[n][e] = -__FLT_MAX__;
                     l[n][e] = 0.f;
                 }
@@ -518,7 +519,13 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
         else cp_commit();
 
         const bool node = cu.t >= cu.s.cache_tiles;
-        const int valid = (node ? cu.s.cnt : cu.s.len - cu.t * S::KT) - 16 * warp;  // of this warp's keys
+        const int tree = cu.t - cu.s.cache_tiles;
+        const int valid = (node ? cu.s.cnt - tree * S::KT : cu.s.len - cu.t * S::KT) - 16 * warp;  // of this warp's keys
+        if (tree > 0)  // (the first tile's came with the queries)
+#pragma unroll
+            for (int n = 0; n < NG; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) bits[n][e] = word(n, e, tree);
         uint32_t pf[NG][S::QP][2];
         if (valid > 0) {
             const uint32_t k_s = smem_u32(mine) + slot * S::UNIT;
@@ -754,368 +761,6 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
             whole = true;
         }
         sa_next<S::KT>(a, cu);
-    }
-    cp_wait<0>();
-    if (CLUSTER) sa_cluster_join<S::RT, HD>(a, item, sh_part, sh_pml);
-}
-
-// ---- more rows -----------------------------------------------------------------
-// Shapes of one instantiation. QP planes of the queries and of the weights
-// (F32: three, all 24 bits; 16-bit types: one), PL planes of K and V. Four
-// warps: MT row tiles of 16 times KS slices of KW keys. The CTAs are small,
-// two to four an SM, so that one's loads, products and softmax run beside
-// another's.
-template <int HD_, int MT_, int PL_, int QT_> struct SaShape {
-    static constexpr int HD = HD_, MT = MT_, PL = PL_, QT = QT_;
-    static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
-    static constexpr int RT = 16 * MT;
-    static constexpr int KT = PL == 2 ? 32 : 64;  // a stage is 32 KB (16 KB for head_dim 64) either way
-    static constexpr int KS = SA_WARPS / MT, KW = KT / KS, NT = KW / 8;
-    static constexpr int PLANE = KT * HD * 2, STAGE = 2 * PL * PLANE;
-    static constexpr int QPLANE = RT * HD * 2;
-    static constexpr int SMEM = SA_STAGES * STAGE + QP * QPLANE;
-    static constexpr int FIT = (226 << 10) / (SMEM + 3072);  // by shared memory
-    static constexpr int PER_SM = FIT < SA_MAX_CTAS ? FIT : SA_MAX_CTAS;
-};
-
-// CLUSTER: an item is shared by one cluster, its tiles cut into the CTAs'
-// runs, and joined through their shared memory.
-template <class S, bool CLUSTER>
-__global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_kernel(const __grid_constant__ SaArgs a) {
-    constexpr int HD = S::HD, KT = S::KT, NT = S::NT, KW = S::KW, CH = HD / 8;
-    constexpr bool F16 = S::QT == DS_CUDA_SPEC_F16, F32 = S::QT == DS_CUDA_SPEC_F32;
-    extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ float2 sh_ml[SA_WARPS][16];
-    __shared__ uint64_t sh_mask[2][S::RT];  // by tile parity
-    // a cluster's part: over the first stage, unused by then
-    float4 *const sh_part = reinterpret_cast<float4 *>(smem);
-    float2 *const sh_pml = reinterpret_cast<float2 *>(smem + S::RT * HD * 4);
-    const ds_cuda_tree_attention_t &d = a.d;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int mt = warp % S::MT, ks = warp / S::MT;
-    const uint32_t q_s = smem_u32(smem) + SA_STAGES * S::STAGE;
-
-    SaCursor ld;
-    int tiles;  // of this CTA's run
-    if (!sa_begin<KT, CLUSTER>(a, ld, tiles)) return;
-    SaCursor cu = ld;
-    const SaCursor item = ld;  // CLUSTER's one item
-    // the rows of tile c into stage st; rows past the valid ones are zeros
-    auto load = [&](const SaCursor &c, int st) {
-        const SaTile src = sa_tile<KT>(d, c);
-        const uint32_t dst = smem_u32(smem) + st * S::STAGE;
-        const int cc = tid % CH, rr = tid / CH;
-#pragma unroll
-        for (int kv = 0; kv < 2; kv++)
-#pragma unroll
-            for (int p = 0; p < S::PL; p++)
-#pragma unroll
-                for (int x = 0; x < KT / (SA_THREADS / CH); x++) {
-                    const int r = rr + x * (SA_THREADS / CH);
-                    const bool ok = r < src.valid && (p == 0 || src.lo[kv]);
-                    cp16(dst + (kv * S::PL + p) * S::PLANE + sw<HD>(r, cc),
-                         ok ? src.base[kv][p] + r * src.step[kv] + 8 * cc : d.q, ok);
-                }
-    };
-
-#pragma unroll
-    for (int i = 0; i < SA_STAGES - 1; i++) {
-        if (i < tiles) {
-            load(ld, i);
-            sa_next<KT>(a, ld);
-        }
-        cp_commit();
-    }
-
-    float o[CH][4], m[2], l[2];
-    bool fresh = true;          // the item's queries are not in shared memory yet
-    bool whole = cu.t == 0;     // this CTA has the item from its first tile
-    int st = 0, fill = SA_STAGES - 1;
-    for (int i = 0; i < tiles; i++) {
-        cp_wait<SA_STAGES - 2>();
-        if (fresh) {  // (the previous item's readers of these are past the last barrier of its end)
-            fresh = false;
-            // (all loads first: stores in between would hold them up)
-            constexpr int QN = S::RT * CH / SA_THREADS;
-            uint4 u[QN][F32 ? 2 : 1];
-#pragma unroll
-            for (int k = 0; k < QN; k++) {
-                const int x = tid + k * SA_THREADS, row = cu.rt * S::RT + x / CH;
-                const int64_t qo = cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
-                                   (cu.g * a.group + row % a.group) * d.q_stride[2] + 8 * (x % CH);
-#pragma unroll
-                for (int h = 0; h < (F32 ? 2 : 1); h++)
-                    u[k][h] = row >= a.rows ? make_uint4(0, 0, 0, 0)
-                              : F32         ? *reinterpret_cast<const uint4 *>((const float *)d.q + qo + 4 * h)
-                                            : *reinterpret_cast<const uint4 *>((const uint16_t *)d.q + qo);
-            }
-#pragma unroll
-            for (int k = 0; k < QN; k++) {
-                const int x = tid + k * SA_THREADS;
-                uint8_t *const q = smem + SA_STAGES * S::STAGE + sw<HD>(x / CH, x % CH);
-                if (F32) {
-                    uint32_t p[4][3];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const uint4 &y = u[k][F32 ? e >> 1 : 0];
-                        split3(__uint_as_float(e & 1 ? y.z : y.x), __uint_as_float(e & 1 ? y.w : y.y), p[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < S::QP; e++)
-                        *reinterpret_cast<uint4 *>(q + e * S::QPLANE) = make_uint4(p[0][e], p[1][e], p[2][e], p[3][e]);
-                } else {
-                    *reinterpret_cast<uint4 *>(q) = u[k][0];
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < CH; c++) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
-            m[0] = m[1] = -__FLT_MAX__;
-            l[0] = l[1] = 0.f;
-        }
-        const bool node = cu.t >= cu.s.cache_tiles;
-        const int r0 = (node ? cu.t - cu.s.cache_tiles : cu.t) * KT;
-        const int valid = (node ? cu.s.cnt : cu.s.len) - r0;
-        if (node)
-            for (int r = tid; r < S::RT; r += SA_THREADS) {
-                const int row = cu.rt * S::RT + r, nd = row / a.group;
-                uint64_t bits = 0;  // KT <= 64 and r0 is a multiple of KT: within one word
-                if (row < a.rows && nd < cu.s.cnt && valid > 0)
-                    bits = d.mask[((size_t)cu.b * d.n_nodes + nd) * a.words + r0 / 64] >> (r0 & 63) &
-                           (valid < 64 ? (1ull << valid) - 1 : ~0ull);
-                sh_mask[i & 1][r] = bits;
-            }
-        __syncthreads();
-        if (i + SA_STAGES - 1 < tiles) {
-            load(ld, fill);
-            sa_next<KT>(a, ld);
-        }
-        cp_commit();
-        fill = fill + 1 == SA_STAGES ? 0 : fill + 1;
-
-        const uint32_t k_s = smem_u32(smem) + st * S::STAGE, v_s = k_s + S::PL * S::PLANE;
-        // scores of 16 rows and KW keys; the planes' products of each order of
-        // magnitude apart (shorter chains, smaller rounding)
-        float s[NT][4], low[F32 ? NT : 1][2][4];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                s[n][e] = 0.f;
-                if (F32) low[n][0][e] = low[n][1][e] = 0.f;
-            }
-        const int qr = 16 * mt + (lane & 15), qc = lane >> 4;
-        {
-            const int kr = ks * KW + (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; kk++) {
-                uint32_t qf[S::QP][4];
-#pragma unroll
-                for (int p = 0; p < S::QP; p++) ldsm4(qf[p], q_s + p * S::QPLANE + sw<HD>(qr, 2 * kk + qc));
-#pragma unroll
-                for (int n = 0; n < NT; n += 2) {
-#pragma unroll
-                    for (int pk = 0; pk < S::PL; pk++) {
-                        uint32_t kf[4];
-                        ldsm4(kf, k_s + pk * S::PLANE + sw<HD>(kr + 8 * n, 2 * kk + kc));
-#pragma unroll
-                        for (int pq = 0; pq < S::QP; pq++)
-                            if (pq + pk < 3)
-#pragma unroll
-                                for (int x = 0; x < 2; x++)
-                                    mma16<F16>(pq + pk ? low[F32 ? n + x : 0][(pq + pk + 1) & 1] : s[n + x], qf[pq],
-                                               kf[2 * x], kf[2 * x + 1]);
-                    }
-                }
-            }
-        }
-        if (F32)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[n][e] += low[n][0][e] + low[n][1][e];
-
-        // running maximum (of the scaled scores, in log2 units), weights, sums
-        const bool masked = node || valid < KT;
-        uint64_t see[2] = {~0ull, ~0ull};
-        if (masked) {
-            const int key = ks * KW;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if (node) see[h] = sh_mask[i & 1][16 * mt + (lane >> 2) + 8 * h] >> key;
-                else see[h] = valid - key >= 64 ? ~0ull : valid > key ? (1ull << (valid - key)) - 1 : 0;
-            }
-        }
-        float mx[2] = {m[0], m[1]};
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (!masked || ((see[e >> 1] >> (8 * n + 2 * (lane & 3) + (e & 1))) & 1))
-                    mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e] * a.scale2);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(DS_FULL, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(DS_FULL, mx[h], 2));
-        }
-        if (__any_sync(DS_FULL, mx[0] > m[0] || mx[1] > m[1])) {
-            const float f0 = ex2(m[0] - mx[0]), f1 = ex2(m[1] - mx[1]);
-            l[0] *= f0;
-            l[1] *= f1;
-#pragma unroll
-            for (int c = 0; c < CH; c++) {
-                o[c][0] *= f0;
-                o[c][1] *= f0;
-                o[c][2] *= f1;
-                o[c][3] *= f1;
-            }
-            m[0] = mx[0];
-            m[1] = mx[1];
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const bool ok = !masked || ((see[e >> 1] >> (8 * n + 2 * (lane & 3) + (e & 1))) & 1);
-                s[n][e] = ok ? ex2(__fmaf_rn(s[n][e], a.scale2, -m[e >> 1])) : 0.f;
-                l[e >> 1] += s[n][e];
-            }
-
-        if (node) {
-            // A node's V may hold NaN or infinities that some rows must not
-            // see, and 0 * NaN would spread through the product: such values
-            // are added here to the rows that attend them, then zeroed.
-            bool bad = false;
-            for (int x = tid; x < KT * CH; x += SA_THREADS) {
-                const uint32_t off = sw<HD>(x / CH, x % CH);
-#pragma unroll
-                for (int p = 0; p < S::PL; p++) {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(smem + st * S::STAGE + (S::PL + p) * S::PLANE + off);
-                    constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t e = ((&u.x)[k] & E) ^ E;
-                        bad |= !(e & 0xffffu) || !(e >> 16);
-                    }
-                }
-            }
-            if (__syncthreads_or(bad)) {
-                for (int kk = 0; kk < KW; kk++) {
-                    const int key = ks * KW + kk;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int r = 16 * mt + (lane >> 2) + 8 * h;
-                        if (!((sh_mask[i & 1][r] >> key) & 1)) continue;
-#pragma unroll
-                        for (int c = 0; c < CH; c++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                float v = 0.f;
-#pragma unroll
-                                for (int p = 0; p < S::PL; p++) {
-                                    const uint16_t w = *reinterpret_cast<const uint16_t *>(
-                                        smem + st * S::STAGE + (S::PL + p) * S::PLANE + sw<HD>(key, c) + 2 * (2 * (lane & 3) + e));
-                                    v += F16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
-                                }
-                                if (!isfinite(v)) o[c][2 * h + e] += v;
-                            }
-                    }
-                }
-                __syncthreads();
-                for (int x = tid; x < KT * HD; x += SA_THREADS) {
-                    const uint32_t off = sw<HD>(x / HD, x % HD / 8) + 2 * (x % 8);
-                    bool nf = false;
-#pragma unroll
-                    for (int p = 0; p < S::PL; p++) {
-                        const uint16_t w = *reinterpret_cast<uint16_t *>(smem + st * S::STAGE + (S::PL + p) * S::PLANE + off);
-                        nf |= (w & (F16 ? 0x7c00 : 0x7f80)) == (F16 ? 0x7c00 : 0x7f80);
-                    }
-                    if (nf)
-#pragma unroll
-                        for (int p = 0; p < S::PL; p++)
-                            *reinterpret_cast<uint16_t *>(smem + st * S::STAGE + (S::PL + p) * S::PLANE + off) = 0;
-                }
-                __syncthreads();
-            }
-        }
-
-        // O += P V
-        {
-            const int vr = ks * KW + (lane & 15), vc = lane >> 4;
-#pragma unroll
-            for (int n = 0; n < NT; n += 2) {
-                uint32_t pf[S::QP][4];
-                if (F32) {
-                    uint32_t t[3];
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        split3(s[n + (x >> 1)][2 * (x & 1)], s[n + (x >> 1)][2 * (x & 1) + 1], t);
-#pragma unroll
-                        for (int p = 0; p < S::QP; p++) pf[p][x] = t[p];
-                    }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        pf[0][x] = pack2<F16>(s[n + (x >> 1)][2 * (x & 1)], s[n + (x >> 1)][2 * (x & 1) + 1]);
-                }
-#pragma unroll
-                for (int c = 0; c < CH; c += 2) {
-                    // (F32: apart and added, as in sa_few_kernel)
-                    float x[2][4] = {};
-#pragma unroll
-                    for (int pk = S::PL - 1; pk >= 0; pk--) {
-                        uint32_t vf[4];
-                        ldsm4t(vf, v_s + pk * S::PLANE + sw<HD>(vr + 8 * n, c + vc));
-#pragma unroll
-                        for (int pq = S::QP - 1; pq >= 0; pq--)
-                            if (pq + pk < 3) {
-                                mma16<F16>(F32 ? x[0] : o[c], pf[pq], vf[0], vf[1]);
-                                mma16<F16>(F32 ? x[1] : o[c + 1], pf[pq], vf[2], vf[3]);
-                            }
-                    }
-                    if (F32)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            o[c][e] += x[0][e];
-                            o[c + 1][e] += x[1][e];
-                        }
-                }
-            }
-        }
-
-        const bool end = cu.t + 1 == cu.s.tiles;
-        if (end || i + 1 == tiles) {
-            // the item, or this CTA's part of it, is done: the warps' parts
-            // are joined through this stage, which is free until the next
-            // iteration's barrier (a cluster's run ends here: every stage is
-            // free, and the join goes from the second into the first)
-            __syncthreads();
-            const float *parts = reinterpret_cast<const float *>(smem + (CLUSTER ? 1 : st) * S::STAGE);
-            float *so = const_cast<float *>(parts) + warp * 16 * HD;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                l[h] += __shfl_xor_sync(DS_FULL, l[h], 1);
-                l[h] += __shfl_xor_sync(DS_FULL, l[h], 2);
-                if ((lane & 3) == 0) sh_ml[warp][(lane >> 2) + 8 * h] = make_float2(m[h], l[h]);
-#pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    const int r = (lane >> 2) + 8 * h, x = 8 * c + 2 * (lane & 3);
-                    *reinterpret_cast<float2 *>(so + r * HD + (x ^ ((r & 3) << 3))) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
-                }
-            }
-            __syncthreads();
-            sa_merge<S::RT, HD, S::KS>([&](int w, int r) { return sh_ml[w * S::MT + (r >> 4)][r & 15]; },
-                                       [&](int w, int r, int c) {
-                                           return parts + ((w * S::MT + (r >> 4)) * 16 + (r & 15)) * HD + (c ^ ((r & 3) << 3));
-                                       },
-                                       [&](int r, int c, float mm, float ll, float (&v)[4]) {
-                                           sa_put<S::RT, HD, CLUSTER>(a, cu, whole, end, sh_part, sh_pml, r, c, mm, ll, v);
-                                       });
-            fresh = true;
-            whole = true;
-            __syncthreads();  // the join's readers are done: the stage and the queries may be refilled
-        }
-        sa_next<KT>(a, cu);
-        st = st + 1 == SA_STAGES ? 0 : st + 1;
     }
     cp_wait<0>();
     if (CLUSTER) sa_cluster_join<S::RT, HD>(a, item, sh_part, sh_pml);
@@ -1871,28 +1516,21 @@ static bool sa_map(const ds_cuda_tree_attention_t &d, int kv, int kt, CUtensorMa
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class S, bool CLUSTER> struct SaKernel {
-    static constexpr auto kernel = sa_kernel<S, CLUSTER>;
-};
-template <int HD, int NG, int PL, int QT, bool CLUSTER> struct SaKernel<SaFew<HD, NG, PL, QT>, CLUSTER> {
-    static constexpr auto kernel = sa_few_kernel<SaFew<HD, NG, PL, QT>, CLUSTER>;
-};
-
-template <int HD, bool DUAL, int QT> struct SaKernel<SaMany<HD, DUAL, QT>, false> {
-    static constexpr auto kernel = sa_many_kernel<SaMany<HD, DUAL, QT>>;
-};
 template <class S> struct SaRun {
     static bool clusters(const SaArgs &a) { return !SaMade<S>::by_dimension && sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
     static size_t workspace(const SaArgs &a) {
         // two parts a CTA, then their maxima and sums
         return clusters(a) ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
     }
+    // A kernel's attributes, once per device (of the first 64).
     template <bool CLUSTER> static cudaError_t attributes(int device) {
-        static std::atomic<uint64_t> ready;  // devices (of the first 64) that have them
+        static std::atomic<uint64_t> ready;
         if (device < 64 && ready.load() >> device & 1) return cudaSuccess;
-        cudaError_t e = cudaFuncSetAttribute(SaKernel<S, CLUSTER>::kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-        if (e == cudaSuccess && CLUSTER)
-            e = cudaFuncSetAttribute(SaKernel<S, CLUSTER>::kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        const void *f;
+        if constexpr (SaMade<S>::by_dimension) f = (const void *)sa_many_kernel<S>;
+        else f = (const void *)sa_few_kernel<S, CLUSTER>;
+        cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e == cudaSuccess && CLUSTER) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess && device < 64) ready.fetch_or(1ull << device);
         return e;
     }
@@ -1912,7 +1550,7 @@ template <class S> struct SaRun {
             attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
-            return cudaLaunchKernelExC(&cfg, (const void *)SaKernel<S, true>::kernel, args);
+            return cudaLaunchKernelExC(&cfg, (const void *)sa_few_kernel<S, true>, args);
         }
         a.ctas = a.sms * S::PER_SM;
         a.part = (float *)a.d.workspace;
@@ -1925,7 +1563,7 @@ template <class S> struct SaRun {
             many.mapped = sa_map(a.d, 0, S::KT, &many.map[0], many.dim[0]) && sa_map(a.d, 1, S::KT, &many.map[1], many.dim[1]);
             sa_many_kernel<S><<<a.ctas, TC_THREADS, S::SMEM, st>>>(many);
         } else {
-            SaKernel<S, false>::kernel<<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
+            sa_few_kernel<S, false><<<a.ctas, SA_THREADS, S::SMEM, st>>>(a);
         }
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
@@ -1937,25 +1575,25 @@ template <class S> struct SaRun {
 
 // f(instantiation) for a call, by its rows. F32 queries take at most 32 at a
 // time: their three planes fill the shared memory.
-template <int HD, int QT, class F> static auto sa_pick16(int rows, F f) {
-    return rows <= 8     ? f(SaRun<SaFew<HD, 1, 1, QT>>())
-           : rows <= 16  ? f(SaRun<SaFew<HD, 2, 1, QT>>())
-           : rows <= 32  ? f(SaRun<SaShape<HD, 2, 1, QT>>())
-           : rows <= 128 ? f(SaRun<SaMany<HD, false, QT>>()) : f(SaRun<SaMany<HD, true, QT>>());
+template <int HD, int QT, class F> static auto sa_pick16(int rows, bool brief, F f) {
+    return rows <= 8             ? f(SaRun<SaFew<HD, 1, 1, QT>>())
+           : rows <= 16 || brief ? f(SaRun<SaFew<HD, 2, 1, QT>>())
+           : rows <= 128         ? f(SaRun<SaMany<HD, false, QT>>()) : f(SaRun<SaMany<HD, true, QT>>());
 }
-template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, F f) {
+template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, int sms, F f) {
     constexpr int P = DS_CUDA_SPEC_F32;
     const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
-    if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, f);
-    if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, f);
+    const bool brief = sa_clusters<SaFew<HD, 2, 1, DS_CUDA_SPEC_BF16>>(d, d->batch * d->n_kv_heads * ((rows + 15) / 16), sms);
+    if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, brief, f);
+    if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, brief, f);
     if (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo)
         return rows <= 8    ? f(SaRun<SaFew<HD, 1, 2, P>>())
-               : rows <= 16 ? f(SaRun<SaFew<HD, 2, 2, P>>()) : f(SaRun<SaShape<HD, 2, 2, P>>());
+               : f(SaRun<SaFew<HD, 2, 2, P>>());
     return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, P>>())
-           : rows <= 16 ? f(SaRun<SaFew<HD, 2, 1, P>>()) : f(SaRun<SaShape<HD, 2, 1, P>>());
+           : f(SaRun<SaFew<HD, 2, 1, P>>());
 }
-template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, F f) {
-    return d->head_dim == 64 ? sa_pick_hd<64>(d, f) : sa_pick_hd<128>(d, f);
+template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, int sms, F f) {
+    return d->head_dim == 64 ? sa_pick_hd<64>(d, sms, f) : sa_pick_hd<128>(d, sms, f);
 }
 template <class S> static S sa_shape(SaRun<S>) { return S(); }
 
@@ -2013,7 +1651,7 @@ static SaArgs sa_args(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
     a.words = (d->n_nodes + 63) / 64;
     a.group = d->n_heads / d->n_kv_heads;
     a.rows = d->n_nodes * a.group;
-    const int rt = sa_pick(d, [](auto r) { return decltype(sa_shape(r))::RT; });
+    const int rt = sa_pick(d, c->sm_count, [](auto r) { return decltype(sa_shape(r))::RT; });
     a.row_tiles = (a.rows + rt - 1) / rt;
     a.per_seq = d->n_kv_heads * a.row_tiles;
     a.sms = c->sm_count;
@@ -2025,7 +1663,7 @@ static SaArgs sa_args(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
 extern "C" size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d) {
     if (!c || !c->ok || sa_check(nullptr, d) < 0) return 0;
     const SaArgs a = sa_args(c, d);
-    return sa_pick(d, [&](auto r) { return decltype(r)::workspace(a); });
+    return sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::workspace(a); });
 }
 
 extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d, void *stream) {
@@ -2053,12 +1691,12 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
             return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: %s has a lo plane, which only the F32 type takes", t.name);
     }
     const SaArgs a = sa_args(c, d);
-    const size_t need = sa_pick(d, [&](auto r) { return decltype(r)::workspace(a); });
+    const size_t need = sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::workspace(a); });
     if (need && (!d->workspace || d->workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->workspace) & 255)))
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: workspace of %zu bytes, 256-byte aligned, wanted", need);
     cudaSetDevice(c->device);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    const cudaError_t e = sa_pick(d, [&](auto r) { return decltype(r)::run(a, c->device, st); });
+    const cudaError_t e = sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::run(a, c->device, st); });
     if (e != cudaSuccess) cudaGetLastError();  // reported here, not by whoever asks next
     return ctx_cuda(c, e, "tree_attention launch");
 }
