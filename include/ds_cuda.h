@@ -603,7 +603,7 @@ int ds_cuda_tree_mask_dev(ds_cuda_ctx_t *ctx, const int *parents, const int *nod
  * is [rows x vocab]. temperature [rows] or NULL (1). A temperature <= 0
  * gives 1 at the row's largest logit (the lowest index wins ties). -infinity
  * is probability 0, a row of nothing else is zeros, a NaN or +infinity
- * makes its row NaN. */
+ * makes its row NaN. Limits: vocab <= 917504. */
 int ds_cuda_token_probs_dev(ds_cuda_ctx_t *ctx, int type, const void *logits, int rows, int vocab, int64_t row_stride,
                             const float *temperature, float *probs, void *stream);
 
