@@ -244,43 +244,50 @@ template <typename T> __device__ __forceinline__ float tp_f(T v) { return (float
 template <> __device__ __forceinline__ float tp_f(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float tp_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// One cluster per row, its CTAs holding consecutive slices in shared memory,
-// so the logits are read once. A CTA takes its own maximum m and sum s of
-// e = 2^((x - m) c), c = log2(e) / temperature; one exchange of (m, s) in the
-// cluster gives every CTA the row's M and S, and p = e * (2^((m - M) c) / S).
-// Bound by the memory: CTAs of 256 threads and at most 28 KB, up to eight an
-// SM, one reading while another sums or writes; 16 bytes a thread at a time
-// between a row's 16-byte boundaries, single elements outside. 512 rows of
-// 50257 BF16 logits: 47 us, 3.3 TB/s (76 us with the slices in registers, two
-// CTAs of 512 threads an SM, and the sums by exp2f); 9 rows of 129280 F32
-// logits, where the launch and the exchange are most of it: 6.7 us.
-constexpr int TP_THREADS = 256, TP_SLICE = 7168, TP_CLUSTER = 16, TP_MOST = 56 << 10;  // values of a CTA: usual, and at most
+// One cluster per row, its CTAs holding consecutive slices in shared memory as
+// they came, so the logits are read once. A CTA takes its own maximum m and
+// sum s of e = 2^((x - m) c), c = log2(e) / temperature; one exchange of
+// (m, s) in the cluster gives every CTA the row's M and S, and p = e * (2^((m
+// - M) c) / S): F32 logits are replaced by their e, of 16-bit ones e is taken
+// twice (as F32 values in shared memory they take 47 us instead of 30).
+// Bound by the memory, with eight CTAs of 128 threads and at most 28 KB an SM,
+// some of them reading while others sum or write. 512 rows of 50257 logits,
+// reads and writes together: BF16 30 us, 5.2 TB/s; F32 43 us, 4.8 TB/s. Twice
+// the threads take 32 and 52 us (the fixed work of a thread: exchanges and
+// ends), slices of 14 KB 35 us and 58 us, of 56 KB 34 and 45 us. 9 rows of
+// 129280 F32 logits, mostly launch and exchange, take 6.0 us.
+constexpr int TP_THREADS = 128, TP_SLICE = 28 << 10, TP_CLUSTER = 16;  // bytes of a CTA's slice, if 16 CTAs can
+constexpr int TP_MOST = 56 << 10;                                      // values of a CTA
 __device__ __forceinline__ float tp_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// E = 16 / sizeof(T) logits as floats.
-__device__ __forceinline__ void tp_wide(const float *p, float (&v)[4]) {
-    const float4 u = __ldcs(reinterpret_cast<const float4 *>(p));
-    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+// Four values from 16 or 8 bytes.
+__device__ __forceinline__ float4 tp_four(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 tp_four(const __half *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    const float2 x = __half22float2(reinterpret_cast<const __half2 &>(u.x)), y = __half22float2(reinterpret_cast<const __half2 &>(u.y));
+    return make_float4(x.x, x.y, y.x, y.y);
 }
-template <typename T> __device__ __forceinline__ void tp_wide(const T *p, float (&v)[8]) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
-    const T *h = reinterpret_cast<const T *>(&u);
-#pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = tp_f(h[k]);
+__device__ __forceinline__ float4 tp_four(const __nv_bfloat16 *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xffff0000u));
 }
+template <typename T> __device__ __forceinline__ T tp_lowest() { return (T)-INFINITY; }
 template <typename T>
 __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *logits, int V, int64_t stride, const float *temp,
                                                                     float *out) {
     constexpr int E = 16 / sizeof(T);
-    extern __shared__ __align__(16) float store[];
+    constexpr bool F32 = sizeof(T) == 4;
+    extern __shared__ __align__(16) uint8_t store_raw[];
     __shared__ float sh[TP_THREADS / 32];
     __shared__ float2 ms[TP_CLUSTER];
     __shared__ unsigned long long key[TP_CLUSTER];
     __shared__ int bad[TP_CLUSTER];
     __shared__ unsigned long long best;
+    T *const store = reinterpret_cast<T *>(store_raw);
     const cg::cluster_group cl = cg::this_cluster();
     cluster_started();
     constexpr int nt = TP_THREADS;
@@ -289,36 +296,29 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
     const int slice = (V + ncta - 1) / ncta, i0 = min(V, rank * slice), len = min(V, i0 + slice) - i0;
     const T *x = logits + row * stride + i0;
     out += (size_t)row * V + i0;
-    const float tt = temp ? temp[row] : 1.f, c1 = __fdiv_rn(1.44269504f, tt);
-    const float c = c1 == 0.f ? FLT_MIN : c1;  // an infinite temperature: -infinity times c stays so
-    // the slice as floats from buf on; store begins and ends with -infinity up
-    // to multiples of four, and the 16-byte reads fall on 16 bytes there too
+    // the slice from buf on; store begins and ends with -infinity up to
+    // multiples of four, and the 16-byte copies fall on 16 bytes there too
     const int head = min(len, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
     const int pad = (E - head) & (E - 1), wide = (len - head) / E, all = (pad + len + 3) & ~3;
-    float *const buf = store + pad;
-    float m = -INFINITY;
-    if (tid < pad) store[tid] = -INFINITY;
-    if (tid < all - pad - len) buf[len + tid] = -INFINITY;
+    T *const buf = store + pad;
+    for (int i = tid; i < wide; i += nt)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(buf + head + i * E)), "l"(x + head + i * E) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (tid < pad) store[tid] = tp_lowest<T>();
+    if (tid < all - pad - len) buf[len + tid] = tp_lowest<T>();
     for (int i = tid; i < len - wide * E; i += nt) {
         const int k = i < head ? i : i + wide * E;
-        const float v = tp_f(x[k]);
-        buf[k] = v;
-        m = fmaxf(m, v);
+        buf[k] = x[k];
     }
-    for (int i = tid; i < wide; i += 2 * nt) {
-        float v[2][E];
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (i + k * nt < wide) tp_wide(x + head + (i + k * nt) * E, v[k]);
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (i + k * nt < wide)
-#pragma unroll
-                for (int e = 0; e < E; e += 4) {
-                    m = fmaxf(m, fmaxf(fmaxf(v[k][e], v[k][e + 1]), fmaxf(v[k][e + 2], v[k][e + 3])));
-                    *reinterpret_cast<float4 *>(buf + head + (i + k * nt) * E + e) =
-                        make_float4(v[k][e], v[k][e + 1], v[k][e + 2], v[k][e + 3]);
-                }
+    const float tt = temp ? temp[row] : 1.f, c1 = __fdiv_rn(1.44269504f, tt);
+    const float c = c1 == 0.f ? FLT_MIN : c1;  // an infinite temperature: -infinity times c stays so
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int i = 4 * tid; i < all; i += 4 * nt) {
+        const float4 v = tp_four(store + i);
+        m = fmaxf(m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
     m = warp_max(m);
     if (lane == 0) sh[warp] = m;
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
         unsigned long long k = 0;
         bool nan = false;
         for (int i = tid; i < len; i += nt) {
-            const float l = buf[i];
+            const float l = tp_f(buf[i]);
             nan |= !(l < INFINITY);
             const unsigned long long kk = argmax_key(l, i0 + i);
             if (l > -INFINITY && kk > k) k = kk;
@@ -358,14 +358,14 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
     for (int w = 0; w < nt / 32; w++) m = fmaxf(m, sh[w]);
     m = fmaxf(m, -FLT_MAX);
     float s = 0.f;
-#pragma unroll 2
+#pragma unroll 4
     for (int i = 4 * tid; i < all; i += 4 * nt) {
-        float4 v = *reinterpret_cast<const float4 *>(store + i);
+        float4 v = tp_four(store + i);
         v.x = tp_ex2((v.x - m) * c);
         v.y = tp_ex2((v.y - m) * c);
         v.z = tp_ex2((v.z - m) * c);
         v.w = tp_ex2((v.w - m) * c);
-        *reinterpret_cast<float4 *>(store + i) = v;
+        if (F32) *reinterpret_cast<float4 *>(store + i) = v;
         s += (v.x + v.y) + (v.z + v.w);
     }
     s = warp_sum(s);
@@ -377,22 +377,22 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
     for (int w = 0; w < nt / 32; w++) s += sh[w];
     if (tid < ncta) cl.map_shared_rank(ms, tid)[rank] = make_float2(m, s);
     cl.sync();
-    float M = -FLT_MAX, S = 0.f;
-    for (int r = 0; r < ncta; r++) M = fmaxf(M, ms[r].x);
-    for (int r = 0; r < ncta; r++) S += ms[r].y * tp_ex2((ms[r].x - M) * c);
+    const float2 part = lane < ncta ? ms[lane] : make_float2(-FLT_MAX, 0.f);
+    const float M = warp_max(part.x), S = warp_sum(part.y * tp_ex2((part.x - M) * c));
     const float f = S == 0.f ? 0.f : tp_ex2((m - M) * c) / S;
+    auto prob = [&](float v) { return (F32 ? v : tp_ex2((v - m) * c)) * f; };
     // four at a time between the output's 16-byte boundaries
     const int first = min(len, (int)((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / 4), quads = (len - first) / 4;
     for (int i = tid; i < len - 4 * quads; i += nt) {
         const int k = i < first ? i : i + 4 * quads;
-        out[k] = buf[k] * f;
+        out[k] = prob(tp_f(buf[k]));
     }
     const bool even = ((pad + first) & 3) == 0;  // the same boundaries as in shared memory
-#pragma unroll 2
+#pragma unroll 4
     for (int i = tid; i < quads; i += nt) {
-        const float *const b = buf + first + 4 * i;
-        const float4 v = even ? *reinterpret_cast<const float4 *>(b) : make_float4(b[0], b[1], b[2], b[3]);
-        __stcs(reinterpret_cast<float4 *>(out + first + 4 * i), make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+        const T *const b = buf + first + 4 * i;
+        const float4 v = even ? tp_four(b) : make_float4(tp_f(b[0]), tp_f(b[1]), tp_f(b[2]), tp_f(b[3]));
+        __stcs(reinterpret_cast<float4 *>(out + first + 4 * i), make_float4(prob(v.x), prob(v.y), prob(v.z), prob(v.w)));
     }
 }
 
@@ -506,8 +506,10 @@ extern "C" int ds_cuda_token_probs_dev(ds_cuda_ctx_t *c, int type, const void *l
     if (vocab > TP_CLUSTER * TP_MOST)
         return ctx_fail(c, DS_CUDA_EINVAL, "token_probs: vocab %d (<= %d)", vocab, TP_CLUSTER * TP_MOST);
     // CTAs for the slices to be small; more where few rows leave SMs idle
+    const int size = type == DS_CUDA_SPEC_F32 ? 4 : 2;
     int ncta = 1;
-    while (ncta < TP_CLUSTER && ((vocab + ncta - 1) / ncta > TP_SLICE || (vocab > ncta * 2048 && rows * ncta * 2 <= c->sm_count)))
+    while (ncta < TP_CLUSTER && ((vocab + ncta - 1) / ncta > TP_SLICE / size ||
+                                 (vocab > ncta * 2048 && rows * ncta * 2 <= c->sm_count)))
         ncta *= 2;
     const void *f = type == DS_CUDA_SPEC_F32   ? (const void *)token_probs_kernel<float>
                     : type == DS_CUDA_SPEC_F16 ? (const void *)token_probs_kernel<__half>
@@ -520,8 +522,8 @@ extern "C" int ds_cuda_token_probs_dev(ds_cuda_ctx_t *c, int type, const void *l
         if (c->device < 64) ready[type].fetch_or(1ull << c->device);
     }
     void *args[] = {(void *)&logits, &vocab, &row_stride, (void *)&temperature, &probs};
-    return ctx_cuda(c, launch_cluster(f, (long long)rows * ncta, TP_THREADS, (size_t)((vocab + ncta - 1) / ncta) * 4 + 64, ncta,
-                                      st, args),
+    return ctx_cuda(c, launch_cluster(f, (long long)rows * ncta, TP_THREADS, (size_t)((vocab + ncta - 1) / ncta) * size + 64,
+                                      ncta, st, args),
                     "token_probs launch");
 }
 

@@ -354,6 +354,22 @@ def test_token_probs_edges(spec):
     assert torch.isnan(spec.token_probs(y, torch.tensor([nan], device="cuda"))).all()
 
 
+def test_token_probs_of_an_infinite_temperature(spec):
+    x = torch.randn(2, 5000, device="cuda")
+    x[1, ::2] = -float("inf")
+    p = spec.token_probs(x, torch.full((2,), float("inf"), device="cuda"))
+    assert float((p[0] * 5000 - 1).abs().max()) < 1e-5
+    assert not p[1, ::2].any() and float((p[1, 1::2] * 2500 - 1).abs().max()) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_probs_of_the_largest_vocabulary(spec, dtype):
+    x = (2 * torch.randn(2, 917504, device="cuda")).to(dtype)
+    assert rel(spec.token_probs(x), torch.softmax(x.double(), -1)) < 5e-6
+    with pytest.raises(DsCudaError):
+        spec.token_probs(torch.zeros(1, 917505, dtype=dtype, device="cuda"))
+
+
 def test_token_probs_refusals(spec):
     x = torch.zeros(2, 8, device="cuda")
     for bad in (x.double(), x.T, x.cpu()):
