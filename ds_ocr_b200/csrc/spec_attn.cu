@@ -49,20 +49,21 @@ struct SaSeq {
 template <int KT>
 __device__ __forceinline__ SaSeq sa_seq(const ds_cuda_tree_attention_t &d, int b) {
     SaSeq s;
+    const int len = d.lens[b];  // (beside the other load, not after it)
     s.cnt = d.nodes ? min(max(d.nodes[b], 0), d.n_nodes) : d.n_nodes;
-    s.len = s.cnt ? min(max(d.lens[b], 0), d.kv_max) : 0;  // no rows: one empty tile, whose results are zeros
+    s.len = s.cnt ? min(max(len, 0), d.kv_max) : 0;  // no rows: one empty tile, whose results are zeros
     s.cache_tiles = (s.len + KT - 1) / KT;
     s.tiles = max(1, s.cache_tiles + (s.cnt + KT - 1) / KT);
     return s;
 }
 // Sums the sequences' tiles over the batch: returns the total, *mine the
-// tiles before this thread's run of sequences [b0, b1). (The host refuses
-// what could pass 2^31 tiles.)
+// tiles before this thread's run of sequences [b0, b1), whose first is `own`.
+// (The host refuses what could pass 2^31 tiles.)
 template <int KT, int THREADS>
-__device__ __forceinline__ int sa_scan(const SaArgs &a, int b0, int b1, int *sh, int *mine) {
+__device__ __forceinline__ int sa_scan(const SaArgs &a, int b0, int b1, const SaSeq &own, int *sh, int *mine) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = 0;
-    for (int b = b0; b < b1; b++) s += sa_seq<KT>(a.d, b).tiles * a.per_seq;
+    int s = b0 < b1 ? own.tiles * a.per_seq : 0;
+    for (int b = b0 + 1; b < b1; b++) s += sa_seq<KT>(a.d, b).tiles * a.per_seq;
     int v = s;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -229,6 +230,7 @@ struct SaCursor {
 template <int KT, bool CLUSTER, int THREADS = SA_THREADS>
 __device__ __forceinline__ bool sa_begin(const SaArgs &a, SaCursor &c, int &tiles) {
     __shared__ int sh_scan[THREADS / 32], sh_off, sh_b;
+    __shared__ SaSeq sh_s;
     const int tid = threadIdx.x;
     if (CLUSTER) {
         cluster_arrive();
@@ -246,22 +248,25 @@ __device__ __forceinline__ bool sa_begin(const SaArgs &a, SaCursor &c, int &tile
     const int chunk = (a.d.batch + THREADS - 1) / THREADS;
     const int b0 = min(a.d.batch, tid * chunk), b1 = min(a.d.batch, b0 + chunk);
     int at;
-    const int total = sa_scan<KT, THREADS>(a, b0, b1, sh_scan, &at);
+    SaSeq s = sa_seq<KT>(a.d, min(b0, a.d.batch - 1));
+    const int total = sa_scan<KT, THREADS>(a, b0, b1, s, sh_scan, &at);
     const SaCut cut(total, a.ctas);
     if ((int)blockIdx.x >= cut.ctas) return false;
     const int first = cut.start(blockIdx.x);
     tiles = cut.start(blockIdx.x + 1) - first;
     for (int b = b0; b < b1; b++) {
-        const int n = sa_seq<KT>(a.d, b).tiles * a.per_seq;
+        if (b > b0) s = sa_seq<KT>(a.d, b);
+        const int n = s.tiles * a.per_seq;
         if (at <= first && first < at + n) {
             sh_b = b;
+            sh_s = s;
             sh_off = first - at;
         }
         at += n;
     }
     __syncthreads();
     c.b = sh_b;
-    c.s = sa_seq<KT>(a.d, c.b);
+    c.s = sh_s;
     const int off = sh_off / c.s.tiles;
     c.t = sh_off - off * c.s.tiles;
     c.rt = off % a.row_tiles;
@@ -872,11 +877,30 @@ struct SaManyArgs {
     int mapped;
     int dim[2][3];  // the map's dimension (1, 2, 3) of row, head, sequence
 };
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar,
+                                            uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        :: "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
+        :: "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
+}
+
+// Queries and mask words into L2 (a share of a CTA each) before K's and V's
+// loads fill the queues to the memory: behind them they take 3 us.
+template <int HD> __device__ __forceinline__ void sa_warm(const SaArgs &a) {
+    const ds_cuda_tree_attention_t &d = a.d;
+    constexpr int LINES = HD * 2 / 128;
+    const int most = 2 * gridDim.x * TC_THREADS, step = gridDim.x * TC_THREADS, x0 = blockIdx.x * TC_THREADS + threadIdx.x;
+    const int64_t rows = (int64_t)d.batch * d.n_nodes, bytes = rows * a.words * 8, lines = rows * d.n_heads * LINES;
+    for (int x = x0; x < most && x < lines; x += step) {
+        const int r = x / LINES, nd = r / d.n_heads;
+        const uint16_t *const q = (const uint16_t *)d.q + nd / d.n_nodes * d.q_stride[0] + nd % d.n_nodes * d.q_stride[1] +
+                                  r % d.n_heads * d.q_stride[2] + x % LINES * 64;
+        asm volatile("prefetch.global.L2 [%0];" :: "l"(q));
+    }
+    for (int64_t x = (int64_t)x0 * 128; x < bytes; x += (int64_t)step * 128)
+        asm volatile("prefetch.global.L2 [%0];" :: "l"(reinterpret_cast<const char *>(d.mask) + x));
 }
 
 template <class S>
@@ -895,7 +919,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
     __shared__ int sh_bad[16];  // by item: a node's V holds NaN or infinities
     const ds_cuda_tree_attention_t &d = a.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) {
+    sa_warm<HD>(a);
+    if (tid == TC_SOFTMAX) {
         for (int u = 0; u < NU; u++) {
             mbar_init(&full[u], 32);
             mbar_init(&empty[u], S::DUAL ? 2 : 1);
@@ -937,6 +962,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         const int rg = __shfl_sync(DS_FULL, warp - TC_SOFTMAX / 32, 0), cc = lane % CH, rr = lane / CH;
         constexpr int RS = 32 / CH;
         int item = 0, units = 0;  // units so far
+        // (rows that one row tile reads once do not push the parts out of L2)
+        uint64_t policy;
+        if (a.row_tiles == 1) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+        else asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
         auto load = [&](int t, int kv) {
             const int slot = rg * S::RING + units % S::RING;
             ok = __all_sync(DS_FULL, ok && tc_wait(&empty[slot], (units / S::RING & 1) ^ 1, a.err));
@@ -953,7 +982,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                     mbar_expect_tx(&full[slot], S::UNIT);
 #pragma unroll
                     for (int k = 0; k < HD / 64; k++)
-                        tma_load_4d(unit + k * S::SUB, &args.map[kv], 64 * k, y, z, v, &full[slot]);
+                        tma_load_4d(unit + k * S::SUB, &args.map[kv], 64 * k, y, z, v, &full[slot], policy);
                 }
                 __syncwarp();
                 return;
@@ -1143,6 +1172,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 q_store();
             }
             const uint64_t *const words = d.mask + ((size_t)cu.b * d.n_nodes + (used ? nd : 0)) * a.words;
+            // the mask's word for this stream's next tile of nodes
+            auto word_of = [&](int k) { return used && k * KT < cu.s.cnt ? (uint32_t)(words[k] >> (32 * h)) : 0u; };
+            int nodes0 = max(0, cu.s.cache_tiles - cu.t);
+            if (!S::DUAL) nodes0 += (nodes0 ^ w) & 1;
+            uint32_t word = word_of(cu.t + nodes0 - cu.s.cache_tiles);
             float m = -__FLT_MAX__, l = 0.f;
             int step = done;
             // (after a wait that gave up: on without waiting, through every
@@ -1157,7 +1191,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                     const int r0 = (node ? cu.t + t - cu.s.cache_tiles : cu.t + t) * KT;
                     const int valid = (node ? cu.s.cnt : cu.s.len) - r0 - 32 * h;  // of this half's keys
                     see = valid >= 32 ? ~0u : valid > 0 ? (1u << valid) - 1 : 0;
-                    if (node) see = used && valid > 0 ? see & (uint32_t)(words[r0 / 64] >> (32 * h)) : 0;
+                    if (node) {
+                        see &= word;
+                        word = word_of(r0 / KT + STEP);
+                    }
                 }
                 ok = ok && tc_wait(&sfull[w][buf], step >> 1 & 1, a.err);
                 __syncwarp();
@@ -1358,6 +1395,23 @@ template <class S> constexpr int sj_ctas(bool wide) {
     return S::RT / sj_rows<S>(wide) * (SaMade<S>::by_dimension && wide ? S::HD / 16 : 1);
 }
 
+// Loads that stay where they are written: the compiler would move each to its
+// use, which makes the parts' latencies follow one another.
+__device__ __forceinline__ float sj_ld(const float *p) {
+    float v;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 sj_ld2(const float2 *p) {
+    float2 v;
+    asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 sj_ld4(const float *p) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
 template <class S, bool WIDE>
 __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_constant__ SaArgs a) {
     constexpr int HD = S::HD, KT = S::KT, RT = S::RT;
@@ -1368,12 +1422,12 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
     const int chunk = (d.batch + SJ_THREADS - 1) / SJ_THREADS;
     const int b0 = min(d.batch, tid * chunk), b1 = min(d.batch, b0 + chunk);
     int at;
-    const int total = sa_scan<KT, SJ_THREADS>(a, b0, b1, sh_scan, &at);
+    const SaSeq s = sa_seq<KT>(d, b);
+    const int total = sa_scan<KT, SJ_THREADS>(a, b0, b1, sa_seq<KT>(d, min(b0, d.batch - 1)), sh_scan, &at);
     if (b0 <= b && b < b1) {
         for (int y = b0; y < b; y++) at += sa_seq<KT>(d, y).tiles * a.per_seq;
         sh_off = at;
     }
-    const SaSeq s = sa_seq<KT>(d, b);
     __syncthreads();
     const SaCut cut(total, a.ctas);
     // this thread's row and first dimension, and the parts it takes
@@ -1388,7 +1442,8 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
     if (c0 == c1) return;
     float m = -__FLT_MAX__, l = 0.f, o[VN] = {};
     if (row < a.rows) {
-        constexpr int AHEAD = BYD && WIDE ? 2 : 4;
+        // four parts at a time, all their loads first
+        constexpr int AHEAD = 4;
         for (int k0 = c0 + (WIDE ? grp : 0); k0 <= c1; k0 += AHEAD * groups) {
             float2 ml[AHEAD];
             float v[AHEAD][VN];
@@ -1396,23 +1451,30 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
             for (int k = 0; k < AHEAD; k++) {
                 const int cc = min(k0 + k * groups, c1);
                 const size_t slot = (size_t)cc * 2 + (cc == c0);
-                ml[k] = a.ml[slot * RT + r];
+                ml[k] = sj_ld2(a.ml + slot * RT + r);
                 if (BYD) {
 #pragma unroll
-                    for (int e = 0; e < VN; e++) v[k][e] = a.part[(slot * HD + c + e) * RT + r];
+                    for (int e = 0; e < VN; e++) v[k][e] = sj_ld(a.part + (slot * HD + c + e) * RT + r);
                 } else {
-                    const float4 u = *reinterpret_cast<const float4 *>(a.part + (slot * RT + r) * HD + c);
+                    const float4 u = sj_ld4(a.part + (slot * RT + r) * HD + c);
                     v[k][0] = u.x, v[k][1] = u.y, v[k][2] = u.z, v[k][3] = u.w;
                 }
             }
+            float mn = m;
+#pragma unroll
+            for (int k = 0; k < AHEAD; k++) mn = fmaxf(mn, ml[k].x);
+            const float f = ex2(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < VN; e++) o[e] *= f;
 #pragma unroll
             for (int k = 0; k < AHEAD; k++) {
-                if (k0 + k * groups > c1) break;
-                const float mn = fmaxf(m, ml[k].x), f = ex2(m - mn), e2 = ex2(ml[k].x - mn);
-                m = mn;
-                l = l * f + ml[k].y * e2;
+                const bool is = k0 + k * groups <= c1;
+                const float e2 = ex2(ml[k].x - mn);
+                l += is ? ml[k].y * e2 : 0.f;
 #pragma unroll
-                for (int e = 0; e < VN; e++) o[e] = o[e] * f + v[k][e] * e2;
+                for (int e = 0; e < VN; e++) o[e] += is ? v[k][e] * e2 : 0.f;
             }
         }
     }
