@@ -2,14 +2,17 @@
 // (ds_cuda_tree_attention_dev), and the trees' mask words.
 //
 // The R = n_nodes * group query rows that share a key head are taken
-// together, so K and V are read once for all of them. The keys of a
-// (sequence, key head, row tile) item come in tiles of KT: first the cached
-// rows, then the tree's nodes. All items' tiles form one list, cut into equal
-// runs, one per CTA (two persistent CTAs an SM, up to four for head_dim 64): a
-// ragged batch and a single long sequence are spread alike, and nothing
-// about the lengths is needed on the host. A run that covers an item writes
-// its result; an item cut between CTAs leaves (max, sum, weighted V) parts
-// in the workspace, joined by sa_join_kernel.
+// together, in tiles of 8, 16, 128 or 256, so K and V are read once for all
+// rows of a tile. The keys of a (sequence, key head, row tile) item come in
+// tiles of 64: first the cached rows, then the tree's nodes. One pass keeps
+// each row's running maximum, sum and weighted V in F32. All items' tiles form
+// one list, cut into equal runs, one per persistent CTA: a ragged batch and a
+// single long sequence are spread alike, and nothing about the lengths is
+// needed on the host. A run that covers an item writes its result; an item cut
+// between CTAs leaves (max, sum, weighted V) parts in the workspace, joined by
+// sa_join_kernel. Small calls have a cluster per item instead, which joins its
+// parts through its shared memory. The order of all sums is fixed by the
+// lengths and the GPU's SM count, so results are repeatable.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -378,7 +381,12 @@ __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor 
 // loads, multiplies and sums its own keys, with no barrier but at an item's
 // end. Its K and V rows of a tile are a unit each in a ring of three: while
 // one is used, two are in flight, with eight warps an SM 128 KB of them. The
-// queries stay in registers.
+// queries stay in registers. F32 queries and weights are three BF16 planes
+// (exact), K and V two; products below 2^-24 of the largest are left out.
+// Bound by the memory for 8 rows: 64 streams of 10 heads, up to 1325 tokens, F32
+// in two planes, 93 us, 6.0 TB/s. With 16 F32 rows bound by mma.sync's rate
+// (five products an element). One stream of 662 tokens is bound by latency:
+// launch, lengths, one tile's rows, the cluster's join: 7.9 us.
 template <int HD_, int NG_, int PL_, int QT_> struct SaFew {
     static constexpr int HD = HD_, NG = NG_, PL = PL_, QT = QT_;
     static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
@@ -772,7 +780,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
 }
 
 // ---- many rows: tcgen05 ----------------------------------------------------------
-// 16-bit types with more than 32 rows. The 128 query rows of a block are the
+// 16-bit types with more than 16 rows. The 128 query rows of a block are the
 // rows of tcgen05.mma (M = 128, accumulators in tensor memory); two softmax
 // groups of 256 threads, two a row, work on two streams:
 //   DUAL (more than 128 rows): the streams are two blocks of rows that share
@@ -786,6 +794,15 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
 // 60 cycles a product, which one warp could not do for both), the next tile's
 // S before this one's P is there. m is the row's maximum of its first tile,
 // or of a later one whose weights passed 2^10, so that O is rarely rescaled.
+// P has the cache's type: its rounding is of the same size as V's. Bound by
+// the memory at 124 rows (8 streams, 32 heads on 8, head_dim 128, up to 8191
+// tokens: 47.6 us, 3.9 TB/s over the whole call, the runs themselves at the
+// memory's rate, 10 us of start and item ends, 8 us of join), by the softmax at
+// 512 rows (one stream, 16 heads on 2, head_dim 64, 131071 tokens: 77 us, 450
+// TFLOP/s; a step of 2 x 128 rows and 64 keys takes 1850 cycles, 1024 of them
+// the exponentials' least). Tried for the latter: P in columns of its own, which
+// lets S be issued a product earlier (82 us), turns of the two streams (97
+// against 85 us at the time), packed F32 operations (no change).
 // Two producer warps bring K and V rows into a ring each (of K and of V, or of
 // the streams) in the 128-byte swizzle, in the order the products take them.
 constexpr int TC_SOFTMAX = 512, TC_PRODUCERS = 64, TC_THREADS = TC_SOFTMAX + TC_PRODUCERS + 64;
@@ -1543,10 +1560,18 @@ constexpr int SA_CLUSTER = 16;
 // Calls whose items are few enough for a cluster each in one wave, with at
 // most 8 tiles a CTA, are joined in the clusters: one launch, no workspace.
 // Their tiles are bounded by the cache's room, the lengths not being known
-// here. Others take the list.
-template <class S> static bool sa_clusters(const ds_cuda_tree_attention_t *d, int items, int sms) {
-    const long long tiles = (d->kv_max + S::KT - 1) / S::KT + (d->n_nodes + S::KT - 1) / S::KT;
-    return (long long)items * SA_CLUSTER <= sms * S::PER_SM && tiles <= 8 * SA_CLUSTER;
+// here. Others take the list. Clusters have 16 CTAs, or 8 with eight rows a
+// tile (with 16, F32, 32 rows of 10 heads over 662 tokens take 14 us in
+// clusters of 8 and 12.6 in the list).
+// (One stream, 10 heads, 662 tokens, F32 in two planes: one node takes 7.9 us
+// on the GPU either way, but the call 7 us of the host's time instead of 13.)
+template <class S> static long long sa_tiles(const ds_cuda_tree_attention_t *d) {
+    return (d->kv_max + S::KT - 1) / S::KT + (d->n_nodes + S::KT - 1) / S::KT;
+}
+template <class S> static int sa_clusters(const ds_cuda_tree_attention_t *d, int items, int sms) {
+    for (int n = SA_CLUSTER; n >= (S::RT == 8 ? 8 : SA_CLUSTER); n /= 2)
+        if ((long long)items * n <= sms * S::PER_SM && sa_tiles<S>(d) <= 8 * n) return n;
+    return 0;
 }
 
 // The cache's K or V as a tensor map: the dimensions after the head's own in
@@ -1579,7 +1604,7 @@ static bool sa_map(const ds_cuda_tree_attention_t &d, int kv, int kt, CUtensorMa
 }
 
 template <class S> struct SaRun {
-    static bool clusters(const SaArgs &a) { return !SaMade<S>::by_dimension && sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
+    static int clusters(const SaArgs &a) { return SaMade<S>::by_dimension ? 0 : sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
     static size_t workspace(const SaArgs &a) {
         // two parts a CTA, then their maxima and sums
         return clusters(a) ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
@@ -1598,17 +1623,17 @@ template <class S> struct SaRun {
     }
     static cudaError_t run(SaArgs a, int device, cudaStream_t st) {
         void *args[] = {&a};
-        if constexpr (!SaMade<S>::by_dimension) if (clusters(a)) {
+        if constexpr (!SaMade<S>::by_dimension) if (const int ncta = clusters(a)) {
             const cudaError_t e = attributes<true>(device);
             if (e != cudaSuccess) return e;
             cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(a.d.batch * a.per_seq * SA_CLUSTER);
+            cfg.gridDim = dim3(a.d.batch * a.per_seq * ncta);
             cfg.blockDim = dim3(SA_THREADS);
             cfg.dynamicSmemBytes = S::SMEM;
             cfg.stream = st;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = SA_CLUSTER;
+            attr[0].val.clusterDim.x = ncta;
             attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 1;
@@ -1635,24 +1660,36 @@ template <class S> struct SaRun {
     }
 };
 
-// f(instantiation) for a call, by its rows. F32 queries take at most 32 at a
-// time: their three planes fill the shared memory.
-template <int HD, int QT, class F> static auto sa_pick16(int rows, bool brief, F f) {
-    return rows <= 8             ? f(SaRun<SaFew<HD, 1, 1, QT>>())
+// f(instantiation) for a call, by its rows a KV head. F32 takes mma.sync, 8 or
+// 16 rows at a time (tcgen05 has no form for its three planes' separate sums).
+// Eight at a time also where each tile of eight has a cluster of at most two
+// tiles a CTA: one stream of 10 heads, 662 tokens, 16 rows, F32 10.1 us
+// against 11.6 us, BF16 8.7 against 9.9 (with three tiles a CTA it loses: 16
+// against 12 us for 20 rows of 8 KV heads, 1000 tokens).
+// 16-bit types take mma.sync up to 16 rows, and for more where the call is brief: at
+// most 8 tiles a CTA, by the cache's room. Else tcgen05, one block of 128 rows
+// or two. BF16, mma.sync against tcgen05: 64 streams of 10 heads, up to 1325
+// tokens, 8 / 16 / 24 / 48 rows 51 / 68 / 118 / 184 us against 79 / 80 / 81 /
+// 84 us (but 8 streams on 8 KV heads, up to 8191 tokens, 16 rows 46 against
+// 41); brief: one stream, 662 tokens, 32 / 64 / 128 rows 11 / 14 / 20 us
+// against 20 / 20 / 27 us.
+template <int HD, int QT, class F> static auto sa_pick16(int rows, bool apart, bool brief, F f) {
+    return apart                 ? f(SaRun<SaFew<HD, 1, 1, QT>>())
            : rows <= 16 || brief ? f(SaRun<SaFew<HD, 2, 1, QT>>())
            : rows <= 128         ? f(SaRun<SaMany<HD, false, QT>>()) : f(SaRun<SaMany<HD, true, QT>>());
 }
 template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, int sms, F f) {
     constexpr int P = DS_CUDA_SPEC_F32;
     const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
-    const bool brief = sa_clusters<SaFew<HD, 2, 1, DS_CUDA_SPEC_BF16>>(d, d->batch * d->n_kv_heads * ((rows + 15) / 16), sms);
-    if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, brief, f);
-    if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, brief, f);
+    using Few = SaFew<HD, 2, 1, DS_CUDA_SPEC_BF16>;
+    const bool brief = (double)d->batch * d->n_kv_heads * ((rows + 15) / 16) * sa_tiles<Few>(d) <= 8.0 * sms * Few::PER_SM;
+    using Eight = SaFew<HD, 1, 2, P>;
+    const bool apart = rows <= 8 || 2 * sa_clusters<Eight>(d, d->batch * d->n_kv_heads * ((rows + 7) / 8), sms) >= sa_tiles<Eight>(d);
+    if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, apart, brief, f);
+    if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, apart, brief, f);
     if (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo)
-        return rows <= 8    ? f(SaRun<SaFew<HD, 1, 2, P>>())
-               : f(SaRun<SaFew<HD, 2, 2, P>>());
-    return rows <= 8    ? f(SaRun<SaFew<HD, 1, 1, P>>())
-           : f(SaRun<SaFew<HD, 2, 1, P>>());
+        return apart ? f(SaRun<SaFew<HD, 1, 2, P>>()) : f(SaRun<SaFew<HD, 2, 2, P>>());
+    return apart ? f(SaRun<SaFew<HD, 1, 1, P>>()) : f(SaRun<SaFew<HD, 2, 1, P>>());
 }
 template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, int sms, F f) {
     return d->head_dim == 64 ? sa_pick_hd<64>(d, sms, f) : sa_pick_hd<128>(d, sms, f);

@@ -117,6 +117,77 @@ def test_attention_many_rows_long(spec, kind, hd, n, group):
     Case(kind, [5003, 0, 517], [n, max(1, n - 9), n], n, 2, group, hd, seed=hd + n).check(spec)
 
 
+# Room for a long cache: calls that are brief by it take the kernel for few rows
+ROOM = 20000
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("layout", ["bhsd", "bshd"])
+@pytest.mark.parametrize("n,group", [(17, 3), (33, 2), (64, 1), (64, 8), (130, 1)])
+def test_attention_many_rows_with_room(spec, kind, hd, layout, n, group):
+    lens = [0, 1, 31, 64, 65, 300]
+    counts = [n, max(1, n - 1), n, 1, 0, max(1, n // 2)]
+    Case(kind, lens, counts, n, 2, group, hd, seed=n + group, pad=ROOM, layout=layout).check(spec)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("masks", ["none", "random"])
+@pytest.mark.parametrize("n,group", [(40, 2), (70, 4)])
+def test_attention_many_rows_masks(spec, kind, masks, n, group):
+    Case(kind, [0, 40, 200], [n, n - 3, n], n, 2, group, 64, seed=5, masks=masks, pad=ROOM).check(spec)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_attention_many_rows_scales(spec, kind, scale):
+    c = Case(kind, [150, 1], [50, 50], 50, 2, 2, 64, seed=21, pad=ROOM)
+    c.scale = scale
+    c.q = (c.q * (0.25 if scale == 3.0 else 1)).to(c.q.dtype)
+    assert rel(c.run(spec, scale=scale), c.want()[0]) < TOL[kind]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [7, 14])
+def test_attention_many_rows_nan_in_a_node(spec, kind, hd, group):
+    c = Case(kind, [70, 3], [10, 10], 10, 2, group, hd, seed=9, pad=ROOM)
+    c.tk[0, :, 7] = float("nan")
+    c.tv[1, :, 8] = float("inf")
+    c.allowed[:, :, 7:9] = False
+    c.allowed[0, 7, 7] = c.allowed[1, 8, 8] = True
+    c.mask = R.words(c.allowed).cuda()
+    out, (o, _) = c.run(spec), c.want()
+    assert torch.isnan(out[0, 7]).all() and not torch.isfinite(out[1, 8]).any()
+    fine = torch.isfinite(o)
+    assert torch.equal(torch.isfinite(out), fine)
+    assert rel(out[fine], o[fine]) < TOL[kind]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("group", [8, 40])
+def test_attention_many_rows_scores_far_apart(spec, kind, group):
+    # the largest score of some rows arrives late and is far above the first
+    c = Case(kind, [400, 333], [4, 4], 4, 2, group, 128, seed=10, pad=ROOM)
+    q0 = c.q[0, 1, 0].float()
+    c.k[0, 0, 390] = (q0 * 60 / q0.norm()).to(c.k.dtype)
+    q1 = c.q[1, 2, group + 1].float()
+    c.k[1, 1, 200] = (q1 * 30 / q1.norm()).to(c.k.dtype)
+    assert rel(c.run(spec), c.want()[0]) < TOL[kind]
+
+
+def test_attention_many_rows_repeatable_and_far(spec):
+    # equal bits again, and rows 2^32 elements apart
+    c = Case("f16", [150, 140], [33, 30], 33, 2, 4, 64, seed=13, pad=ROOM)
+    want = c.check(spec)
+    room = torch.empty((1 << 32) + 2 * (150 + ROOM) * 64, dtype=torch.float16, device="cuda")
+    far = room.as_strided(c.k.shape, (1 << 32, (150 + ROOM) * 64, 64, 1))
+    far.copy_(c.k)
+    c.k = far
+    for _ in range(5):
+        assert torch.equal(c.run(spec), want)
+
+
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
 @pytest.mark.parametrize("kind,n", [("pair", 7), ("pair", 20), ("f16", 12), ("bf16", 20), ("bf16", 50)])
 def test_attention_scales(spec, kind, n, scale):
