@@ -601,7 +601,8 @@ int ds_cuda_tree_mask_dev(ds_cuda_ctx_t *ctx, const int *parents, const int *nod
 /* probs[r] = softmax(logits[r] / temperature[r]) in F32 for `rows` rows of
  * `vocab` logits of a DS_CUDA_SPEC_* type, row_stride elements apart; probs
  * is [rows x vocab]. temperature [rows] or NULL (1). A temperature <= 0
- * gives 1 at the row's largest logit (the lowest index wins ties). -infinity
+ * gives 1 at the row's largest logit (the lowest index wins ties), an
+ * infinite one equal shares to all logits but -infinity. A logit of -infinity
  * is probability 0, a row of nothing else is zeros, a NaN or +infinity
  * makes its row NaN. Limits: vocab <= 917504. */
 int ds_cuda_token_probs_dev(ds_cuda_ctx_t *ctx, int type, const void *logits, int rows, int vocab, int64_t row_stride,
