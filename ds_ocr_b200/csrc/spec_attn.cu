@@ -30,6 +30,7 @@ namespace ds {
 constexpr int SA_MAX_NODES = 256;
 constexpr int SA_THREADS = 128;
 constexpr int SA_WARPS = SA_THREADS / 32;
+constexpr int SA_CLUSTER = 16;  // CTAs of a cluster, at most
 
 struct SaArgs {
     ds_cuda_tree_attention_t d;
@@ -236,11 +237,10 @@ __device__ __forceinline__ bool sa_begin(const SaArgs &a, SaCursor &c, int &tile
     __shared__ SaSeq sh_s;
     const int tid = threadIdx.x;
     if (CLUSTER) {
-        cluster_arrive();
-        const int item = blockIdx.x / cluster_ctas(), rank = cluster_rank();
-        c.b = item / a.per_seq;
-        c.rt = item % a.row_tiles;
-        c.g = item % a.per_seq / a.row_tiles;
+        const int rank = cluster_rank();
+        c.b = blockIdx.z;
+        c.g = blockIdx.y;
+        asm("mov.u32 %0, %%clusterid.x;" : "=r"(c.rt));
         c.s = sa_seq<KT>(a.d, c.b);
         const SaCut cut(c.s.tiles, cluster_ctas());
         c.t = rank < cut.ctas ? cut.start(rank) : 0;
@@ -355,17 +355,27 @@ template <int RT, int HD>
 __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor &c, const float4 *sh_part,
                                                 const float2 *sh_pml) {
     __syncwarp();
-    cluster_wait();  // (the arrival at the start)
     cluster_arrive();
     cluster_wait();  // every CTA's part is in its shared memory
     const int n = cluster_ctas(), used = min(n, c.s.tiles), left = min(RT, a.rows - c.rt * RT);
     for (int x = cluster_rank() * SA_THREADS + threadIdx.x; x < left * (HD / 4); x += n * SA_THREADS) {
         const int r = x / (HD / 4);
+        // (loads in batches: one after the other they take 3000 cycles)
+        float2 ml[SA_CLUSTER];
         float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < used; k++) mm = fmaxf(mm, cluster_ld2(&sh_pml[r], k).x);
-        for (int k = 0; k < used; k++) {
-            const float2 ml = cluster_ld2(&sh_pml[r], k);
-            sa_add(v, ll, cluster_ld4(&sh_part[x], k), ml.y, ex2(ml.x - mm));
+#pragma unroll
+        for (int k = 0; k < SA_CLUSTER; k++) ml[k] = cluster_ld2(&sh_pml[r], min(k, used - 1));
+#pragma unroll
+        for (int k = 0; k < SA_CLUSTER; k++) mm = fmaxf(mm, ml[k].x);
+#pragma unroll
+        for (int k0 = 0; k0 < SA_CLUSTER; k0 += 8) {
+            if (k0 >= used) break;
+            float4 u[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) u[k] = cluster_ld4(&sh_part[x], min(k0 + k, used - 1));
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k0 + k < used) sa_add(v, ll, u[k], ml[k0 + k].y, ex2(ml[k0 + k].x - mm));
         }
         sa_finish(a, c.b, c.g, c.rt * RT + r, c.s.cnt, 4 * (x % (HD / 4)), mm, ll, v);
     }
@@ -474,6 +484,37 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
 #pragma unroll
             for (int p = 0; p < S::PL; p++) from[kv][p] += step[kv] * (S::KT / RS);
     };
+    uint64_t bits[NG][2];                 // of rows 2 gc and 2 gc + 1 of each group, for the tree's tile at hand
+    auto word = [&](int n, int e, int k) -> uint64_t {
+        const int row = cu.rt * S::RT + 8 * n + 2 * gc + e, nd = row / a.group, left = cu.s.cnt - 64 * k;
+        if (row >= a.rows || nd >= cu.s.cnt || left <= 0) return 0;
+        return d.mask[((size_t)cu.b * d.n_nodes + nd) * a.words + k] & (left < 64 ? (1ull << left) - 1 : ~0ull);
+    };
+    // an item's queries as they are (16-bit ones two in the first float)
+    float2 qu[NG][KK][2];
+    auto q_load = [&]() {
+#pragma unroll
+        for (int n = 0; n < NG; n++) {
+            const int row = cu.rt * S::RT + 8 * n + gr;
+            const bool ok = row < a.rows;
+            const int64_t qo = ok ? cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
+                                        (cu.g * a.group + row % a.group) * d.q_stride[2] + 2 * gc : 0;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float2 &u = qu[n][kk][h];
+                    u = make_float2(0.f, 0.f);
+                    if (!ok) continue;
+                    if (F32) u = *reinterpret_cast<const float2 *>((const float *)d.q + qo + 16 * kk + 8 * h);
+                    else u.x = *reinterpret_cast<const float *>((const uint16_t *)d.q + qo + 16 * kk + 8 * h);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; e++) bits[n][e] = word(n, e, 0);
+        }
+    };
+    // (the first item's before the rows: they arrive while those are asked for)
+    q_load();
     if (tiles > 0) {
         aim();
         load(0, 0);
@@ -482,42 +523,30 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
     }
 
     uint32_t qf[NG][S::QP][KK][2];
-    uint64_t bits[NG][2];                 // of rows 2 gc and 2 gc + 1 of each group, for the tree's tile at hand
-    auto word = [&](int n, int e, int k) -> uint64_t {
-        const int row = cu.rt * S::RT + 8 * n + 2 * gc + e, nd = row / a.group, left = cu.s.cnt - 64 * k;
-        if (row >= a.rows || nd >= cu.s.cnt || left <= 0) return 0;
-        return d.mask[((size_t)cu.b * d.n_nodes + nd) * a.words + k] & (left < 64 ? (1ull << left) - 1 : ~0ull);
-    };
     float o[KK][NG][4], m[NG][2], l[NG][2];
     bool fresh = true, whole = cu.t == 0;
     int slot = 0;  // of K; V's follows it, then the next tile's
     for (int i = 0; i < tiles; i++, slot = wrap(slot + 2)) {
         if (fresh) {
             fresh = false;
+            if (i > 0) q_load();
 #pragma unroll
             for (int n = 0; n < NG; n++) {
-                const int row = cu.rt * S::RT + 8 * n + gr;
-                const bool ok = row < a.rows;
-                const int64_t qo = ok ? cu.b * d.q_stride[0] + (row / a.group) * d.q_stride[1] +
-                                            (cu.g * a.group + row % a.group) * d.q_stride[2] + 2 * gc : 0;
 #pragma unroll
                 for (int kk = 0; kk < KK; kk++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         if (F32) {
-                            float2 u = make_float2(0.f, 0.f);
-                            if (ok) u = *reinterpret_cast<const float2 *>((const float *)d.q + qo + 16 * kk + 8 * h);
                             uint32_t p[3];
-                            split3(u.x, u.y, p);
+                            split3(qu[n][kk][h].x, qu[n][kk][h].y, p);
 #pragma unroll
                             for (int k = 0; k < S::QP; k++) qf[n][k][kk][h] = p[k];
                         } else {
-                            qf[n][0][kk][h] = ok ? *reinterpret_cast<const uint32_t *>((const uint16_t *)d.q + qo + 16 * kk + 8 * h) : 0;
+                            qf[n][0][kk][h] = __float_as_uint(qu[n][kk][h].x);
                         }
                     }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    bits[n][e] = word(n, e, 0);
                     m[n][e] = -__FLT_MAX__;
                     l[n][e] = 0.f;
                 }
@@ -1555,7 +1584,6 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
     }
 }
 
-constexpr int SA_CLUSTER = 16;
 
 // Calls whose items are few enough for a cluster each in one wave, with at
 // most 8 tiles a CTA, are joined in the clusters: one launch, no workspace.
@@ -1627,7 +1655,7 @@ template <class S> struct SaRun {
             const cudaError_t e = attributes<true>(device);
             if (e != cudaSuccess) return e;
             cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(a.d.batch * a.per_seq * ncta);
+            cfg.gridDim = dim3(a.row_tiles * ncta, a.d.n_kv_heads, a.d.batch);
             cfg.blockDim = dim3(SA_THREADS);
             cfg.dynamicSmemBytes = S::SMEM;
             cfg.stream = st;
