@@ -357,12 +357,14 @@ __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor 
     __syncwarp();
     cluster_arrive();
     cluster_wait();  // every CTA's part is in its shared memory
-    const int n = cluster_ctas(), used = min(n, c.s.tiles), left = min(RT, a.rows - c.rt * RT);
-    for (int x = cluster_rank() * SA_THREADS + threadIdx.x; x < left * (HD / 4); x += n * SA_THREADS) {
-        const int r = x / (HD / 4);
+    const int used = min(cluster_ctas(), c.s.tiles), left = min(RT, a.rows - c.rt * RT);
+    static_assert(RT * (HD / 4) <= 8 * SA_THREADS, "a cluster's threads take four dimensions of a row at most");
+    const int x = cluster_rank() * SA_THREADS + threadIdx.x, r = x / (HD / 4);
+    const bool mine = x < left * (HD / 4);
+    float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (mine) {
         // (loads in batches: one after the other they take 3000 cycles)
         float2 ml[SA_CLUSTER];
-        float mm = -__FLT_MAX__, ll = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < SA_CLUSTER; k++) ml[k] = cluster_ld2(&sh_pml[r], min(k, used - 1));
 #pragma unroll
@@ -377,10 +379,10 @@ __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor 
             for (int k = 0; k < 8; k++)
                 if (k0 + k < used) sa_add(v, ll, u[k], ml[k0 + k].y, ex2(ml[k0 + k].x - mm));
         }
-        sa_finish(a, c.b, c.g, c.rt * RT + r, c.s.cnt, 4 * (x % (HD / 4)), mm, ll, v);
     }
     __syncwarp();
-    cluster_arrive();
+    cluster_arrive();  // before the results are written: it would wait for them
+    if (mine) sa_finish(a, c.b, c.g, c.rt * RT + r, c.s.cnt, 4 * (x % (HD / 4)), mm, ll, v);
     cluster_wait();  // no CTA leaves while another reads its part
 }
 
