@@ -398,7 +398,8 @@ __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor 
 // Bound by the memory for 8 rows: 64 streams of 10 heads, up to 1325 tokens, F32
 // in two planes, 93 us, 6.0 TB/s. With 16 F32 rows bound by mma.sync's rate
 // (five products an element). One stream of 662 tokens is bound by latency:
-// launch, lengths, one tile's rows, the cluster's join: 7.9 us.
+// lengths, one tile's rows, the tile's steps, the cluster's join follow one
+// another: 7.1 us for one node, 9.1 us for 16.
 template <int HD_, int NG_, int PL_, int QT_> struct SaFew {
     static constexpr int HD = HD_, NG = NG_, PL = PL_, QT = QT_;
     static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
@@ -1593,8 +1594,8 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
 // here. Others take the list. Clusters have 16 CTAs, or 8 with eight rows a
 // tile (with 16, F32, 32 rows of 10 heads over 662 tokens take 14 us in
 // clusters of 8 and 12.6 in the list).
-// (One stream, 10 heads, 662 tokens, F32 in two planes: one node takes 7.9 us
-// on the GPU either way, but the call 7 us of the host's time instead of 13.)
+// (One stream, 10 heads, 662 tokens, F32 in two planes: one node takes 7.1 us
+// on the GPU against 7.9, and the call 7 us of the host's time instead of 13.)
 template <class S> static long long sa_tiles(const ds_cuda_tree_attention_t *d) {
     return (d->kv_max + S::KT - 1) / S::KT + (d->n_nodes + S::KT - 1) / S::KT;
 }
@@ -1694,7 +1695,8 @@ template <class S> struct SaRun {
 // 16 rows at a time (tcgen05 has no form for its three planes' separate sums).
 // Eight at a time also where each tile of eight has a cluster of at most two
 // tiles a CTA: one stream of 10 heads, 662 tokens, 16 rows, F32 10.1 us
-// against 11.6 us, BF16 8.7 against 9.9 (with three tiles a CTA it loses: 16
+// against 11.6 us, BF16 8.7 against 9.9, both before the join's loads were
+// batched (with three tiles a CTA it loses: 16
 // against 12 us for 20 rows of 8 KV heads, 1000 tokens).
 // 16-bit types take mma.sync up to 16 rows, and for more where the call is brief: at
 // most 8 tiles a CTA, by the cache's room. Else tcgen05, one block of 128 rows
