@@ -155,6 +155,16 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// With 16-bit queries the softmax weights are rounded to that type for the
+// product with V (as V itself has been), while their sums stay in F32. FP16 ends
+// at 2^-24: against a maximum of 1, weights below 2^-25 would be zero in the
+// product, all of a result whose larger weights meet small V. Its weights are
+// therefore 2^SA_LIFT times as large (maximum, sum and weighted V alike, so that
+// nothing has to be taken back), which leaves an error of 2^-32 each. More would
+// not fit: sums of weights may reach 2^15, and near 2^24 the maximum less
+// SA_LIFT is rounded. (Where V is large throughout, the F32 sums end at 2^-25.)
+constexpr float SA_LIFT = 7.f;
+template <bool F16> __device__ __forceinline__ float sa_lift() { return F16 ? SA_LIFT : 0.f; }
 // Byte offset of 16-byte chunk c of row r in a [rows][HD] 16-bit tile: the
 // chunk is xor-ed with the row, so that ldmatrix's 8 rows meet 8 bank groups.
 template <int HD> __device__ __forceinline__ uint32_t sw(int r, int c) { return (uint32_t)(r * HD * 2 + ((c ^ (r & 7)) << 4)); }
@@ -632,8 +642,8 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     mx[n][e] = m[n][e];
-                    if (see >> (4 * n + e) & 1) mx[n][e] = fmaxf(mx[n][e], s[n][e] * a.scale2);
-                    if (see >> (4 * n + e + 2) & 1) mx[n][e] = fmaxf(mx[n][e], s[n][e + 2] * a.scale2);
+                    if (see >> (4 * n + e) & 1) mx[n][e] = fmaxf(mx[n][e], __fmul_rn(s[n][e], a.scale2));
+                    if (see >> (4 * n + e + 2) & 1) mx[n][e] = fmaxf(mx[n][e], __fmul_rn(s[n][e + 2], a.scale2));
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(DS_FULL, mx[n][e], w));
                     grew |= mx[n][e] > m[n][e];
@@ -658,11 +668,15 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
             }
             // the weights, and their fragments: the score fragment's 8 x 8
             // blocks [key][row] transposed are those of P^T [key] for the rows
+            // (FP16: from the rounded products that the maximum was taken of,
+            // so that the largest weight is 2^SA_LIFT whatever the scores' size)
 #pragma unroll
             for (int n = 0; n < NG; n++) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    s[n][e] = see >> (4 * n + e) & 1 ? ex2(__fmaf_rn(s[n][e], a.scale2, -m[n][e & 1])) : 0.f;
+                    const float x = F16 ? __fsub_rn(__fmul_rn(s[n][e], a.scale2), m[n][e & 1] - sa_lift<F16>())
+                                        : __fmaf_rn(s[n][e], a.scale2, -m[n][e & 1]);
+                    s[n][e] = see >> (4 * n + e) & 1 ? ex2(x) : 0.f;
                     l[n][e & 1] += s[n][e];
                 }
 #pragma unroll
@@ -775,7 +789,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
                 for (int e = 0; e < 2; e++) {
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(DS_FULL, l[n][e], w);
-                    if (gr == 0) sh_ml[warp][8 * n + 2 * gc + e] = make_float2(m[n][e], l[n][e]);
+                    if (gr == 0) sh_ml[warp][8 * n + 2 * gc + e] = make_float2(m[n][e] - sa_lift<F16>(), l[n][e]);
                 }
 #pragma unroll
             for (int ph = 0; ph < S::PHASES; ph++) {
@@ -825,8 +839,8 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
 // operand. A warp of its own issues a stream's products (issuing takes about
 // 60 cycles a product, which one warp could not do for both), the next tile's
 // S before this one's P is there. m is the row's maximum of its first tile,
-// or of a later one whose weights passed 2^10, so that O is rarely rescaled.
-// P has the cache's type: its rounding is of the same size as V's. Bound by
+// or of a later one whose weights passed 2^10 (FP16: 2^8), so that O is rarely
+// rescaled. P has the cache's type: its rounding is of the same size as V's. Bound by
 // the memory at 124 rows (8 streams, 32 heads on 8, head_dim 128, up to 8191
 // tokens: 47.6 us, 3.9 TB/s over the whole call, the runs themselves at the
 // memory's rate, 10 us of start and item ends, 8 us of join), by the softmax at
@@ -1263,7 +1277,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 };
                 // weights of the row's keys with m, their sum, and packed in pairs
                 auto weigh = [&]() {
-                    const float mc = fmaxf(m * c, -__FLT_MAX__);
+                    const float mc = fmaxf(m * c, -__FLT_MAX__) - sa_lift<F16>();
                     float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
@@ -1290,9 +1304,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                     // The sum tells whether m still serves: a tile that passes
                     // 2^10 in either half of any of the 32 rows is done again
                     // with the true maxima. (So a weight is at most 2^10, and m
-                    // never above the row's maximum.)
+                    // never above the row's maximum. FP16: 2^15, which is 2^8
+                    // times 2^SA_LIFT.)
                     weigh();
-                    if (bar_or(pair, 64, !(lt <= 1024.f))) {
+                    if (bar_or(pair, 64, !(lt <= (F16 ? 32768.f : 1024.f)))) {
                         const float was = m;
                         tmem_ld32(ts + 32 * h, v);
                         look();
@@ -1338,7 +1353,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 to_next_item();
                 q_load();
             }
-            sh_ml[w][h][i] = make_float2(fmaxf(m * c, -__FLT_MAX__), l);
+            sh_ml[w][h][i] = make_float2(fmaxf(m * c, -__FLT_MAX__) - sa_lift<F16>(), l);
             if (ok) ok = tc_wait(&odone[0], item & 1, a.err);
             if (ok) ok = tc_wait(&odone[1], item & 1, a.err);
             ok = __all_sync(DS_FULL, ok);

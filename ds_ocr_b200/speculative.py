@@ -79,9 +79,10 @@ class Speculative:
         cached rows k, v [batch x n_kv_heads x kv_max x head_dim] below lens
         [batch] (int32) and the tree's own tree_k, tree_v [batch x n_kv_heads
         x n_nodes x head_dim] where the mask words [batch x n_nodes x words]
-        (int64) allow it. bfloat16 and float16 throughout, or float32 q with
-        each of k, v, tree_k, tree_v a bfloat16 plane or a (plane, lo plane)
-        pair (the decoder's cache form). counts [batch]: nodes in use (the
+        (int64) allow it. bfloat16 and float16 throughout (weights rounded
+        to that type for the product with v, sums in float32), or float32 q
+        with each of k, v, tree_k, tree_v a bfloat16 plane or a (plane, lo
+        plane) pair (the decoder's cache form). counts [batch]: nodes in use (the
         other rows are zeros); scale: default head_dim ** -0.5; lse: optional
         [batch x n_nodes x n_heads] float32 output. Returns out."""
         return self._spec.tree_attention(self.ctx.h, self._index, q, k, v, tree_k, tree_v, lens, mask, counts, scale, out, lse)

@@ -557,8 +557,10 @@ int ds_cuda_prefill_stage_ms(ds_cuda_ctx_t *ctx, float *ms);
 /* Attention of the trees' nodes over cache and tree. Node i of sequence b
  * attends the lens[b] cached rows and the nodes j < nodes[b] whose bit j is
  * set in its mask words; head h reads K and V head h / (n_heads / n_kv_heads).
- * out = softmax(scale * q k) v with maximum, sums and products in F32. A row
- * that attends nothing, and padding, is zeros (its lse -infinity). Rows and
+ * out = softmax(scale * q k) v with maximum, weights and sums in F32; BF16
+ * and F16 calls round the weights to that type for the product with v (by
+ * 2^-9 or 2^-12 of each; F16 by 2^-32 of the row's largest where that is more),
+ * as they round the result; F32 calls do not. A row that attends nothing, and padding, is zeros (its lse -infinity). Rows and
  * nodes that a query does not attend have no influence, whatever they hold
  * (NaN and infinities included). lens and nodes are clamped to
  * [0, kv_max] and [0, n_nodes].

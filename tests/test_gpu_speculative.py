@@ -257,6 +257,28 @@ def test_attention_scores_far_apart(spec, kind):
     assert rel(out, o) < max(TOL[kind], 1.5e-5)
 
 
+@pytest.mark.parametrize("kind,tol", [("f16", 2.0 ** -6), ("bf16", TOL["bf16"])])
+@pytest.mark.parametrize("group", [4, 40])
+def test_attention_small_weights_are_not_lost(spec, kind, tol, group):
+    # Eight keys of weight 1 and V 0 at the start, and 2^15 of weight 2^-25.03
+    # (below half of float16's smallest value) and V 1, which make all of the
+    # result. Enough sequences for some to be one CTA's alone; they share one
+    # cache. float16: a weight's error is 2^-32, 2^-6.97 of these, and the
+    # sums' and the result's (2^-10 each) come on top.
+    keys, b, hd = 1 << 15, 4 * torch.cuda.get_device_properties(0).multi_processor_count + 8, 64
+    t = torch.float16 if kind == "f16" else torch.bfloat16
+    k = torch.zeros(1, 1, keys, hd, dtype=t, device="cuda")
+    v = torch.ones_like(k)
+    k[:, :, :128:16, 0], v[:, :, :128:16] = 16, 0
+    q = torch.zeros(b, 1, group, hd, dtype=t, device="cuda")
+    q[..., 0] = 1
+    node = torch.zeros(b, 1, 1, hd, dtype=t, device="cuda")
+    out = spec.tree_attention(q, k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1), node, node, torch.full((b,), keys, **I32),
+                              torch.zeros(b, 1, 1, dtype=torch.long, device="cuda"), scale=25.03 * np.log(2) / 16)
+    x = (keys - 8) * 2.0 ** -25.03
+    assert float((out.double() * (8 + x) / x - 1).abs().max()) < tol
+
+
 def test_attention_lowest_values(spec):
     # keys so large that scores reach the float32 range's end: minus infinity
     # for one query (it attends nothing), plus infinity (NaN) for another
