@@ -124,7 +124,11 @@ __global__ void __launch_bounds__(SV_THREADS) tree_verify_kernel(const __grid_co
             if (j < jn) r[j] = __ldg(row + v0 + 32 * j);
     };
 
-    int cur = 0, nrej = 0, deep = 0;
+    // Rejections are numbered through the whole walk, those at the current node
+    // from `base` on: no entry of mass and gone is written twice, so a warp that
+    // still replays an earlier node's reads what was there, and those it reads
+    // have a barrier (sum's) behind them.
+    int cur = 0, nrej = 0, base = 0, deep = 0;
     float m = 1.f;
     if (tid == 0) way[0] = 0;
     for (int c = 1; c < cnt; c++) {
@@ -132,18 +136,18 @@ __global__ void __launch_bounds__(SV_THREADS) tree_verify_kernel(const __grid_co
         const int x = tok[c];
         const float p = pd[c];
         float rx = pt[c];  // r(x): the rejections so far replayed for one token
-        for (int k = 0; k < nrej; k++)
+        for (int k = base; k < nrej; k++)
             if (draft || gone[k] == x) rx = fmaxf(__fsub_rn(rx, __fmul_rn(mass[k], p)), 0.f);
         if (x >= 0 && x < V && __fmul_rn(acc_u[c], __fmul_rn(p, m)) < rx) {
             cur = c;
-            nrej = 0;
+            base = nrej;
             m = 1.f;
             deep++;
             if (tid == 0) way[deep] = c;
             continue;
         }
         const float *row = target + cur * d.target_stride[1];
-        if (nrej == 0) load(row);
+        if (nrej == base) load(row);
         if (draft) {
             const float *drow = draft + cur * d.draft_stride[1];
             float q[VPT];
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(SV_THREADS) tree_verify_kernel(const __grid_co
     }
     // the next token: from the residual whose sums were taken last, or from
     // the target's row where nothing was rejected or no mass is left
-    if (nrej == 0 || total == 0) {
+    if (nrej == base || total == 0) {
         load(target + cur * d.target_stride[1]);
         sum();
     }

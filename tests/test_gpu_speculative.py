@@ -533,6 +533,32 @@ def test_verify_many_rejections_at_one_node(spec):
     check_verify(spec, s)
 
 
+def test_verify_chains_of_one_token_after_a_rejection(spec):
+    # certain drafts: at every level a child is rejected, its sibling accepted,
+    # and the sibling's first child, rejected, has the sibling's own token, so
+    # that the rejected tokens of a node must not be taken for those of the next
+    b, vocab, levels = 256, 12, 40
+    n = 1 + 2 * levels
+    rng = np.random.default_rng(15)
+    s = sampled(b, n, vocab, 15, certain=True)
+    s["counts"][:] = n
+    up = np.arange(n)
+    s["parents"][:] = np.where(up == 0, -1, 2 * ((up - 1) // 2))
+    s["tokens"][:, 0] = 0
+    for level in range(levels):
+        first, second = 1 + 2 * level, 2 + 2 * level
+        s["tokens"][:, first] = s["tokens"][:, first - 1]
+        s["tokens"][:, second] = (s["tokens"][:, first] + 1 + rng.integers(0, vocab - 1, b)) % vocab
+        s["accept_u"][:, first], s["accept_u"][:, second] = 1 - 2.0 ** -24, 0
+    want = check_verify(spec, s)
+    assert (want[1] == levels).all()
+    g = on_gpu(s)
+    for _ in range(20):
+        assert all(np.array_equal(x, y.cpu().numpy()) for x, y in zip(want, spec.verify(**g)))
+    s["accept_u"][:] = (rng.integers(0, 1 << 24, (b, n)) / 2.0 ** 24).astype(np.float32) * np.float32(0.2)
+    check_verify(spec, s)
+
+
 def test_verify_edges(spec):
     n, vocab = 4, 700
     s = sampled(12, n, vocab, 9)
