@@ -979,7 +979,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
     __shared__ uint32_t tmem_base;
     __shared__ float2 sh_ml[2][2][128];  // by stream, half and row: maximum and sum
     __shared__ float sh_mx[2][2][128];
-    __shared__ int sh_bad[16];  // by item: a node's V holds NaN or infinities
+    __shared__ int sh_bad[17];  // a node's V holds NaN or infinities: by item, and (16) any so far in the odd tiles' ring
     const ds_cuda_tree_attention_t &d = a.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     sa_warm<HD>(a);
@@ -1001,7 +1001,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
         }
         mbar_fence_init();
     }
-    if (tid < 16) sh_bad[tid] = 0;
+    if (tid < 17) sh_bad[tid] = 0;
     if (warp == (TC_SOFTMAX + TC_PRODUCERS) / 32) tmem_alloc(&tmem_base, 512);
     SaCursor cu;
     int tiles;
@@ -1067,7 +1067,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                 // A node's V may hold NaN or infinities that some rows must not
                 // see, and 0 * NaN would spread through the product: they are
                 // zeroed here, and added to the results of the rows that attend
-                // them when those are written.
+                // them when those are written. (Every item has units in ring 0,
+                // which is thus fewer than 16 items ahead. Ring 1 of the odd
+                // tiles runs past any number of one-tile items: its flag stays
+                // set, and the later items' nodes are looked through.)
                 cp_commit();
                 cp_wait<0>();
                 // (an exponent of all ones carries into the bit above it)
@@ -1092,7 +1095,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
                         }
                         *v = u;
                     });
-                    *reinterpret_cast<volatile int *>(&sh_bad[item & 15]) = 1;
+                    *reinterpret_cast<volatile int *>(&sh_bad[S::DUAL || rg == 0 ? item & 15 : 16]) = 1;
                 }
                 fence_proxy_async();
                 mbar_arrive(&full[slot]);
@@ -1375,7 +1378,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) sa_many_kernel(const __grid_con
             if (ok) {
                 const bool alone = whole && end, none = !used || ll == 0.f;
                 const float inv = alone ? (none ? 0.f : 1.f / ll) : 1.f;
-                const bool bad = *reinterpret_cast<volatile int *>(&sh_bad[item & 15]) != 0;
+                const bool bad = (*reinterpret_cast<volatile int *>(&sh_bad[item & 15]) | (S::DUAL ? 0 : *reinterpret_cast<volatile int *>(&sh_bad[16]))) != 0;
                 const size_t slot = (size_t)blockIdx.x * 2 + whole;
                 const int r = (S::DUAL ? w * 128 : 0) + i;
 #pragma unroll 1

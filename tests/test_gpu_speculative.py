@@ -165,6 +165,27 @@ def test_attention_many_rows_nan_in_a_node(spec, kind, hd, group):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("n", [20, 140])
+def test_attention_infinite_node_after_idle_sequences(spec, kind, n):
+    # a sequence whose node holds an infinity (in its second or third tile of
+    # 64 keys) after hundreds without a tree, of one empty tile each
+    live = [i % 25 == 24 for i in range(1500)]
+    c = Case(kind, [30 if x else 0 for x in live], [n if x else 0 for x in live], n, 8, 1, 64, seed=19, garbage=False)
+    at = torch.tensor(live, device="cuda")
+    c.tv[at, :, n - 2] = float("inf")
+    c.allowed[:, :, n - 2] = False
+    c.allowed[live, n - 2, n - 2] = True
+    c.mask = R.words(c.allowed).cuda()
+    out = c.run(spec)
+    assert torch.isposinf(out[at, n - 2]).all()
+    out[at, n - 2] = 0
+    c.tv[at, :, n - 2] = 0  # (finite for the plain form; nobody else attends it)
+    o = c.want()[0]
+    o[at, n - 2] = 0
+    assert rel(out, o) < TOL[kind]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
 @pytest.mark.parametrize("group", [8, 40])
 def test_attention_many_rows_scores_far_apart(spec, kind, group):
     # the largest score of some rows arrives late and is far above the first
