@@ -31,6 +31,7 @@ constexpr int SA_MAX_NODES = 256;
 constexpr int SA_THREADS = 128;
 constexpr int SA_WARPS = SA_THREADS / 32;
 constexpr int SA_CLUSTER = 16;  // CTAs of a cluster, at most
+constexpr int SA_KT = 64;       // keys of a tile
 
 struct SaArgs {
     ds_cuda_tree_attention_t d;
@@ -413,7 +414,7 @@ __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor 
 template <int HD_, int NG_, int PL_, int QT_> struct SaFew {
     static constexpr int HD = HD_, NG = NG_, PL = PL_, QT = QT_;
     static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
-    static constexpr int RT = 8 * NG, KT = 64;
+    static constexpr int RT = 8 * NG, KT = SA_KT;
     static constexpr int PLANE = 16 * HD * 2, UNIT = PL * PLANE;  // of a warp
     static constexpr int SMEM = SA_WARPS * 3 * UNIT;
     static constexpr int PHASES = RT * HD * 4 > UNIT ? RT * HD * 4 / UNIT : 1;  // of a join through one unit a warp
@@ -858,7 +859,7 @@ template <int HD_, bool DUAL_, int QT_> struct SaMany {
     static constexpr int HD = HD_, QT = QT_, PL = 1;
     static constexpr bool DUAL = DUAL_;
     static constexpr int RT = DUAL ? 256 : 128;
-    static constexpr int KT = 64;
+    static constexpr int KT = SA_KT;
     static constexpr int SUB = KT * 128;           // 64 dimensions of a unit
     static constexpr int UNIT = KT * HD * 2;       // 16 KB, 8 KB for head_dim 64
     static constexpr int QSUB = 128 * 128, QBLOCK = QSUB * (HD / 64);
@@ -1614,12 +1615,12 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
 // clusters of 8 and 12.6 in the list).
 // (One stream, 10 heads, 662 tokens, F32 in two planes: one node takes 7.1 us
 // on the GPU against 7.9, and the call 7 us of the host's time instead of 13.)
-template <class S> static long long sa_tiles(const ds_cuda_tree_attention_t *d) {
-    return (d->kv_max + S::KT - 1) / S::KT + (d->n_nodes + S::KT - 1) / S::KT;
+static long long sa_most_tiles(const ds_cuda_tree_attention_t *d, int kt) {
+    return ((long long)d->kv_max + kt - 1) / kt + (d->n_nodes + kt - 1) / kt;
 }
-template <class S> static int sa_clusters(const ds_cuda_tree_attention_t *d, int items, int sms) {
+template <class S> static int sa_clusters(const ds_cuda_tree_attention_t *d, long long items, int sms) {
     for (int n = SA_CLUSTER; n >= (S::RT == 8 ? 8 : SA_CLUSTER); n /= 2)
-        if ((long long)items * n <= sms * S::PER_SM && sa_tiles<S>(d) <= 8 * n) return n;
+        if (items * n <= sms * S::PER_SM && sa_most_tiles(d, S::KT) <= 8 * n) return n;
     return 0;
 }
 
@@ -1653,7 +1654,7 @@ static bool sa_map(const ds_cuda_tree_attention_t &d, int kv, int kt, CUtensorMa
 }
 
 template <class S> struct SaRun {
-    static int clusters(const SaArgs &a) { return SaMade<S>::by_dimension ? 0 : sa_clusters<S>(&a.d, a.d.batch * a.per_seq, a.sms); }
+    static int clusters(const SaArgs &a) { return SaMade<S>::by_dimension ? 0 : sa_clusters<S>(&a.d, (long long)a.d.batch * a.per_seq, a.sms); }
     static size_t workspace(const SaArgs &a) {
         // two parts a CTA, then their maxima and sums
         return clusters(a) ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
@@ -1732,9 +1733,10 @@ template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t
     constexpr int P = DS_CUDA_SPEC_F32;
     const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
     using Few = SaFew<HD, 2, 1, DS_CUDA_SPEC_BF16>;
-    const bool brief = (double)d->batch * d->n_kv_heads * ((rows + 15) / 16) * sa_tiles<Few>(d) <= 8.0 * sms * Few::PER_SM;
+    const bool brief = (double)d->batch * d->n_kv_heads * ((rows + 15) / 16) * sa_most_tiles(d, SA_KT) <= 8.0 * sms * Few::PER_SM;
     using Eight = SaFew<HD, 1, 2, P>;
-    const bool apart = rows <= 8 || 2 * sa_clusters<Eight>(d, d->batch * d->n_kv_heads * ((rows + 7) / 8), sms) >= sa_tiles<Eight>(d);
+    const long long eights = (long long)d->batch * d->n_kv_heads * ((rows + 7) / 8);
+    const bool apart = rows <= 8 || 2 * sa_clusters<Eight>(d, eights, sms) >= sa_most_tiles(d, SA_KT);
     if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, apart, brief, f);
     if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, apart, brief, f);
     if (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo)
@@ -1791,13 +1793,13 @@ static int sa_check(ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
                         d->batch, d->n_nodes, d->n_heads, d->n_kv_heads, d->head_dim, d->kv_max, SA_MAX_NODES);
     if (d->batch > 65535 || d->n_heads > 65535)
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: batch and n_heads are at most 65535");
-    if ((double)d->batch * d->n_heads * d->n_nodes * (d->kv_max / 32.0 + 16) >= 2147483648.0)
-        return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: more than 2^31 tiles");
     return DS_CUDA_OK;
 }
 
-static SaArgs sa_args(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
-    SaArgs a = {};
+// The kernels' arguments but for what run() adds; `err` is told of a refusal.
+static int sa_args(const ds_cuda_ctx *c, ds_cuda_ctx *err, const ds_cuda_tree_attention_t *d, SaArgs &a) {
+    const int rc = sa_check(err, d);
+    if (rc < 0) return rc;
     a.d = *d;
     a.words = (d->n_nodes + 63) / 64;
     a.group = d->n_heads / d->n_kv_heads;
@@ -1805,21 +1807,26 @@ static SaArgs sa_args(const ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
     const int rt = sa_pick(d, c->sm_count, [](auto r) { return decltype(sa_shape(r))::RT; });
     a.row_tiles = (a.rows + rt - 1) / rt;
     a.per_seq = d->n_kv_heads * a.row_tiles;
+    // (the list's places are 32-bit; its lengths are known on the device alone)
+    const long long tiles = (long long)d->batch * a.per_seq * std::max(1ll, sa_most_tiles(d, SA_KT));
+    if (tiles > INT32_MAX)
+        return ctx_fail(err, DS_CUDA_EINVAL, "tree_attention: up to %lld tiles of %d keys and %d rows (< 2^31)", tiles, SA_KT, rt);
     a.sms = c->sm_count;
     a.err = c->d_spec_err;
     a.scale2 = d->scale * 1.44269504f;
-    return a;
+    return DS_CUDA_OK;
 }
 
 extern "C" size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d) {
-    if (!c || !c->ok || sa_check(nullptr, d) < 0) return 0;
-    const SaArgs a = sa_args(c, d);
+    SaArgs a = {};
+    if (!c || !c->ok || sa_args(c, nullptr, d, a) < 0) return 0;
     return sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::workspace(a); });
 }
 
 extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d, void *stream) {
     if (!c || !c->ok) return DS_CUDA_EINVAL;
-    int rc = sa_check(c, d);
+    SaArgs a = {};
+    const int rc = sa_args(c, c, d, a);
     if (rc < 0 || d->batch == 0) return rc;
     if (!d->q || !d->out || !d->lens || !d->mask || !d->tree_k || !d->tree_v || (d->kv_max > 0 && (!d->k || !d->v)))
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: null pointer");
@@ -1841,7 +1848,6 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
         if (t.lo && d->type != DS_CUDA_SPEC_F32)
             return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: %s has a lo plane, which only the F32 type takes", t.name);
     }
-    const SaArgs a = sa_args(c, d);
     const size_t need = sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::workspace(a); });
     if (need && (!d->workspace || d->workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->workspace) & 255)))
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: workspace of %zu bytes, 256-byte aligned, wanted", need);

@@ -343,6 +343,26 @@ def test_attention_offsets_past_32_bits(spec):
     c.check(spec)
 
 
+def test_attention_of_many_sequences_with_room(spec):
+    # 256 sequences, 64 heads on 8, trees of 64, room for 65536 rows (one
+    # cache for all): as four calls of 64 sequences give it
+    g = torch.Generator("cuda").manual_seed(23)
+    b, n, kv, hd, cap = 256, 64, 8, 64, 65536
+
+    def rnd(*s):
+        return torch.randn(s, generator=g, device="cuda", dtype=torch.bfloat16)
+
+    q, k, v, tk, tv = rnd(b, n, 64, hd), rnd(1, kv, cap, hd), rnd(1, kv, cap, hd), rnd(b, kv, n, hd), rnd(b, kv, n, hd)
+    lens = torch.randint(0, 300, (b,), generator=g, device="cuda").int()
+    lens[77] = cap
+    mask = torch.randint(-2 ** 63, 2 ** 63 - 1, (b, n, 1), generator=g, device="cuda")
+    parts = [x.split(64) for x in (q, tk, tv, lens, mask)]
+    want = torch.cat([spec.tree_attention(x, k.expand(64, -1, -1, -1), v.expand(64, -1, -1, -1), *r) for x, *r in zip(*parts)])
+    got = spec.tree_attention(q, k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1), tk, tv, lens, mask)
+    # (other cuts: each side within the tolerance of the exact one)
+    assert torch.isfinite(got).all() and rel(got, want) < 2 * TOL["bf16"]
+
+
 def test_attention_is_repeatable_on_streams_and_in_graphs(spec):
     cs = [Case("pair", [900, 40], [16, 9], 16, 4, 1, 128, seed=s) for s in (15, 16)]
     want = [c.run(spec) for c in cs]

@@ -1,0 +1,91 @@
+"""The host side of the speculative-decoding entry points, without a GPU: the
+library's own objects over a CUDA runtime of counters (fake_cuda.cu)."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from ds_ocr_b200 import build, speculative as S
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+class State(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("devices", ctypes.c_int), ("launches", ctypes.c_int),
+                ("launch_device", ctypes.c_int), ("word", ctypes.c_uint), ("error", ctypes.c_int)]
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    objs = [os.path.join(build.BUILD, f + ".cu.o") for f in ("spec_attn", "spec_verify")]
+    if not all(map(os.path.exists, objs)):
+        build.build()
+    tmp = tmp_path_factory.mktemp("fake")
+    obj, so = str(tmp / "fake.o"), str(tmp / "fake.so")
+    subprocess.check_call([build._nvcc(), *build.NVCC_FLAGS, "-I", build.CSRC, "-I", os.path.join(build.ROOT, "include"),
+                           "-c", os.path.join(HERE, "fake_cuda.cu"), "-o", obj])
+    # (-Bsymbolic: its own runtime, whatever else the process has loaded)
+    subprocess.check_call(["g++", "-shared", "-Wl,-Bsymbolic", "-Wl,-z,defs", "-o", so, obj, *objs])
+    lib = ctypes.CDLL(so)
+    P, I = ctypes.c_void_p, ctypes.c_int
+    for name, res, args in (("fake_new", P, [I, I]), ("fake_free", None, [P]), ("fake_state", ctypes.POINTER(State), []),
+                            ("fake_message", ctypes.c_char_p, [P])):
+        f = getattr(lib, name)
+        f.restype, f.argtypes = res, args
+    from ds_ocr_b200 import _lib
+    for name, (res, args) in _lib.SIGNATURES.items():
+        if name.startswith(("ds_cuda_tree", "ds_cuda_token")):
+            f = getattr(lib, name)
+            f.restype, f.argtypes = res, args
+    return lib
+
+
+@pytest.fixture
+def ctx(lib):
+    h = lib.fake_new(1, 148)
+    yield h
+    lib.fake_free(h)
+
+
+def attention(type=S.BF16, batch=2, n_nodes=4, n_heads=4, n_kv_heads=2, head_dim=64, kv_max=128):
+    """A descriptor with addresses that nothing reads."""
+    d = S.TreeAttentionDesc(type=type, batch=batch, n_nodes=n_nodes, n_heads=n_heads, n_kv_heads=n_kv_heads,
+                            head_dim=head_dim, kv_max=kv_max, scale=0.125)
+    for i, name in enumerate(("q", "k", "v", "tree_k", "tree_v", "lens", "mask", "out")):
+        setattr(d, name, 4096 * (i + 1))
+    for name, rows in (("k", kv_max), ("v", kv_max), ("tree_k", n_nodes), ("tree_v", n_nodes)):
+        setattr(d, name + "_stride", (ctypes.c_int64 * 3)(n_kv_heads * rows * head_dim, rows * head_dim, head_dim))
+    for name in ("q", "out"):
+        setattr(d, name + "_stride", (ctypes.c_int64 * 3)(n_nodes * n_heads * head_dim, n_heads * head_dim, head_dim))
+    return d
+
+
+def attend(lib, ctx, d):
+    d.workspace_bytes = lib.ds_cuda_tree_attention_workspace(ctx, ctypes.byref(d))
+    d.workspace = 1 << 20
+    return lib.ds_cuda_tree_attention_dev(ctx, ctypes.byref(d), None)
+
+
+@pytest.mark.parametrize("sizes", [
+    # 256 sequences with room for 65536 rows, 64 heads on 8, trees of 64: 8.4 million tiles
+    dict(batch=256, n_nodes=64, n_heads=64, n_kv_heads=8, kv_max=65536),
+    # one sequence of 2^28 tiles, and many of 16392 each
+    dict(batch=1, n_nodes=256, n_heads=64, n_kv_heads=64, kv_max=1 << 24, type=S.F32),
+    dict(batch=65535, n_nodes=1, n_heads=8, n_kv_heads=8, kv_max=131072),
+])
+def test_attention_takes_any_list_of_tiles_below_2_to_31(lib, ctx, sizes):
+    d = attention(**sizes)
+    assert attend(lib, ctx, d) == 0, lib.fake_message(ctx)
+    assert d.workspace_bytes > 0 and lib.fake_state().contents.launches == 2
+
+
+@pytest.mark.parametrize("sizes", [
+    dict(batch=65535, n_nodes=256, n_heads=65535, n_kv_heads=65535, kv_max=1024),
+    dict(batch=65535, n_nodes=1, n_heads=64, n_kv_heads=64, kv_max=131072),
+    dict(batch=60000, n_nodes=256, n_heads=65000, n_kv_heads=1, kv_max=0),
+])
+def test_attention_refuses_more_tiles(lib, ctx, sizes):
+    d = attention(**sizes)
+    assert attend(lib, ctx, d) < 0 and b"tiles" in lib.fake_message(ctx)
+    assert d.workspace_bytes == 0 and lib.fake_state().contents.launches == 0
