@@ -62,6 +62,23 @@ struct ds_cuda_ctx {
     std::vector<std::pair<void *, size_t>> key_ranges;
 };
 
+// The context's device is the thread's current one while this lives; then the
+// caller's is again (its framework may allocate on whatever is current).
+class CtxDevice {
+    int was = -1;
+
+  public:
+    explicit CtxDevice(const ds_cuda_ctx *c) {
+        if (cudaGetDevice(&was) != cudaSuccess || was == c->device) was = -1;
+        cudaSetDevice(c->device);
+    }
+    ~CtxDevice() {
+        if (was >= 0) cudaSetDevice(was);
+    }
+    CtxDevice(const CtxDevice &) = delete;
+    CtxDevice &operator=(const CtxDevice &) = delete;
+};
+
 int ctx_fail(ds_cuda_ctx *c, int code, const char *fmt, ...);
 int ctx_cuda(ds_cuda_ctx *c, cudaError_t e, const char *what);
 int ctx_grow(ds_cuda_ctx *c, void **p, size_t *cap, size_t need);

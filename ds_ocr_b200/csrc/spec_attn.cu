@@ -1851,7 +1851,7 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
     const size_t need = sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::workspace(a); });
     if (need && (!d->workspace || d->workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->workspace) & 255)))
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: workspace of %zu bytes, 256-byte aligned, wanted", need);
-    cudaSetDevice(c->device);
+    const CtxDevice on(c);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     const cudaError_t e = sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::run(a, c->device, st); });
     if (e != cudaSuccess) cudaGetLastError();  // reported here, not by whoever asks next
@@ -1860,7 +1860,7 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
 
 extern "C" int ds_cuda_tree_attention_check(ds_cuda_ctx_t *c, void *stream) {
     if (!c || !c->ok) return DS_CUDA_EINVAL;
-    cudaSetDevice(c->device);
+    const CtxDevice on(c);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     unsigned err = 0;
     cudaError_t e = cudaMemcpyAsync(&err, c->d_spec_err, sizeof err, cudaMemcpyDeviceToHost, st);
@@ -1878,7 +1878,7 @@ extern "C" int ds_cuda_tree_mask_dev(ds_cuda_ctx_t *c, const int *parents, const
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_mask: batch=%d n_nodes=%d (<= %d)", batch, n_nodes, SA_MAX_NODES);
     if (batch == 0) return DS_CUDA_OK;  // an empty tensor has no address
     if (!parents || !mask) return ctx_fail(c, DS_CUDA_EINVAL, "tree_mask: null pointer");
-    cudaSetDevice(c->device);
+    const CtxDevice on(c);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
     tree_mask_kernel<<<batch, (n_nodes + 31) & ~31, 0, st>>>(parents, nodes, n_nodes, (n_nodes + 63) / 64, mask, depth);
     return ctx_cuda(c, cudaGetLastError(), "tree_mask launch");

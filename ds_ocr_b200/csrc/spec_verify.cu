@@ -462,10 +462,7 @@ __global__ void __launch_bounds__(CM_THREADS) tree_commit_kernel(const __grid_co
 
 using namespace ds;
 
-static cudaStream_t sv_stream(ds_cuda_ctx *c, void *s) {
-    cudaSetDevice(c->device);
-    return s ? (cudaStream_t)s : c->stream;
-}
+static cudaStream_t sv_stream(const ds_cuda_ctx *c, void *s) { return s ? (cudaStream_t)s : c->stream; }
 
 static cudaError_t launch_cluster(const void *f, long long ctas, int threads, size_t smem, int ncta, cudaStream_t st,
                                   void **args) {
@@ -493,6 +490,7 @@ extern "C" int ds_cuda_tree_verify_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_veri
     if (d->batch == 0) return DS_CUDA_OK;  // an empty tensor has no address
     if (!d->tokens || !d->parents || !d->target || !d->accept_u || !d->sample_u || !d->path || !d->accepted || !d->token)
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_verify: null pointer");
+    const CtxDevice on(c);
     cudaStream_t st = sv_stream(c, stream);
     // enough CTAs for the row to fit the registers; more where the batch
     // leaves SMs idle, which shortens a row's pass
@@ -517,6 +515,7 @@ extern "C" int ds_cuda_tree_verify_greedy_dev(ds_cuda_ctx_t *c, const int *token
     if (batch == 0) return DS_CUDA_OK;  // an empty tensor has no address
     if (!tokens || !parents || !target_tokens || !path || !accepted || !token)
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_verify_greedy: null pointer");
+    const CtxDevice on(c);
     cudaStream_t st = sv_stream(c, stream);
     tree_verify_greedy_kernel<<<batch, 32, 0, st>>>(tokens, parents, nodes, target_tokens, n_nodes, path, accepted, token);
     return ctx_cuda(c, cudaGetLastError(), "tree_verify_greedy launch");
@@ -529,6 +528,7 @@ extern "C" int ds_cuda_token_probs_dev(ds_cuda_ctx_t *c, int type, const void *l
         return ctx_fail(c, DS_CUDA_EINVAL, "token_probs: type=%d rows=%d vocab=%d", type, rows, vocab);
     if (rows == 0) return DS_CUDA_OK;  // an empty tensor has no address
     if (!logits || !probs) return ctx_fail(c, DS_CUDA_EINVAL, "token_probs: null pointer");
+    const CtxDevice on(c);
     cudaStream_t st = sv_stream(c, stream);
     if (vocab > TP_CLUSTER * TP_MOST)
         return ctx_fail(c, DS_CUDA_EINVAL, "token_probs: vocab %d (<= %d)", vocab, TP_CLUSTER * TP_MOST);
@@ -574,6 +574,7 @@ extern "C" int ds_cuda_tree_commit_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_comm
         if (!d->cache[t] || !d->tree[t] || bits % 16)
             return ctx_fail(c, DS_CUDA_EINVAL, "tree_commit: tensor %d: null, or base or strides not multiples of 16 bytes", t);
     }
+    const CtxDevice on(c);
     cudaStream_t st = sv_stream(c, stream);
     // as many rows as could be accepted; about eight CTAs an SM
     const int work = (d->n_kv_heads * d->n_nodes * (d->head_dim / 8) + 4 * CM_THREADS - 1) / (4 * CM_THREADS);

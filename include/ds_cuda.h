@@ -548,7 +548,8 @@ int ds_cuda_prefill_stage_ms(ds_cuda_ctx_t *ctx, float *ms);
  * `stream` (NULL = the context's stream; a caller on the legacy default
  * stream passes cudaStreamLegacy) and nothing is allocated, synchronised or
  * kept between calls, so calls on several streams may overlap and may be
- * captured in a CUDA graph. Limits: n_nodes <= 256.
+ * captured in a CUDA graph. The calling thread's current device is the same
+ * after a call as before. Limits: n_nodes <= 256.
  * --------------------------------------------------------------------- */
 #define DS_CUDA_SPEC_BF16 0 /* BF16 */
 #define DS_CUDA_SPEC_F16 1  /* FP16 */

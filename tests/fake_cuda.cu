@@ -17,6 +17,7 @@ struct Fake {
     int error;            // what the next launch answers
 };
 static Fake fake;
+static cudaError_t last;
 
 extern "C" {
 ds_cuda_ctx *fake_new(int device, int sms) {
@@ -40,7 +41,7 @@ static cudaError_t launched() {
     fake.launch_device = fake.device;
     const cudaError_t e = (cudaError_t)fake.error;
     fake.error = 0;
-    return e;
+    return last = e;
 }
 #ifndef __CUDA_ARCH__
 cudaError_t cudaGetDevice(int *d) { return *d = fake.device, cudaSuccess; }
@@ -48,7 +49,10 @@ cudaError_t cudaSetDevice(int d) {
     if (d < 0 || d >= fake.devices) return cudaErrorInvalidDevice;
     return fake.device = d, cudaSuccess;
 }
-cudaError_t cudaGetLastError() { return cudaSuccess; }
+cudaError_t cudaGetLastError() {
+    const cudaError_t e = last;
+    return last = cudaSuccess, e;
+}
 cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int) { return cudaSuccess; }
 cudaError_t cudaLaunchKernel(const void *, dim3, dim3, void **, size_t, cudaStream_t) { return launched(); }
 cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t *, const void *, void **) { return launched(); }

@@ -89,3 +89,41 @@ def test_attention_refuses_more_tiles(lib, ctx, sizes):
     d = attention(**sizes)
     assert attend(lib, ctx, d) < 0 and b"tiles" in lib.fake_message(ctx)
     assert d.workspace_bytes == 0 and lib.fake_state().contents.launches == 0
+
+
+def calls(lib, h):
+    """name -> a call that launches."""
+    a, v, c = attention(), S.TreeVerifyDesc(batch=2, n_nodes=3, vocab=100), S.TreeCommitDesc(
+        n_tensors=1, layers=1, batch=2, n_nodes=3, n_kv_heads=1, head_dim=8, kv_max=9, lens=64, path=128, accepted=192, new_lens=256)
+    for name in ("tokens", "parents", "target", "accept_u", "sample_u", "path", "accepted", "token"):
+        setattr(v, name, 4096)
+    c.cache[0] = c.tree[0] = 4096
+    for t in (c.cache_stride[0], c.tree_stride[0]):
+        t[:] = [256, 128, 64, 8]
+    ref = ctypes.byref
+    return {
+        "attention": lambda: attend(lib, h, a),
+        "mask": lambda: lib.ds_cuda_tree_mask_dev(h, 64, None, 2, 3, 64, None, None),
+        "probs": lambda: lib.ds_cuda_token_probs_dev(h, S.F32, 4096, 2, 100, 100, None, 4096, None),
+        "verify": lambda: lib.ds_cuda_tree_verify_dev(h, ref(v), None),
+        "greedy": lambda: lib.ds_cuda_tree_verify_greedy_dev(h, 64, 64, None, 64, 2, 3, 64, 64, 64, None),
+        "commit": lambda: lib.ds_cuda_tree_commit_dev(h, ref(c), None),
+    }
+
+
+@pytest.mark.parametrize("name", ["attention", "mask", "probs", "verify", "greedy", "commit"])
+@pytest.mark.parametrize("current", [0, 1, 3])
+def test_a_call_leaves_the_current_device(lib, ctx, name, current):
+    f = lib.fake_state().contents
+    call = calls(lib, ctx)[name]
+    f.device = current
+    assert call() == 0, lib.fake_message(ctx)
+    assert f.launches >= 1 and f.launch_device == 1 and f.device == current
+    f.error = 700  # a launch that fails
+    assert call() < 0 and f.device == current
+
+
+def test_the_check_leaves_the_current_device(lib, ctx):
+    f = lib.fake_state().contents
+    f.device = 3
+    assert lib.ds_cuda_tree_attention_check(ctx, None) == 0 and f.device == 3
