@@ -44,7 +44,8 @@ struct ds_cuda_ctx {
     // multi-stream GEMM standalone entry: planes + tile list
     void *d_sk_scratch = nullptr;
     size_t sk_scratch_cap = 0;
-    unsigned *d_spec_err = nullptr;         // tree attention: a bounded wait gave up
+    unsigned *d_spec_err = nullptr;         // tree attention: bounded waits that gave up, and
+    std::map<cudaStream_t, unsigned> spec_err_seen;  // how many a stream's check has reported
     // pinned staging
     void *pin = nullptr;
     size_t pin_cap = 0;

@@ -42,7 +42,7 @@ struct SaArgs {
     int per_seq;    // n_kv_heads * row_tiles: items of a sequence
     int sms, ctas;  // SMs; runs the tile list is cut into, at most
     float scale2;   // scale * log2(e)
-    unsigned *err;  // set where a bounded wait gave up
+    unsigned *err;  // bounded waits that gave up
     float *part;    // workspace: [ctas][2][row tile][head_dim], then ...
     float2 *ml;     // ... [ctas][2][row tile] (max in log2 units, sum)
 };
@@ -894,7 +894,7 @@ __device__ __forceinline__ bool tc_wait(uint64_t *bar, uint32_t parity, unsigned
         for (int i = 0; i < 64; i++)
             if (mbar_try_wait(bar, parity)) return true;
     } while (ds_gtime() - t0 < 2000000000ull);
-    if (err) atomicExch(err, 1u);
+    if (err) atomicAdd(err, 1u);
     return false;
 }
 __device__ __forceinline__ bool elect_one() {
@@ -1866,8 +1866,10 @@ extern "C" int ds_cuda_tree_attention_check(ds_cuda_ctx_t *c, void *stream) {
     cudaError_t e = cudaMemcpyAsync(&err, c->d_spec_err, sizeof err, cudaMemcpyDeviceToHost, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return ctx_cuda(c, e, "tree_attention_check");
-    if (!err) return DS_CUDA_OK;
-    cudaMemsetAsync(c->d_spec_err, 0, sizeof err, st);
+    // the count is never reset, or another stream's check would not see it
+    const auto seen = c->spec_err_seen.find(st);
+    if (err == (seen == c->spec_err_seen.end() ? 0 : seen->second)) return DS_CUDA_OK;
+    c->spec_err_seen[st] = err;
     return ctx_fail(c, DS_CUDA_ETIMEOUT, "tree_attention: a bounded wait gave up");
 }
 

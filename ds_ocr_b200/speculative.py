@@ -89,7 +89,7 @@ class Speculative:
 
     def check(self):
         """Synchronise the current stream and raise if a tree attention
-        kernel's bounded wait gave up since the last check."""
+        kernel's bounded wait gave up since this stream's last check."""
         import torch
         st = torch.cuda.current_stream(self.device).cuda_stream or 1  # cudaStreamLegacy
         self.ctx.check(self.ctx.lib.ds_cuda_tree_attention_check(self.ctx.h, st), "tree_attention")

@@ -592,9 +592,10 @@ typedef struct {
  * sizes are refused); of the pointers only the lo planes' presence matters. */
 size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *ctx, const ds_cuda_tree_attention_t *d);
 int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *ctx, const ds_cuda_tree_attention_t *d, void *stream);
-/* Synchronises `stream` and reports DS_CUDA_ETIMEOUT if a tree attention
- * kernel's bounded wait gave up since the last check (its results are then
- * incomplete). */
+/* Synchronises `stream` and reports DS_CUDA_ETIMEOUT if a bounded wait of a
+ * tree attention call gave up (its results are then incomplete), on this
+ * stream since its last check or on any other of the context's by now: each
+ * stream's check reports it once. */
 int ds_cuda_tree_attention_check(ds_cuda_ctx_t *ctx, void *stream);
 
 /* Mask words and depths (root 0) of trees given by parents

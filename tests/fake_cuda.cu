@@ -62,7 +62,6 @@ cudaError_t cudaGetDriverEntryPoint(const char *, void **, unsigned long long, c
 cudaError_t cudaMemcpyAsync(void *dst, const void *, size_t n, cudaMemcpyKind, cudaStream_t) {
     return memcpy(dst, &fake.word, n < sizeof fake.word ? n : sizeof fake.word), cudaSuccess;
 }
-cudaError_t cudaMemsetAsync(void *, int, size_t, cudaStream_t) { return fake.word = 0, cudaSuccess; }
 cudaError_t cudaStreamSynchronize(cudaStream_t) { return cudaSuccess; }
 unsigned __cudaPushCallConfiguration(dim3, dim3, size_t, CUstream_st *) { return 0; }
 cudaError_t __cudaPopCallConfiguration(dim3 *, dim3 *, size_t *, void *) { return cudaSuccess; }

@@ -127,3 +127,16 @@ def test_the_check_leaves_the_current_device(lib, ctx):
     f = lib.fake_state().contents
     f.device = 3
     assert lib.ds_cuda_tree_attention_check(ctx, None) == 0 and f.device == 3
+
+
+def test_every_stream_hears_of_a_wait_that_gave_up(lib, ctx):
+    f = lib.fake_state().contents
+    a, b = 0x1000, 0x2000
+    check = lib.ds_cuda_tree_attention_check
+    assert check(ctx, a) == 0 and check(ctx, b) == 0
+    f.word = 3  # what a kernel on either stream, or on a third, leaves
+    for s in (a, b, None):
+        assert check(ctx, s) == -7 and b"wait" in lib.fake_message(ctx)
+        assert check(ctx, s) == 0
+    f.word += 1
+    assert [check(ctx, s) for s in (b, b, a, a)] == [-7, 0, -7, 0]
