@@ -86,7 +86,8 @@ def build(verbose=False, force=False):
 
 
 def build_spec(verbose=False, force=False):
-    """The torch module _spec.so, linked to libds_cuda.so beside it."""
+    """The torch module _spec.so (it is given the C ABI's addresses, not linked
+    to the library: DS_CUDA_LIB may name another one)."""
     try:
         import torch
     except ImportError:
@@ -101,9 +102,8 @@ def build_spec(verbose=False, force=False):
            "-I", os.path.join(ROOT, "include"), "-isystem", sysconfig.get_paths()["include"],
            "-isystem", os.path.join(base, "include"),
            "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"), "-isystem", cuda,
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-L", HERE, "-l:libds_cuda.so",
-           "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
-           "-Wl,-rpath,$ORIGIN"]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-L", os.path.join(base, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     if verbose:
         print(" ".join(cmd))
     subprocess.check_call(cmd)

@@ -29,6 +29,18 @@ struct Raised {};  // a Python error is already set
 
 PyObject *g_error = nullptr;  // DsCudaError
 
+// The C ABI's entry points, of the library that the contexts come from (this
+// module is not linked to one: there may be several).
+#define ENTRIES(X)                                                                                                      \
+    X(last_error) X(tree_attention_workspace) X(tree_attention_dev) X(tree_mask_dev) X(token_probs_dev) X(tree_verify_dev) \
+        X(tree_verify_greedy_dev) X(tree_commit_dev)
+#define X(f) decltype(&ds_cuda_##f) f;
+struct {
+    bool bound;
+    ENTRIES(X)
+} abi;
+#undef X
+
 std::string text(c10::IntArrayRef s) {
     std::string r = "(";
     for (size_t i = 0; i < s.size(); i++) r += (i ? ", " : "") + std::to_string(s[i]);
@@ -41,6 +53,7 @@ struct Call {
     c10::TensorOptions options;
 
     Call(PyObject *const *args, Py_ssize_t n, Py_ssize_t want) {
+        if (!abi.bound) throw Failed("the module is not bound to the library");
         if (n != want) throw Bad("expected " + std::to_string(want) + " arguments");
         ctx = static_cast<ds_cuda_ctx_t *>(PyLong_AsVoidPtr(args[0]));
         device = static_cast<c10::DeviceIndex>(PyLong_AsLong(args[1]));
@@ -54,7 +67,7 @@ struct Call {
         return s ? s : cudaStreamLegacy;
     }
     void check(int rc, const char *what) const {
-        if (rc < 0) throw Failed(std::string(what) + " failed (" + std::to_string(rc) + "): " + ds_cuda_last_error(ctx));
+        if (rc < 0) throw Failed(std::string(what) + " failed (" + std::to_string(rc) + "): " + abi.last_error(ctx));
     }
 
     const at::Tensor &tensor(const char *name, PyObject *o) const {
@@ -153,12 +166,12 @@ PyObject *tree_attention(PyObject *const *x, Py_ssize_t n_args) {
     d.out = out.data_ptr();
     c.strides(out, d.out_stride, 3);
     at::Tensor ws;
-    d.workspace_bytes = ds_cuda_tree_attention_workspace(c.ctx, &d);
+    d.workspace_bytes = abi.tree_attention_workspace(c.ctx, &d);
     if (d.workspace_bytes) {
         ws = at::empty({(int64_t)d.workspace_bytes}, c.options.dtype(at::kByte));
         d.workspace = ws.data_ptr();
     }
-    c.check(ds_cuda_tree_attention_dev(c.ctx, &d, c.stream()), "tree_attention");
+    c.check(abi.tree_attention_dev(c.ctx, &d, c.stream()), "tree_attention");
     return THPVariable_Wrap(out);
 }
 
@@ -169,7 +182,7 @@ PyObject *tree_mask(PyObject *const *x, Py_ssize_t n_args) {
     const int64_t b = p.size(0), n = p.size(1);
     const int *parents = c.ptr<int>("parents", x[2], {b, n}, at::kInt), *nodes = c.maybe<int>("counts", x[3], {b}, at::kInt);
     const at::Tensor mask = at::empty({b, n, (n + 63) / 64}, c.options.dtype(at::kLong)), depth = at::empty({b, n}, c.options.dtype(at::kInt));
-    c.check(ds_cuda_tree_mask_dev(c.ctx, parents, nodes, (int)b, (int)n, static_cast<uint64_t *>(mask.data_ptr()),
+    c.check(abi.tree_mask_dev(c.ctx, parents, nodes, (int)b, (int)n, static_cast<uint64_t *>(mask.data_ptr()),
                                   static_cast<int *>(depth.data_ptr()), c.stream()), "tree_mask");
     return Py_BuildValue("(NN)", THPVariable_Wrap(mask), THPVariable_Wrap(depth));
 }
@@ -183,7 +196,7 @@ PyObject *token_probs(PyObject *const *x, Py_ssize_t n_args) {
     c.strided("logits", x[2], shape, l.scalar_type());
     const float *temp = c.maybe<float>("temperature", x[3], {shape[0]}, at::kFloat);
     const at::Tensor out = x[4] == Py_None ? at::empty(shape, c.options.dtype(at::kFloat)) : c.whole("out", x[4], shape, at::kFloat);
-    c.check(ds_cuda_token_probs_dev(c.ctx, type, l.data_ptr(), (int)shape[0], (int)shape[1], l.stride(0), temp,
+    c.check(abi.token_probs_dev(c.ctx, type, l.data_ptr(), (int)shape[0], (int)shape[1], l.stride(0), temp,
                                     static_cast<float *>(out.data_ptr()), c.stream()), "token_probs");
     return THPVariable_Wrap(out);
 }
@@ -220,7 +233,7 @@ PyObject *verify(PyObject *const *x, Py_ssize_t n_args) {
     d.nodes = c.maybe<int>("counts", x[8], {b}, at::kInt);
     const Results r(c, b, n);
     d.path = r.p(r.path), d.accepted = r.p(r.accepted), d.token = r.p(r.token);
-    c.check(ds_cuda_tree_verify_dev(c.ctx, &d, c.stream()), "tree_verify");
+    c.check(abi.tree_verify_dev(c.ctx, &d, c.stream()), "tree_verify");
     return r.wrap();
 }
 
@@ -232,7 +245,7 @@ PyObject *verify_greedy(PyObject *const *x, Py_ssize_t n_args) {
     const int *tokens = c.ptr<int>("tokens", x[2], {b, n}, at::kInt), *parents = c.ptr<int>("parents", x[3], {b, n}, at::kInt);
     const int *want = c.ptr<int>("target_tokens", x[4], {b, n}, at::kInt), *nodes = c.maybe<int>("counts", x[5], {b}, at::kInt);
     const Results r(c, b, n);
-    c.check(ds_cuda_tree_verify_greedy_dev(c.ctx, tokens, parents, nodes, want, (int)b, (int)n, r.p(r.path), r.p(r.accepted),
+    c.check(abi.tree_verify_greedy_dev(c.ctx, tokens, parents, nodes, want, (int)b, (int)n, r.p(r.path), r.p(r.accepted),
                                            r.p(r.token), c.stream()), "tree_verify_greedy");
     return r.wrap();
 }
@@ -266,7 +279,7 @@ PyObject *commit(PyObject *const *x, Py_ssize_t n_args) {
     d.accepted = c.ptr<int>("accepted", x[6], {b}, at::kInt);
     const at::Tensor lens = at::empty({b}, c.options.dtype(at::kInt));
     d.new_lens = static_cast<int *>(lens.data_ptr());
-    c.check(ds_cuda_tree_commit_dev(c.ctx, &d, c.stream()), "tree_commit");
+    c.check(abi.tree_commit_dev(c.ctx, &d, c.stream()), "tree_commit");
     return THPVariable_Wrap(lens);
 }
 
@@ -284,6 +297,23 @@ template <PyObject *(*F)(PyObject *const *, Py_ssize_t)> PyObject *guarded(PyObj
     return nullptr;
 }
 
+// bind({"ds_cuda_...": address}): every entry of the list, or KeyError.
+PyObject *bind(PyObject *, PyObject *table) {
+    abi.bound = false;
+    auto find = [&](const char *name) {
+        PyObject *p = PyMapping_GetItemString(table, name);
+        void *at = p ? PyLong_AsVoidPtr(p) : nullptr;
+        Py_XDECREF(p);
+        return at;
+    };
+#define X(f) \
+    if (!(abi.f = reinterpret_cast<decltype(abi.f)>(find("ds_cuda_" #f)))) return nullptr;
+    ENTRIES(X)
+#undef X
+    abi.bound = true;
+    Py_RETURN_NONE;
+}
+
 PyObject *set_error(PyObject *, PyObject *type) {
     Py_INCREF(type);
     Py_XDECREF(g_error);
@@ -293,7 +323,7 @@ PyObject *set_error(PyObject *, PyObject *type) {
 
 #define ENTRY(f) {#f, (PyCFunction)(void (*)(void))guarded<f>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(tree_attention), ENTRY(tree_mask), ENTRY(token_probs), ENTRY(verify), ENTRY(verify_greedy),
-                         ENTRY(commit), {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(commit), {"bind", bind, METH_O, nullptr}, {"set_error", set_error, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_spec", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -21,7 +21,7 @@ synchronises and nothing is kept between calls.
 """
 import ctypes
 
-from ._lib import DsCudaError
+from ._lib import SIGNATURES, DsCudaError, load
 from .cuda import Context
 
 BF16, F16, F32 = 0, 1, 2
@@ -127,7 +127,8 @@ class Speculative:
 
 
 def _module():
-    """ds_ocr_b200._spec, built first if only the sources are present."""
+    """ds_ocr_b200._spec, built first if only the sources are present, on the
+    entry points of the library that the contexts come from."""
     import torch  # noqa: F401  (its libraries have to be loaded)
     try:
         from . import _spec
@@ -135,5 +136,7 @@ def _module():
         from . import build
         build.build_spec()
         from . import _spec
+    lib = load()
+    _spec.bind({name: ctypes.cast(getattr(lib, name), _ptr).value for name in SIGNATURES})
     _spec.set_error(DsCudaError)
     return _spec
