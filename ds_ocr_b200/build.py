@@ -16,6 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libds_cuda.so")
 SPEC = os.path.join(HERE, "_spec.so")
 BUILD = os.path.join(ROOT, "_build")
+SPEC_FOR = os.path.join(BUILD, "_spec.for")  # the torch and Python that SPEC was built for
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -88,6 +89,32 @@ def build(verbose=False, force=False):
     return LIB
 
 
+def _read(path):
+    try:
+        with open(path) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def _write(path, text):
+    os.makedirs(os.path.dirname(path), exist_ok=True)
+    with open(path, "w") as f:
+        f.write(text)
+
+
+def _spec_abi():
+    """What the torch module depends on beside its sources."""
+    import sysconfig
+    import torch
+    return f"torch {torch.__version__} cuda {torch.version.cuda} {sysconfig.get_config_var('SOABI')}"
+
+
+def spec_is_for_another():
+    """Whether the torch module was built for another torch or Python."""
+    return _read(SPEC_FOR) not in (None, _spec_abi())
+
+
 def build_spec(verbose=False, force=False):
     """The torch module _spec.so (it is given the C ABI's addresses, not linked
     to the library: DS_CUDA_LIB may name another one)."""
@@ -99,7 +126,7 @@ def build_spec(verbose=False, force=False):
         return None
     import sysconfig
     src = os.path.join(CSRC, "spec_torch.cpp")
-    if not (force or _stale(SPEC, [src, os.path.join(ROOT, "include", "ds_cuda.h")])):
+    if not (force or _read(SPEC_FOR) != _spec_abi() or _stale(SPEC, [src, os.path.join(ROOT, "include", "ds_cuda.h")])):
         return SPEC
     base = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())) or "/usr/local/cuda", "include")
@@ -114,6 +141,7 @@ def build_spec(verbose=False, force=False):
     if os.path.exists(SPEC):  # (an old one with other structs must not stay where this fails)
         os.remove(SPEC)
     subprocess.check_call(cmd)
+    _write(SPEC_FOR, _spec_abi())
     return SPEC
 
 

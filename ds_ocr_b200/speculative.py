@@ -127,14 +127,20 @@ class Speculative:
 
 
 def _module():
-    """ds_ocr_b200._spec, built first if only the sources are present, on the
-    entry points of the library that the contexts come from."""
+    """ds_ocr_b200._spec, built first if only the sources are present or it was
+    built for another torch, on the entry points of the library that the
+    contexts come from."""
+    import importlib
     import torch  # noqa: F401  (its libraries have to be loaded)
+    from . import build
+    if build.spec_is_for_another():
+        build.build_spec()
+        importlib.invalidate_caches()
     try:
         from . import _spec
     except ImportError:
-        from . import build
-        build.build_spec()
+        build.build_spec(force=True)
+        importlib.invalidate_caches()
         from . import _spec
     lib = load()
     _spec.bind({name: ctypes.cast(getattr(lib, name), _ptr).value for name in SIGNATURES})

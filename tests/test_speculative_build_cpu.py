@@ -49,3 +49,34 @@ def test_an_old_module_does_not_outlive_a_failed_build(monkeypatch, tmp_path):
     with pytest.raises(subprocess.CalledProcessError):
         build.build_spec(force=True)
     assert not old.exists()
+
+
+def test_another_torch_or_python_rebuilds_the_module(monkeypatch):
+    assert build.build_spec() == build.SPEC  # up to date now
+    built = []
+    monkeypatch.setattr(subprocess, "check_call", lambda cmd: built.append(cmd))
+    monkeypatch.setattr(os, "remove", lambda path: None)
+    assert build.build_spec() == build.SPEC and not built
+    with monkeypatch.context() as m:
+        m.setattr(build, "SPEC_FOR", os.devnull)  # built for something else; written to nowhere
+        build.build_spec()
+        assert len(built) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0")
+    monkeypatch.setattr(build, "_write", lambda path, text: None)
+    build.build_spec()
+    assert len(built) == 2
+
+
+def test_a_module_that_does_not_load_is_built_again(monkeypatch):
+    import ds_ocr_b200
+    from ds_ocr_b200 import speculative
+    good, name, asked = speculative._module(), "ds_ocr_b200._spec", []
+    monkeypatch.delattr(ds_ocr_b200, "_spec")
+    monkeypatch.setitem(sys.modules, name, None)  # its import fails
+
+    def rebuilt(verbose=False, force=False):
+        asked.append(force)
+        sys.modules[name] = good
+
+    monkeypatch.setattr(build, "build_spec", rebuilt)
+    assert speculative._module() is good and asked == [True]
