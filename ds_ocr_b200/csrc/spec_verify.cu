@@ -339,7 +339,11 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
         buf[k] = x[k];
     }
     const float tt = temp ? temp[row] : 1.f, c1 = __fdiv_rn(1.44269504f, tt);
-    const float c = c1 == 0.f ? FLT_MIN : c1;  // an infinite temperature: -infinity times c stays so
+    // An infinite temperature: the least c, so that -infinity times c stays so
+    // and all else is equal. Differences are taken by halves, (x / 2 - m / 2) 2 c,
+    // because those of the largest logits pass F32's range.
+    const float c = c1 == 0.f ? FLT_TRUE_MIN : c1, c2 = 2.f * c == INFINITY ? FLT_MAX : 2.f * c;
+    auto weight = [&](float v, float half_m) { return tp_ex2(__fmaf_rn(0.5f, v, -half_m) * c2); };
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float m = -INFINITY;
@@ -385,14 +389,15 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
 #pragma unroll
     for (int w = 0; w < nt / 32; w++) m = fmaxf(m, sh[w]);
     m = fmaxf(m, -FLT_MAX);
+    const float hm = 0.5f * m;
     float s = 0.f;
 #pragma unroll 4
     for (int i = 4 * tid; i < all; i += 4 * nt) {
         float4 v = tp_four(store + i);
-        v.x = tp_ex2((v.x - m) * c);
-        v.y = tp_ex2((v.y - m) * c);
-        v.z = tp_ex2((v.z - m) * c);
-        v.w = tp_ex2((v.w - m) * c);
+        v.x = weight(v.x, hm);
+        v.y = weight(v.y, hm);
+        v.z = weight(v.z, hm);
+        v.w = weight(v.w, hm);
         if (F32) *reinterpret_cast<float4 *>(store + i) = v;
         s += (v.x + v.y) + (v.z + v.w);
     }
@@ -406,9 +411,9 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
     if (tid < ncta) cl.map_shared_rank(ms, tid)[rank] = make_float2(m, s);
     cl.sync();
     const float2 part = lane < ncta ? ms[lane] : make_float2(-FLT_MAX, 0.f);
-    const float M = warp_max(part.x), S = warp_sum(part.y * tp_ex2((part.x - M) * c));
-    const float f = S == 0.f ? 0.f : tp_ex2((m - M) * c) / S;
-    auto prob = [&](float v) { return (F32 ? v : tp_ex2((v - m) * c)) * f; };
+    const float M = warp_max(part.x), S = warp_sum(part.y * weight(part.x, 0.5f * M));
+    const float f = S == 0.f ? 0.f : weight(m, 0.5f * M) / S;
+    auto prob = [&](float v) { return (F32 ? v : weight(v, hm)) * f; };
     // four at a time between the output's 16-byte boundaries
     const int first = min(len, (int)((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / 4), quads = (len - first) / 4;
     for (int i = tid; i < len - 4 * quads; i += nt) {

@@ -497,6 +497,24 @@ def test_token_probs_of_an_infinite_temperature(spec):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [64, 70001])
+def test_token_probs_of_the_largest_logits(spec, dtype, vocab):
+    # logits over the type's whole range, whose differences pass it, at
+    # temperatures as large: -infinity alone is excluded by an infinite one
+    top, inf = torch.finfo(dtype).max, float("inf")
+    x = torch.linspace(-1, 1, vocab, device="cuda").mul(top).to(dtype).repeat(4, 1)
+    x[:, 5] = -inf
+    x[:, 6] = top
+    t = torch.tensor([inf, 3e38, 1e38, 2e37], device="cuda")
+    p = spec.token_probs(x, t)
+    y = x.double() / t.double()[:, None]
+    y[0] = torch.where(torch.isinf(x[0]), -inf, 0.0)
+    assert rel(p, torch.softmax(y, -1)) < 5e-6
+    assert not p[:, 5].any()
+    assert float((p[0, 6:] * (vocab - 1) - 1).abs().max()) < 5e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_token_probs_of_the_largest_vocabulary(spec, dtype):
     x = (2 * torch.randn(2, 917504, device="cuda")).to(dtype)
     assert rel(spec.token_probs(x), torch.softmax(x.double(), -1)) < 5e-6
