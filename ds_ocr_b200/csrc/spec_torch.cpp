@@ -101,6 +101,12 @@ struct Call {
     }
 };
 
+// A size for the C ABI, whose sizes are ints.
+int size(const char *name, int64_t n) {
+    if (n > INT32_MAX) throw Bad(std::string(name) + ": " + std::to_string(n) + " (at most 2^31 - 1)");
+    return (int)n;
+}
+
 int spec_type(const char *name, at::ScalarType t) {
     if (t == at::kBFloat16) return DS_CUDA_SPEC_BF16;
     if (t == at::kHalf) return DS_CUDA_SPEC_F16;
@@ -138,8 +144,8 @@ PyObject *tree_attention(PyObject *const *x, Py_ssize_t n_args) {
     if (k0.dim() != 4) throw Bad("k: expected [batch x n_kv_heads x kv_max x head_dim]");
     const int64_t kv = k0.size(1), cap = k0.size(2);
     const int64_t shape[4] = {b, n, heads, hd}, cache[4] = {b, kv, cap, hd}, tree[4] = {b, kv, n, hd};
-    d.batch = (int)b, d.n_nodes = (int)n, d.n_heads = (int)heads, d.n_kv_heads = (int)kv;
-    d.head_dim = (int)hd, d.kv_max = (int)cap;
+    d.batch = size("batch", b), d.n_nodes = size("n_nodes", n), d.n_heads = size("n_heads", heads);
+    d.n_kv_heads = size("n_kv_heads", kv), d.head_dim = size("head_dim", hd), d.kv_max = size("kv_max", cap);
     d.scale = x[10] == Py_None ? 1.f / std::sqrt((float)hd) : (float)PyFloat_AsDouble(x[10]);
     if (PyErr_Occurred()) throw Raised();
     const at::Tensor &q = c.strided("q", x[2], shape, type);
@@ -179,7 +185,7 @@ PyObject *tree_mask(PyObject *const *x, Py_ssize_t n_args) {
     const Call c(x, n_args, 4);
     const at::Tensor &p = c.tensor("parents", x[2]);
     if (p.dim() != 2) throw Bad("parents: expected [batch x n_nodes]");
-    const int64_t b = p.size(0), n = p.size(1);
+    const int64_t b = size("batch", p.size(0)), n = size("n_nodes", p.size(1));
     const int *parents = c.ptr<int>("parents", x[2], {b, n}, at::kInt), *nodes = c.maybe<int>("counts", x[3], {b}, at::kInt);
     const at::Tensor mask = at::empty({b, n, (n + 63) / 64}, c.options.dtype(at::kLong)), depth = at::empty({b, n}, c.options.dtype(at::kInt));
     c.check(abi.tree_mask_dev(c.ctx, parents, nodes, (int)b, (int)n, static_cast<uint64_t *>(mask.data_ptr()),
@@ -191,7 +197,7 @@ PyObject *token_probs(PyObject *const *x, Py_ssize_t n_args) {
     const Call c(x, n_args, 5);
     const at::Tensor &l = c.tensor("logits", x[2]);
     if (l.dim() != 2) throw Bad("logits: expected [rows x vocab]");
-    const int64_t shape[2] = {l.size(0), l.size(1)};
+    const int64_t shape[2] = {size("rows", l.size(0)), size("vocab", l.size(1))};
     const int type = spec_type("logits", l.scalar_type());
     c.strided("logits", x[2], shape, l.scalar_type());
     const float *temp = c.maybe<float>("temperature", x[3], {shape[0]}, at::kFloat);
@@ -218,7 +224,7 @@ PyObject *verify(PyObject *const *x, Py_ssize_t n_args) {
     if (p0.dim() != 3) throw Bad("target: expected [batch x n_nodes x vocab]");
     const int64_t b = t0.size(0), n = t0.size(1), vocab = p0.size(2), shape[3] = {b, n, vocab};
     ds_cuda_tree_verify_t d = {};
-    d.batch = (int)b, d.n_nodes = (int)n, d.vocab = (int)vocab;
+    d.batch = size("batch", b), d.n_nodes = size("n_nodes", n), d.vocab = size("vocab", vocab);
     d.tokens = c.ptr<int>("tokens", x[2], {b, n}, at::kInt);
     d.parents = c.ptr<int>("parents", x[3], {b, n}, at::kInt);
     auto probs = [&](const char *name, PyObject *o, const float *&p, int64_t *st) {
@@ -241,7 +247,7 @@ PyObject *verify_greedy(PyObject *const *x, Py_ssize_t n_args) {
     const Call c(x, n_args, 6);
     const at::Tensor &t0 = c.tensor("tokens", x[2]);
     if (t0.dim() != 2) throw Bad("tokens: expected [batch x n_nodes]");
-    const int64_t b = t0.size(0), n = t0.size(1);
+    const int64_t b = size("batch", t0.size(0)), n = size("n_nodes", t0.size(1));
     const int *tokens = c.ptr<int>("tokens", x[2], {b, n}, at::kInt), *parents = c.ptr<int>("parents", x[3], {b, n}, at::kInt);
     const int *want = c.ptr<int>("target_tokens", x[4], {b, n}, at::kInt), *nodes = c.maybe<int>("counts", x[5], {b}, at::kInt);
     const Results r(c, b, n);
@@ -264,8 +270,8 @@ PyObject *commit(PyObject *const *x, Py_ssize_t n_args) {
     const int64_t b = path.size(0), n = path.size(1), layers = first.size(0), kv = first.size(2), cap = first.size(3), hd = first.size(4);
     const int64_t cache[5] = {layers, b, kv, cap, hd}, tree[5] = {layers, b, kv, n, hd};
     ds_cuda_tree_commit_t d = {};
-    d.n_tensors = (int)m, d.layers = (int)layers, d.batch = (int)b, d.n_nodes = (int)n, d.n_kv_heads = (int)kv;
-    d.head_dim = (int)hd, d.kv_max = (int)cap;
+    d.n_tensors = (int)m, d.layers = size("layers", layers), d.batch = size("batch", b), d.n_nodes = size("n_nodes", n);
+    d.n_kv_heads = size("n_kv_heads", kv), d.head_dim = size("head_dim", hd), d.kv_max = size("kv_max", cap);
     for (Py_ssize_t i = 0; i < m; i++) {
         const at::Tensor &t = c.strided("cache", PySequence_Fast_GET_ITEM(x[2], i), cache, first.scalar_type());
         const at::Tensor &u = c.strided("tree", PySequence_Fast_GET_ITEM(x[3], i), tree, first.scalar_type());

@@ -761,6 +761,20 @@ def test_commit_refusals(spec):
         spec.commit([c[..., :4]], [t[..., :4]], *ok)
 
 
+def test_sizes_past_32_bits_are_refused(spec):
+    # sizes whose low 32 bits alone would be taken for small ones (views of one row)
+    far = (1 << 32) + 4
+    with pytest.raises(ValueError, match="rows"):
+        spec.token_probs(torch.zeros(1, 1, device="cuda").expand(far, 1))
+    c = Case("bf16", [3], [2], 2, 1, 1, 64, seed=1)
+    k = c.k[:, :, :1].expand(-1, -1, far, -1)
+    with pytest.raises(ValueError, match="kv_max"):
+        spec.tree_attention(c.q, k, k, c.tk, c.tv, c.lens, c.mask)
+    t, ints = torch.zeros(1, 1, 1, 1, 8, dtype=torch.float16, device="cuda"), torch.zeros(1, **I32)
+    with pytest.raises(ValueError, match="kv_max"):
+        spec.commit([t.expand(-1, -1, -1, far, -1)], [t], ints, ints[None], ints)
+
+
 def test_c_abi_refusals(cuda_ctx):
     lib, h = _lib.load(), cuda_ctx.h
     assert lib.ds_cuda_tree_attention_dev(h, None, None) < 0
