@@ -28,6 +28,7 @@
 namespace ds {
 
 constexpr int SA_MAX_NODES = 256;
+constexpr int SA_MAX_KV = INT32_MAX - 1023;  // lengths are rounded up to whole tiles, and the nodes' tiles further, in 32 bits
 constexpr int SA_THREADS = 128;
 constexpr int SA_WARPS = SA_THREADS / 32;
 constexpr int SA_CLUSTER = 16;  // CTAs of a cluster, at most
@@ -1786,11 +1787,11 @@ static int sa_check(ds_cuda_ctx *c, const ds_cuda_tree_attention_t *d) {
     if (!d) return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: null descriptor");
     if (d->type < 0 || d->type > DS_CUDA_SPEC_F32) return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: type %d", d->type);
     if (d->batch < 0 || d->n_nodes <= 0 || d->n_nodes > SA_MAX_NODES || d->n_kv_heads <= 0 || d->n_heads <= 0 ||
-        d->n_heads % d->n_kv_heads || (d->head_dim != 64 && d->head_dim != 128) || d->kv_max < 0)
+        d->n_heads % d->n_kv_heads || (d->head_dim != 64 && d->head_dim != 128) || d->kv_max < 0 || d->kv_max > SA_MAX_KV)
         return ctx_fail(c, DS_CUDA_EINVAL,
                         "tree_attention: unsupported shape batch=%d n_nodes=%d n_heads=%d n_kv_heads=%d head_dim=%d "
-                        "kv_max=%d (n_nodes <= %d, head_dim 64 or 128, n_heads a multiple of n_kv_heads)",
-                        d->batch, d->n_nodes, d->n_heads, d->n_kv_heads, d->head_dim, d->kv_max, SA_MAX_NODES);
+                        "kv_max=%d (n_nodes <= %d, head_dim 64 or 128, n_heads a multiple of n_kv_heads, kv_max <= %d)",
+                        d->batch, d->n_nodes, d->n_heads, d->n_kv_heads, d->head_dim, d->kv_max, SA_MAX_NODES, SA_MAX_KV);
     if (d->batch > 65535 || d->n_heads > 65535)
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: batch and n_heads are at most 65535");
     return DS_CUDA_OK;

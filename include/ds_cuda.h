@@ -568,7 +568,7 @@ int ds_cuda_prefill_stage_ms(ds_cuda_ctx_t *ctx, float *ms);
  * Strides are in elements; the head dimension is contiguous; base addresses
  * and strides are multiples of 16 bytes. The lo planes share their
  * tensor's strides and may be NULL (rows exact in BF16). head_dim 64 or 128.
- * Limits: batch and n_heads 65535; fewer than 2^31 tiles, i.e. batch x
+ * Limits: batch and n_heads 65535; kv_max 2^31 - 1024; fewer than 2^31 tiles, i.e. batch x
  * n_kv_heads x tiles of 8 to 256 query rows x (tiles of 64 rows that kv_max and
  * n_nodes have room for). */
 typedef struct {

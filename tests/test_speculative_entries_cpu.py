@@ -91,6 +91,16 @@ def test_attention_refuses_more_tiles(lib, ctx, sizes):
     assert d.workspace_bytes == 0 and lib.fake_state().contents.launches == 0
 
 
+@pytest.mark.parametrize("type", [S.BF16, S.F32])
+def test_attention_room_stays_below_2_to_31(lib, ctx, type):
+    # the kernels round lengths up to tiles in 32 bits
+    d = attention(type=type, batch=1, n_nodes=1, n_heads=1, n_kv_heads=1, kv_max=2 ** 31 - 1024)
+    assert attend(lib, ctx, d) == 0, lib.fake_message(ctx)
+    for room in (2 ** 31 - 1023, 2 ** 31 - 1):
+        d = attention(type=type, batch=1, n_nodes=1, n_heads=1, n_kv_heads=1, kv_max=room)
+        assert attend(lib, ctx, d) < 0 and b"kv_max" in lib.fake_message(ctx)
+
+
 def calls(lib, h):
     """name -> a call that launches."""
     a, v, c = attention(), S.TreeVerifyDesc(batch=2, n_nodes=3, vocab=100), S.TreeCommitDesc(
