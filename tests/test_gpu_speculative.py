@@ -388,6 +388,36 @@ def test_attention_is_repeatable_on_streams_and_in_graphs(spec):
     assert rel(out, c.want()[0]) < TOL["pair"]
 
 
+@pytest.mark.parametrize("kind,n,group", [("pair", 16, 1), ("bf16", 12, 1), ("bf16", 20, 4), ("f16", 60, 4)])
+def test_attention_with_room_on_streams_and_in_graphs(spec, kind, n, group):
+    # the same for calls that cut a list of tiles and join the parts in a second
+    # kernel, on mma.sync and on tcgen05; replays with other lengths, so that
+    # the items are cut elsewhere
+    cs = [Case(kind, [900, 40, 0], [n, n // 2, n], n, 4, group, 64, seed=s, pad=ROOM, garbage=False) for s in (25, 26)]
+    want = [c.run(spec) for c in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cs]
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(c.run(spec))
+    torch.cuda.synchronize()
+    for w, many in zip(want, got):
+        assert all(torch.equal(w, x) for x in many)
+    c = cs[0]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = c.run(spec)
+    for lens, counts in (([5, 2000, 64], [1, n, 0]), ([4097, 1, 127], [n, n, 3])):
+        c.lens.copy_(torch.tensor(lens, **I32))
+        c.counts.copy_(torch.tensor(counts, **I32))
+        g.replay()
+        torch.cuda.synchronize()
+        assert rel(out, c.want()[0]) < TOL[kind]
+    spec.check()
+
+
 def test_attention_clamps_lengths_and_counts(spec):
     c = Case("bf16", [30, 30], [4, 4], 4, 2, 1, 64, seed=17, pad=0, garbage=False)
     want = c.run(spec)
@@ -759,6 +789,65 @@ def test_commit_refusals(spec):
         spec.commit([c[..., 4:12]], [t[..., :8]], *ok)
     with pytest.raises(DsCudaError):
         spec.commit([c[..., :4]], [t[..., :4]], *ok)
+
+
+def test_a_step_on_streams_and_in_a_graph(spec):
+    # probabilities, verification and commit as one captured sequence, replayed
+    # on other inputs, and on two streams at once
+    rng = np.random.default_rng(27)
+    b, n, vocab, cap = 5, 9, 3001, 40
+
+    def inputs():
+        s = sampled(b, n, vocab, int(rng.integers(1 << 30)), certain=True)
+        s["logits"] = rng.normal(0, 2, (b * n, vocab)).astype(np.float32)
+        s["lens"] = rng.integers(0, cap, b).astype(np.int32)
+        del s["target"], s["draft"]
+        return s
+
+    def state():
+        g = on_gpu(inputs())
+        g["temperature"] = torch.full((b * n,), 0.7, device="cuda")
+        g["cache"] = torch.zeros(2, b, 2, cap, 8, dtype=torch.bfloat16, device="cuda")
+        g["tree"] = torch.randn(2, b, 2, n, 8, device="cuda").bfloat16()
+        return g
+
+    def step(g):
+        p = spec.token_probs(g["logits"], g["temperature"]).view(b, n, vocab)
+        path, acc, tok = spec.verify(g["tokens"], g["parents"], p, None, g["accept_u"], g["sample_u"], g["counts"])
+        return p, path, acc, tok, spec.commit([g["cache"]], [g["tree"]], g["lens"], path, acc), g["cache"]
+
+    def check(g, got):
+        p, path, acc, tok, lens, cache = (t.float().cpu().numpy() if t.dtype == torch.bfloat16 else t.cpu().numpy() for t in got)
+        h = {k: v.float().cpu().numpy() if v.dtype == torch.bfloat16 else v.cpu().numpy() for k, v in g.items()}
+        want = np.zeros_like(cache)
+        for i in range(b):
+            w, t = R.verify(h["tokens"][i], h["parents"][i], h["counts"][i], p[i], None, h["accept_u"][i], h["sample_u"][i])
+            assert path[i].tolist() == w + [-1] * (n - len(w)) and acc[i] == len(w) - 1 and tok[i] == t
+            m = min(len(w), cap - h["lens"][i])
+            want[:, i, :, h["lens"][i]:h["lens"][i] + m] = h["tree"][:, i][:, :, w[:m]]
+            assert lens[i] == h["lens"][i] + m
+        assert np.array_equal(cache, want)
+
+    g = state()
+    check(g, step(g))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(g)
+    for _ in range(3):
+        for k, v in state().items():
+            g[k].copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(g, got)
+    gs, streams = [state() for _ in range(8)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i, g in enumerate(gs):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(step(g))
+    torch.cuda.synchronize()
+    for g, o in zip(gs, outs):
+        check(g, o)
 
 
 def test_sizes_past_32_bits_are_refused(spec):
