@@ -528,8 +528,13 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
             for (int e = 0; e < 2; e++) bits[n][e] = word(n, e, 0);
         }
     };
-    // (the first item's before the rows: they arrive while those are asked for)
-    q_load();
+    // The first item's before the rows: they arrive while those are asked for.
+    // Not where the registers are short (F32, 16 rows or three CTAs an SM): held
+    // ahead they make the loop spill, 64 streams of 10 heads, up to 1325 tokens:
+    // 16 / 32 / 64 nodes 182 / 348 / 700 us instead of 126 / 243 / 480, 8 nodes
+    // on a single plane 61 instead of 54.
+    constexpr bool AHEAD = !F32 || (NG == 1 && S::PL == 2);
+    if (AHEAD) q_load();
     if (tiles > 0) {
         aim();
         load(0, 0);
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
     for (int i = 0; i < tiles; i++, slot = wrap(slot + 2)) {
         if (fresh) {
             fresh = false;
-            if (i > 0) q_load();
+            if (!AHEAD || i > 0) q_load();
 #pragma unroll
             for (int n = 0; n < NG; n++) {
 #pragma unroll

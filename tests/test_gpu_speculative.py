@@ -418,6 +418,26 @@ def test_attention_with_room_on_streams_and_in_graphs(spec, kind, n, group):
     spec.check()
 
 
+@pytest.mark.parametrize("kind", ["pair", "plane"])
+def test_attention_of_sixteen_nodes_is_cheaper_than_twice_eight(spec, kind):
+    # both read the cache once: 1.4 times the time of eight, 2.0 where the kernel spills
+    times = []
+    for n in (8, 16):
+        c = Case(kind, [1325] * 64, [n] * 64, n, 10, 1, 128, seed=n, garbage=False)
+        c.run(spec)
+        e = [torch.cuda.Event(enable_timing=True) for _ in range(11)]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(5):
+                c.run(spec)
+        for x in e:
+            g.replay()
+            x.record()
+        torch.cuda.synchronize()
+        times.append(min(x.elapsed_time(y) for x, y in zip(e, e[1:])))
+    assert times[1] < 1.75 * times[0], times
+
+
 def test_attention_clamps_lengths_and_counts(spec):
     c = Case("bf16", [30, 30], [4, 4], 4, 2, 1, 64, seed=17, pad=0, garbage=False)
     want = c.run(spec)
