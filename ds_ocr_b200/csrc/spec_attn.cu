@@ -42,6 +42,7 @@ struct SaArgs {
     int row_tiles;  // ceil(rows / row tile)
     int per_seq;    // n_kv_heads * row_tiles: items of a sequence
     int sms, ctas;  // SMs; runs the tile list is cut into, at most
+    int cluster;    // CTAs of an item's cluster; 0: the list
     float scale2;   // scale * log2(e)
     unsigned *err;  // bounded waits that gave up
     float *part;    // workspace: [ctas][2][row tile][head_dim], then ...
@@ -1616,17 +1617,61 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
 // Calls whose items are few enough for a cluster each in one wave, with at
 // most 8 tiles a CTA, are joined in the clusters: one launch, no workspace.
 // Their tiles are bounded by the cache's room, the lengths not being known
-// here. Others take the list. Clusters have 16 CTAs, or 8 with eight rows a
-// tile (with 16, F32, 32 rows of 10 heads over 662 tokens take 14 us in
+// here. Others take the list. How many clusters are a wave the runtime says: a
+// cluster is of one GPC, whose SMs need not be a multiple of its CTAs (one node,
+// 16 heads, 662 tokens, F32: two waves of 16 CTAs take 12.7 us, one of 8 CTAs
+// 8.7 us). Clusters have 16 CTAs, or 8 with eight rows a tile (with 16, F32, 32 rows of 10 heads over 662 tokens take 14 us in
 // clusters of 8 and 12.6 in the list).
 // (One stream, 10 heads, 662 tokens, F32 in two planes: one node takes 7.1 us
 // on the GPU against 7.9, and the call 7 us of the host's time instead of 13.)
 static long long sa_most_tiles(const ds_cuda_tree_attention_t *d, int kt) {
     return ((long long)d->kv_max + kt - 1) / kt + (d->n_nodes + kt - 1) / kt;
 }
-template <class S> static int sa_clusters(const ds_cuda_tree_attention_t *d, long long items, int sms) {
+// A kernel's attributes, once per device (of the first 64).
+template <class S, bool CLUSTER> static cudaError_t sa_attributes(int device) {
+    static std::atomic<uint64_t> ready;
+    if (device < 64 && ready.load() >> device & 1) return cudaSuccess;
+    const void *f;
+    if constexpr (SaMade<S>::by_dimension) f = (const void *)sa_many_kernel<S>;
+    else f = (const void *)sa_few_kernel<S, CLUSTER>;
+    cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e == cudaSuccess && CLUSTER) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && device < 64) ready.fetch_or(1ull << device);
+    return e;
+}
+template <class S> static cudaLaunchConfig_t sa_cluster_config(cudaLaunchAttribute &attr, dim3 grid, int n, cudaStream_t st) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = n;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(SA_THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+// Clusters of n CTAs that the (current) device holds at once; asked once per
+// device of the first 64. 0 where it cannot say, which leaves the list.
+template <class S> static int sa_wave(int device, int n) {
+    static std::atomic<int> known[64][2];  // 1 + the answer, of 8 and of 16 CTAs
+    std::atomic<int> *const k = device < 64 ? &known[device][n > 8] : nullptr;
+    if (const int v = k ? k->load() : 0) return v - 1;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = sa_cluster_config<S>(attr, dim3(n), n, nullptr);
+    int most = 0;
+    if (sa_attributes<S, true>(device) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&most, (const void *)sa_few_kernel<S, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        most = 0;
+    }
+    if (k) k->store(1 + most);
+    return most;
+}
+template <class S> static int sa_clusters(const ds_cuda_tree_attention_t *d, long long items, int device) {
     for (int n = SA_CLUSTER; n >= (S::RT == 8 ? 8 : SA_CLUSTER); n /= 2)
-        if (items * n <= sms * S::PER_SM && sa_most_tiles(d, S::KT) <= 8 * n) return n;
+        if (sa_most_tiles(d, S::KT) <= 8 * n && items <= sa_wave<S>(device, n)) return n;
     return 0;
 }
 
@@ -1660,45 +1705,27 @@ static bool sa_map(const ds_cuda_tree_attention_t &d, int kv, int kt, CUtensorMa
 }
 
 template <class S> struct SaRun {
-    static int clusters(const SaArgs &a) { return SaMade<S>::by_dimension ? 0 : sa_clusters<S>(&a.d, (long long)a.d.batch * a.per_seq, a.sms); }
+    static int clusters(const ds_cuda_tree_attention_t *d, long long items, int device) {
+        if constexpr (SaMade<S>::by_dimension) return 0;
+        else return sa_clusters<S>(d, items, device);
+    }
     static size_t workspace(const SaArgs &a) {
         // two parts a CTA, then their maxima and sums
-        return clusters(a) ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
-    }
-    // A kernel's attributes, once per device (of the first 64).
-    template <bool CLUSTER> static cudaError_t attributes(int device) {
-        static std::atomic<uint64_t> ready;
-        if (device < 64 && ready.load() >> device & 1) return cudaSuccess;
-        const void *f;
-        if constexpr (SaMade<S>::by_dimension) f = (const void *)sa_many_kernel<S>;
-        else f = (const void *)sa_few_kernel<S, CLUSTER>;
-        cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-        if (e == cudaSuccess && CLUSTER) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e == cudaSuccess && device < 64) ready.fetch_or(1ull << device);
-        return e;
+        return a.cluster ? 0 : (size_t)a.sms * S::PER_SM * 2 * S::RT * (S::HD * 4 + 8);
     }
     static cudaError_t run(SaArgs a, int device, cudaStream_t st) {
         void *args[] = {&a};
-        if constexpr (!SaMade<S>::by_dimension) if (const int ncta = clusters(a)) {
-            const cudaError_t e = attributes<true>(device);
+        if constexpr (!SaMade<S>::by_dimension) if (a.cluster) {
+            const cudaError_t e = sa_attributes<S, true>(device);
             if (e != cudaSuccess) return e;
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(a.row_tiles * ncta, a.d.n_kv_heads, a.d.batch);
-            cfg.blockDim = dim3(SA_THREADS);
-            cfg.dynamicSmemBytes = S::SMEM;
-            cfg.stream = st;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = ncta;
-            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
+            cudaLaunchAttribute attr;
+            const cudaLaunchConfig_t cfg = sa_cluster_config<S>(attr, dim3(a.row_tiles * a.cluster, a.d.n_kv_heads, a.d.batch), a.cluster, st);
             return cudaLaunchKernelExC(&cfg, (const void *)sa_few_kernel<S, true>, args);
         }
         a.ctas = a.sms * S::PER_SM;
         a.part = (float *)a.d.workspace;
         a.ml = (float2 *)(a.part + (size_t)a.ctas * 2 * S::RT * S::HD);
-        cudaError_t e = attributes<false>(device);
+        cudaError_t e = sa_attributes<S, false>(device);
         if (e != cudaSuccess) return e;
         if constexpr (SaMade<S>::by_dimension) {
             SaManyArgs many = {};
@@ -1735,22 +1762,22 @@ template <int HD, int QT, class F> static auto sa_pick16(int rows, bool apart, b
            : rows <= 16 || brief ? f(SaRun<SaFew<HD, 2, 1, QT>>())
            : rows <= 128         ? f(SaRun<SaMany<HD, false, QT>>()) : f(SaRun<SaMany<HD, true, QT>>());
 }
-template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, int sms, F f) {
+template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t *d, const ds_cuda_ctx *c, F f) {
     constexpr int P = DS_CUDA_SPEC_F32;
     const int rows = d->n_nodes * (d->n_heads / d->n_kv_heads);
     using Few = SaFew<HD, 2, 1, DS_CUDA_SPEC_BF16>;
-    const bool brief = (double)d->batch * d->n_kv_heads * ((rows + 15) / 16) * sa_most_tiles(d, SA_KT) <= 8.0 * sms * Few::PER_SM;
+    const bool brief = (double)d->batch * d->n_kv_heads * ((rows + 15) / 16) * sa_most_tiles(d, SA_KT) <= 8.0 * c->sm_count * Few::PER_SM;
     using Eight = SaFew<HD, 1, 2, P>;
     const long long eights = (long long)d->batch * d->n_kv_heads * ((rows + 7) / 8);
-    const bool apart = rows <= 8 || 2 * sa_clusters<Eight>(d, eights, sms) >= sa_most_tiles(d, SA_KT);
+    const bool apart = rows <= 8 || 2 * sa_clusters<Eight>(d, eights, c->device) >= sa_most_tiles(d, SA_KT);
     if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, apart, brief, f);
     if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, apart, brief, f);
     if (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo)
         return apart ? f(SaRun<SaFew<HD, 1, 2, P>>()) : f(SaRun<SaFew<HD, 2, 2, P>>());
     return apart ? f(SaRun<SaFew<HD, 1, 1, P>>()) : f(SaRun<SaFew<HD, 2, 1, P>>());
 }
-template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, int sms, F f) {
-    return d->head_dim == 64 ? sa_pick_hd<64>(d, sms, f) : sa_pick_hd<128>(d, sms, f);
+template <class F> static auto sa_pick(const ds_cuda_tree_attention_t *d, const ds_cuda_ctx *c, F f) {
+    return d->head_dim == 64 ? sa_pick_hd<64>(d, c, f) : sa_pick_hd<128>(d, c, f);
 }
 template <class S> static S sa_shape(SaRun<S>) { return S(); }
 
@@ -1810,7 +1837,7 @@ static int sa_args(const ds_cuda_ctx *c, ds_cuda_ctx *err, const ds_cuda_tree_at
     a.words = (d->n_nodes + 63) / 64;
     a.group = d->n_heads / d->n_kv_heads;
     a.rows = d->n_nodes * a.group;
-    const int rt = sa_pick(d, c->sm_count, [](auto r) { return decltype(sa_shape(r))::RT; });
+    const int rt = sa_pick(d, c, [](auto r) { return decltype(sa_shape(r))::RT; });
     a.row_tiles = (a.rows + rt - 1) / rt;
     a.per_seq = d->n_kv_heads * a.row_tiles;
     // (the list's places are 32-bit; its lengths are known on the device alone)
@@ -1818,19 +1845,23 @@ static int sa_args(const ds_cuda_ctx *c, ds_cuda_ctx *err, const ds_cuda_tree_at
     if (tiles > INT32_MAX)
         return ctx_fail(err, DS_CUDA_EINVAL, "tree_attention: up to %lld tiles of %d keys and %d rows (< 2^31)", tiles, SA_KT, rt);
     a.sms = c->sm_count;
+    a.cluster = sa_pick(d, c, [&](auto r) { return decltype(r)::clusters(d, (long long)d->batch * a.per_seq, c->device); });
     a.err = c->d_spec_err;
     a.scale2 = d->scale * 1.44269504f;
     return DS_CUDA_OK;
 }
 
 extern "C" size_t ds_cuda_tree_attention_workspace(const ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d) {
+    if (!c || !c->ok) return 0;
+    const CtxDevice on(c);
     SaArgs a = {};
-    if (!c || !c->ok || sa_args(c, nullptr, d, a) < 0) return 0;
-    return sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::workspace(a); });
+    if (sa_args(c, nullptr, d, a) < 0) return 0;
+    return sa_pick(d, c, [&](auto r) { return decltype(r)::workspace(a); });
 }
 
 extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_attention_t *d, void *stream) {
     if (!c || !c->ok) return DS_CUDA_EINVAL;
+    const CtxDevice on(c);
     SaArgs a = {};
     const int rc = sa_args(c, c, d, a);
     if (rc < 0 || d->batch == 0) return rc;
@@ -1854,12 +1885,11 @@ extern "C" int ds_cuda_tree_attention_dev(ds_cuda_ctx_t *c, const ds_cuda_tree_a
         if (t.lo && d->type != DS_CUDA_SPEC_F32)
             return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: %s has a lo plane, which only the F32 type takes", t.name);
     }
-    const size_t need = sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::workspace(a); });
+    const size_t need = sa_pick(d, c, [&](auto r) { return decltype(r)::workspace(a); });
     if (need && (!d->workspace || d->workspace_bytes < need || (reinterpret_cast<uintptr_t>(d->workspace) & 255)))
         return ctx_fail(c, DS_CUDA_EINVAL, "tree_attention: workspace of %zu bytes, 256-byte aligned, wanted", need);
-    const CtxDevice on(c);
     cudaStream_t st = stream ? (cudaStream_t)stream : c->stream;
-    const cudaError_t e = sa_pick(d, c->sm_count, [&](auto r) { return decltype(r)::run(a, c->device, st); });
+    const cudaError_t e = sa_pick(d, c, [&](auto r) { return decltype(r)::run(a, c->device, st); });
     if (e != cudaSuccess) cudaGetLastError();  // reported here, not by whoever asks next
     return ctx_cuda(c, e, "tree_attention launch");
 }

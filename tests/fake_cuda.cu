@@ -15,6 +15,8 @@ struct Fake {
     int launch_device;    // the current device at the last of them
     unsigned word;        // what a copy from the device finds
     int error;            // what the next launch answers
+    int cluster;          // CTAs of a cluster at the last launch that named it
+    int room[17];         // clusters of so many CTAs that the GPU holds at once
 };
 static Fake fake;
 static cudaError_t last;
@@ -24,6 +26,7 @@ ds_cuda_ctx *fake_new(int device, int sms) {
     fake = Fake();
     fake.devices = 4;
     fake.launch_device = -1;
+    for (int n = 1; n <= 16; n++) fake.room[n] = sms / n;
     ds_cuda_ctx *c = new ds_cuda_ctx;
     c->device = device;
     c->sm_count = sms;
@@ -55,7 +58,14 @@ cudaError_t cudaGetLastError() {
 }
 cudaError_t cudaFuncSetAttribute(const void *, cudaFuncAttribute, int) { return cudaSuccess; }
 cudaError_t cudaLaunchKernel(const void *, dim3, dim3, void **, size_t, cudaStream_t) { return launched(); }
-cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t *, const void *, void **) { return launched(); }
+cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t *c, const void *, void **) {
+    for (unsigned i = 0; i < c->numAttrs; i++)
+        if (c->attrs[i].id == cudaLaunchAttributeClusterDimension) fake.cluster = c->attrs[i].val.clusterDim.x;
+    return launched();
+}
+cudaError_t cudaOccupancyMaxActiveClusters(int *n, const void *, const cudaLaunchConfig_t *c) {
+    return *n = fake.room[c->attrs[0].val.clusterDim.x], cudaSuccess;
+}
 cudaError_t cudaGetDriverEntryPoint(const char *, void **, unsigned long long, cudaDriverEntryPointQueryResult *) {
     return cudaErrorNotSupported;
 }

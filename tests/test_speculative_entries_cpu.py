@@ -13,7 +13,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 class State(ctypes.Structure):
     _fields_ = [("device", ctypes.c_int), ("devices", ctypes.c_int), ("launches", ctypes.c_int),
-                ("launch_device", ctypes.c_int), ("word", ctypes.c_uint), ("error", ctypes.c_int)]
+                ("launch_device", ctypes.c_int), ("word", ctypes.c_uint), ("error", ctypes.c_int), ("cluster", ctypes.c_int),
+                ("room", ctypes.c_int * 17)]
 
 
 @pytest.fixture(scope="module")
@@ -150,3 +151,19 @@ def test_every_stream_hears_of_a_wait_that_gave_up(lib, ctx):
         assert check(ctx, s) == 0
     f.word += 1
     assert [check(ctx, s) for s in (b, b, a, a)] == [-7, 0, -7, 0]
+
+
+@pytest.mark.parametrize("sixteen,eight,heads,cluster", [
+    (14, 30, 14, 16), (14, 30, 15, 8), (14, 30, 30, 8), (14, 30, 31, 0),
+    (0, 0, 1, 0),  # a share of a GPU that holds none at all
+])
+def test_clusters_are_as_many_as_the_gpu_holds_at_once(lib, sixteen, eight, heads, cluster):
+    # (what a GPU holds is asked once a device: each case has its own)
+    device = 10 + sixteen + heads
+    h = lib.fake_new(device, 148)
+    f = lib.fake_state().contents
+    f.devices, f.room[16], f.room[8] = 64, sixteen, eight
+    d = attention(type=S.F32, batch=1, n_nodes=1, n_heads=heads, n_kv_heads=heads, head_dim=128, kv_max=680)
+    assert attend(lib, h, d) == 0, lib.fake_message(h)
+    assert (f.cluster, f.launches, d.workspace_bytes > 0) == (cluster, 1 if cluster else 2, not cluster)
+    lib.fake_free(h)
