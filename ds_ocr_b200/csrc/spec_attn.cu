@@ -1620,10 +1620,10 @@ __global__ void __launch_bounds__(SJ_THREADS) sa_join_kernel(const __grid_consta
 // here. Others take the list. How many clusters are a wave the runtime says: a
 // cluster is of one GPC, whose SMs need not be a multiple of its CTAs (one node,
 // 16 heads, 662 tokens, F32: two waves of 16 CTAs take 12.7 us, one of 8 CTAs
-// 8.7 us). Clusters have 16 CTAs, or 8 with eight rows a tile (with 16, F32, 32 rows of 10 heads over 662 tokens take 14 us in
-// clusters of 8 and 12.6 in the list).
-// (One stream, 10 heads, 662 tokens, F32 in two planes: one node takes 7.1 us
-// on the GPU against 7.9, and the call 7 us of the host's time instead of 13.)
+// 8.7 us). Clusters have 16 CTAs, or 8 with eight rows a tile (with 16, F32, 32 rows of 10 heads over 662 tokens take 13.7 us in
+// clusters of 8 and 12.5 in the list).
+// (One stream, 10 heads, 662 tokens, F32 in two planes: one node takes 7.3 us
+// on the GPU against 8.0, and the call 7 us of the host's time instead of 13.)
 static long long sa_most_tiles(const ds_cuda_tree_attention_t *d, int kt) {
     return ((long long)d->kv_max + kt - 1) / kt + (d->n_nodes + kt - 1) / kt;
 }
@@ -1745,17 +1745,17 @@ template <class S> struct SaRun {
 
 // f(instantiation) for a call, by its rows a KV head. F32 takes mma.sync, 8 or
 // 16 rows at a time (tcgen05 has no form for its three planes' separate sums).
-// Eight at a time also where each tile of eight has a cluster of at most two
-// tiles a CTA: one stream of 10 heads, 662 tokens, 16 rows, F32 10.1 us
-// against 11.6 us, BF16 8.7 against 9.9, both before the join's loads were
-// batched (with three tiles a CTA it loses: 16
-// against 12 us for 20 rows of 8 KV heads, 1000 tokens).
+// Eight at a time also where each tile of eight has a cluster: one stream of 10
+// heads, 16 rows, room for 1024 rows of which 662 are used, F32 9.1 us against
+// 12.4, BF16 8.2 against 10.4; 20 rows of 8 KV heads, 1900 / 3900 tokens, F32
+// 13.2 / 20.3 against 17.2 / 22.3; one head, 200 rows, 662 / 4000 tokens, F32
+// 10.4 / 23.1 against 12.8 / 23.2.
 // 16-bit types take mma.sync up to 16 rows, and for more where the call is brief: at
 // most 8 tiles a CTA, by the cache's room. Else tcgen05, one block of 128 rows
 // or two. BF16, mma.sync against tcgen05: 64 streams of 10 heads, up to 1325
-// tokens, 8 / 16 / 24 / 48 rows 51 / 68 / 118 / 184 us against 79 / 80 / 81 /
-// 84 us (but 8 streams on 8 KV heads, up to 8191 tokens, 16 rows 46 against
-// 41); brief: one stream, 662 tokens, 32 / 64 / 128 rows 11 / 14 / 20 us
+// tokens, 8 / 16 / 24 / 48 rows 51 / 66 / 118 / 184 us against 79 / 80 / 81 /
+// 84 us (but 8 streams on 8 KV heads, up to 8191 tokens, 16 rows 45 against
+// 41); brief: one stream, 662 tokens, 32 / 64 / 128 rows 12 / 13 / 20 us
 // against 20 / 20 / 27 us.
 template <int HD, int QT, class F> static auto sa_pick16(int rows, bool apart, bool brief, F f) {
     return apart                 ? f(SaRun<SaFew<HD, 1, 1, QT>>())
@@ -1769,7 +1769,7 @@ template <int HD, class F> static auto sa_pick_hd(const ds_cuda_tree_attention_t
     const bool brief = (double)d->batch * d->n_kv_heads * ((rows + 15) / 16) * sa_most_tiles(d, SA_KT) <= 8.0 * c->sm_count * Few::PER_SM;
     using Eight = SaFew<HD, 1, 2, P>;
     const long long eights = (long long)d->batch * d->n_kv_heads * ((rows + 7) / 8);
-    const bool apart = rows <= 8 || 2 * sa_clusters<Eight>(d, eights, c->device) >= sa_most_tiles(d, SA_KT);
+    const bool apart = rows <= 8 || sa_clusters<Eight>(d, eights, c->device) > 0;
     if (d->type == DS_CUDA_SPEC_F16) return sa_pick16<HD, DS_CUDA_SPEC_F16>(rows, apart, brief, f);
     if (d->type == DS_CUDA_SPEC_BF16) return sa_pick16<HD, DS_CUDA_SPEC_BF16>(rows, apart, brief, f);
     if (d->k_lo || d->v_lo || d->tree_k_lo || d->tree_v_lo)

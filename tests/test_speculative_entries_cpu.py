@@ -167,3 +167,16 @@ def test_clusters_are_as_many_as_the_gpu_holds_at_once(lib, sixteen, eight, head
     assert attend(lib, h, d) == 0, lib.fake_message(h)
     assert (f.cluster, f.launches, d.workspace_bytes > 0) == (cluster, 1 if cluster else 2, not cluster)
     lib.fake_free(h)
+
+
+@pytest.mark.parametrize("type", [S.F32, S.BF16])
+def test_room_alone_does_not_change_a_small_call(lib, type):
+    # one stream of 10 heads and a tree of 16: tiles of 8 rows in 20 clusters of
+    # 8 CTAs up to 8 tiles a CTA, then tiles of 16 rows in 10 clusters of 16
+    h = lib.fake_new(40 + type, 148)
+    f = lib.fake_state().contents
+    f.devices, f.room[16], f.room[8] = 64, 14, 30
+    for room, cluster in ((680, 8), (961, 8), (1024, 8), (4032, 8), (4096, 16)):
+        d = attention(type=type, batch=1, n_nodes=16, n_heads=10, n_kv_heads=10, head_dim=128, kv_max=room)
+        assert attend(lib, h, d) == 0 and f.cluster == cluster, room
+    lib.fake_free(h)
