@@ -408,11 +408,14 @@ __device__ __forceinline__ void sa_cluster_join(const SaArgs &a, const SaCursor 
 // one is used, two are in flight, with eight warps an SM 128 KB of them. The
 // queries stay in registers. F32 queries and weights are three BF16 planes
 // (exact), K and V two; products below 2^-24 of the largest are left out.
+// (Times here and below are of calls in a graph, the same inputs each time.)
 // Bound by the memory for 8 rows: 64 streams of 10 heads, up to 1325 tokens, F32
-// in two planes, 93 us, 6.0 TB/s. With 16 F32 rows bound by mma.sync's rate
-// (five products an element). One stream of 662 tokens is bound by latency:
-// lengths, one tile's rows, the tile's steps, the cluster's join follow one
-// another: 7.1 us for one node, 9.1 us for 16.
+// in two planes, 93 us, 6.0 TB/s. Two groups of F32 rows take 126 us for them:
+// five products an element with eight warps an SM, short of both the memory's
+// rate and mma.sync's (a quarter of it). More rows read K and V once per 16:
+// 243 us for 32, 480 us for 64 nodes. One stream of 662 tokens is bound by
+// latency: lengths, one tile's rows, the tile's steps, the cluster's join follow
+// one another: 7.2 us for one node, 9.1 us for 16.
 template <int HD_, int NG_, int PL_, int QT_> struct SaFew {
     static constexpr int HD = HD_, NG = NG_, PL = PL_, QT = QT_;
     static constexpr int QP = QT == DS_CUDA_SPEC_F32 ? 3 : 1;
@@ -850,11 +853,12 @@ __global__ void __launch_bounds__(SA_THREADS, S::PER_SM) sa_few_kernel(const __g
 // or of a later one whose weights passed 2^10 (FP16: 2^8), so that O is rarely
 // rescaled. P has the cache's type: its rounding is of the same size as V's. Bound by
 // the memory at 124 rows (8 streams, 32 heads on 8, head_dim 128, up to 8191
-// tokens: 47.6 us, 3.9 TB/s over the whole call, the runs themselves at the
+// tokens: 47.4 us, 3.9 TB/s over the whole call, the runs themselves at the
 // memory's rate, 10 us of start and item ends, 8 us of join), by the softmax at
-// 512 rows (one stream, 16 heads on 2, head_dim 64, 131071 tokens: 77 us, 450
+// 512 rows (one stream, 16 heads on 2, head_dim 64, 131071 tokens: 78 us, 440
 // TFLOP/s; a step of 2 x 128 rows and 64 keys takes 1850 cycles, 1024 of them
-// the exponentials' least). Tried for the latter: P in columns of its own, which
+// the exponentials' least, and a CTA's 56 steps 53 us; the rest is start, parts
+// and join). Tried for the latter: P in columns of its own, which
 // lets S be issued a product earlier (82 us), turns of the two streams (97
 // against 85 us at the time), packed F32 operations (no change).
 // Two producer warps bring K and V rows into a ring each (of K and of V, or of
@@ -1744,7 +1748,9 @@ template <class S> struct SaRun {
 };
 
 // f(instantiation) for a call, by its rows a KV head. F32 takes mma.sync, 8 or
-// 16 rows at a time (tcgen05 has no form for its three planes' separate sums).
+// 16 rows at a time (on tcgen05 the planes' products could have columns of their
+// own, but its sums round towards zero, so that they would have to be folded
+// into F32 every few tiles: not built).
 // Eight at a time also where each tile of eight has a cluster: one stream of 10
 // heads, 16 rows, room for 1024 rows of which 662 are used, F32 9.1 us against
 // 12.4, BF16 8.2 against 10.4; 20 rows of 8 KV heads, 1900 / 3900 tokens, F32
@@ -1783,7 +1789,7 @@ template <class S> static S sa_shape(SaRun<S>) { return S(); }
 
 // One CTA per sequence, one thread per node: a node's word bits are set by
 // walking up its parents (kept in shared memory; at most n_nodes steps).
-// Bound by the walk's latency: one tree of 16 takes 2.3 us, 64 random ones of
+// Bound by the walk's latency: one tree of 16 takes 2.4 us, 64 random ones of
 // 64 or 256 nodes 5.2 and 16 us, once a step for all layers.
 __global__ void tree_mask_kernel(const int *parents, const int *nodes, int n, int words, uint64_t *mask, int *depth) {
     __shared__ int par[SA_MAX_NODES];

@@ -57,9 +57,11 @@ __device__ __forceinline__ unsigned long long warp_scan_u64(unsigned long long v
 // What bounds it is latency: the gather, then per row pass one read of the
 // row (two with a draft) and one exchange of sums in the cluster. A chain of 7
 // over 129280 tokens takes 7.8 us (5.8 with nothing to verify), 16 trees of 30
-// with up to two rows and three exchanges 15.8 us, 64 trees of 15 over 32001
-// tokens 15.3 us. Rows read ahead of the walk make the first 10.8 us: most of
-// them turn out not to be needed.
+// with up to two rows and three exchanges 15.9 us, 64 trees of 15 over 32001
+// tokens 15.2 us; with certain drafts 7.2, 17.5 and 10.6 us (in a graph, the
+// same inputs each time). Rows read ahead of the walk make the first 10.8 us:
+// most of them turn out not to be needed. VPT = 64 (more than 131072 tokens)
+// spills 196 bytes.
 template <int VPT>
 __global__ void __launch_bounds__(SV_THREADS) tree_verify_kernel(const __grid_constant__ ds_cuda_tree_verify_t d) {
     __shared__ int par[SV_MAX_NODES], tok[SV_MAX_NODES], way[SV_MAX_NODES];
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(SV_THREADS) tree_verify_kernel(const __grid_co
 
 // A warp per sequence, its trees in shared memory; the current node's children
 // are looked for 32 nodes at a time. Bound by latency: one tree of 16
-// takes 2.1 us, 64 of 64 or 256 nodes 3.1 and 3.4 us (9.2 and 30 with a thread
+// takes 2.3 us, 64 of 64 or 256 nodes 3.1 and 3.4 us (9.2 and 30 with a thread
 // per sequence).
 __global__ void __launch_bounds__(32) tree_verify_greedy_kernel(const int *tokens, const int *parents, const int *nodes,
                                                                 const int *want, int n, int *path, int *accepted, int *token) {
@@ -280,7 +282,8 @@ template <> __device__ __forceinline__ float tp_f(__nv_bfloat16 v) { return __bf
 // twice (as F32 values in shared memory they take 47 us instead of 30).
 // Bound by the memory, with eight CTAs of 128 threads and at most 28 KB an SM,
 // some of them reading while others sum or write. 512 rows of 50257 logits,
-// reads and writes together: BF16 30 us, 5.2 TB/s; F32 43 us, 4.8 TB/s. Twice
+// reads and writes together, in a graph on the same inputs: BF16 30 us, 5.2 TB/s;
+// F32 43 us, 4.8 TB/s (BF16 on changing inputs 33.5 us, 4.6 TB/s). Twice
 // the threads take 32 and 52 us (the fixed work of a thread: exchanges and
 // ends), slices of 14 KB 35 us and 58 us, of 56 KB 34 and 45 us. 9 rows of
 // 129280 F32 logits, mostly launch and exchange, take 6.0 us.
@@ -431,8 +434,9 @@ __global__ void __launch_bounds__(TP_THREADS, 8) token_probs_kernel(const T *log
 
 // A CTA per tensor, layer and sequence (and share of its rows): 16 bytes a
 // thread at a time, four reads before the writes. Bound by the memory, and by
-// the launch where little moves: 2.7 us for one sequence's rows in 12 layers,
-// 11.7 us for 16 sequences of 16 nodes (13 us with one read a thread).
+// the launch where little moves: 2.6 us for one sequence's rows in 12 layers,
+// 11.8 us for 16 sequences of 6 to 43 rows (13 us with one read a thread), in a
+// graph on the same rows; 5 and 14.3 us on changing ones.
 constexpr int CM_THREADS = 256;
 __global__ void __launch_bounds__(CM_THREADS) tree_commit_kernel(const __grid_constant__ ds_cuda_tree_commit_t d) {
     __shared__ int from[SV_MAX_NODES];
