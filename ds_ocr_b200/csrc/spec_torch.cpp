@@ -157,7 +157,8 @@ PyObject *tree_attention(PyObject *const *x, Py_ssize_t n_args) {
         c.strides(t, st, 3);
         if (!p.lo) return;
         const at::Tensor &u = c.strided(name, p.lo, s, rows);
-        if (u.strides() != t.strides()) throw Bad(std::string(name) + ": the planes must have the same strides");
+        for (int i = 0; i < 3; i++)  // (the stride of a dimension of one element is never used)
+            if (t.size(i) > 1 && u.stride(i) != t.stride(i)) throw Bad(std::string(name) + ": the planes must have the same strides");
         lo = u.data_ptr();
     };
     side("k", k, cache, d.k, d.k_lo, d.k_stride);

@@ -449,6 +449,23 @@ def test_attention_clamps_lengths_and_counts(spec):
     assert not c.run(spec).any()
 
 
+def test_attention_planes_whose_unused_strides_differ(spec):
+    # one sequence, one KV head: those dimensions' strides mean nothing
+    c = Case("pair", [30], [4], 4, 1, 2, 64, seed=31)
+    want = c.run(spec)
+
+    def odd(planes):
+        hi, lo = planes
+        return hi, lo.as_strided(lo.shape, (7, 13, *lo.stride()[2:]))
+
+    c.k, c.v, c.tk, c.tv = map(odd, (c.k, c.v, c.tk, c.tv))
+    assert torch.equal(c.run(spec), want)
+    c = Case("pair", [30], [4], 4, 2, 2, 64, seed=31)
+    c.k = c.k[0], c.k[1].as_strided(c.k[1].shape, (1, 64, 128, 1))  # the heads side by side
+    with pytest.raises(ValueError, match="strides"):
+        c.run(spec)
+
+
 def test_attention_refusals(spec):
     c = Case("bf16", [30], [4], 4, 2, 2, 64, seed=18)
     ok = (c.q, c.k, c.v, c.tk, c.tv, c.lens, c.mask)
